@@ -1,0 +1,420 @@
+// acc[m, n] = sum_k A(m, k) B(n, k) of bf16 or fp16 matrices, on CTA pairs, with the epilogues of a head's cross entropy.
+//
+// A persistent kernel of clusters of two CTAs, one CTA per SM; a pair takes 256 x 256 tiles one after another:
+//   warp 0, one lane : TMA producer - this CTA's 128 rows of A and its 128 of the tile's 256 rows of B, 64 of K, per stage of 32 KB
+//   warp 1, one lane : MMA issuer (leader CTA) - M 256 x N 256 x K 16, cta_group::2
+//   warps 2..9       : epilogue - each a quarter of the CTA's 128 rows and half of the columns
+// The accumulator takes 256 of TMEM's 512 columns, so that the epilogue of a tile runs beside the products of the next.
+// Operands whose M or N runs along memory's rows go in as they lie (kUmmaMnMajorA, kUmmaMnMajorB): the gradients' products
+// read the logits' gradient in both directions, and no matrix is transposed.
+//
+// The accumulator is drained once, after the whole of K.  The tensor core truncates as it adds, 2^-24 of the running sum per 16 of K on
+// average: at most 3e-5 of a logit's own size at K = 8192, and 5e-4 of a gradient's over 128256 words, a quarter of what its
+// rounding to bf16 costs.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <stdexcept>
+#include <string>
+#include <type_traits>
+
+#include "gemm16.h"
+#include "launch_util.h"
+#include "ptx.cuh"
+#include "tensor_map.h"
+
+namespace soapb200 {
+namespace {
+
+constexpr int kTile = 256;                       // of the pair, both ways
+constexpr int kRows = 128;                       // of a CTA, of either operand
+constexpr int kBK = 64;                          // one 128-byte swizzle row of K-major operands
+constexpr int kOperandBytes = kRows * kBK * 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 6;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kWarpStaging = 32 * 128;           // 32 rows of 128 bytes
+constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kWarpStaging + 1024 + 256;
+constexpr int kWarpColumns = kTile / 2;          // of the tile, per epilogue thread
+static_assert(kWarpColumns == kLogitPart, "an epilogue thread's columns are one part of its row");
+constexpr int kGroup = 8;                        // tile rows that share their tiles of B in L2 while they sweep the columns
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));      // off by 2^-22 at most
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float low, float high) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+struct Tiles {
+  int m, n, per_group;
+  __device__ __forceinline__ Tiles(int M, int N) : m((M + kTile - 1) / kTile), n((N + kTile - 1) / kTile), per_group(kGroup * n) {}
+  __device__ __forceinline__ int count() const { return m * n; }
+  __device__ __forceinline__ void place(int index, int& m0, int& n0) const {
+    const int first = index / per_group * kGroup;
+    const int rows = min(kGroup, m - first);
+    const int within = index % per_group;
+    m0 = (first + within % rows) * kTile;
+    n0 = within / rows * kTile;
+  }
+};
+
+// 32 rows of 128 bytes, one per lane, to 32 rows of a matrix: staged in shared memory (16-byte words swizzled by row, so that
+// neither side has bank conflicts) and stored with whole 128-byte lines.  `valid` bytes of each row are inside the matrix.
+__device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&words)[32], uint8_t* first, int64_t pitch, int rows,
+                                            int valid, int element, bool wide, int lane) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(staging + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2], words[4 * c + 3]);
+  __syncwarp();
+  const int chunk = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 4 * i + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(staging + row * 128 + ((chunk ^ (row & 7)) << 4));
+    if (row < rows) {
+      uint8_t* dst = first + row * pitch + chunk * 16;
+      const int left = valid - chunk * 16;
+      if (wide && left >= 16) {
+        *reinterpret_cast<uint4*>(dst) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (element == 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (4 * e < left) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (2 * e < left) reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// An epilogue thread's row of the tile: `taddr` is the first of its 128 columns.
+template <int EPI, typename T>
+__device__ __forceinline__ void epilogue_row(const Gemm16Problem& p, uint32_t taddr, int m_warp, int n0, uint8_t* staging, int lane) {
+  const int row = m_warp + lane;
+  const bool inside = row < p.M;
+  const int cols = min(kWarpColumns, p.N - n0);           // of this thread's part; may be negative
+  if constexpr (EPI == kLogitStatistics) {
+    const int64_t target = inside ? p.targets[row] - p.first_word - n0 : -1;
+    float largest = -INFINITY, sum = 0.f, picked = 0.f;
+#pragma unroll
+    for (int c = 0; c < kWarpColumns; c += 32) {
+      uint32_t raw[32];
+      tmem_ld_32x32(taddr + c, raw);
+      tmem_ld_wait();
+      if (c + 32 > cols) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j >= cols) raw[j] = __float_as_uint(-INFINITY);
+      }
+      float most = __uint_as_float(raw[0]);
+#pragma unroll
+      for (int j = 1; j < 32; ++j) most = fmaxf(most, __uint_as_float(raw[j]));
+      most = fmaxf(most, largest);
+      // (a row of no finite logit is taken relative to zero, so that its sum is zero, or NaN where a logit is)
+      const float base = most == -INFINITY ? 0.f : most * kLog2e;
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) part += exp2_fast(fmaf(__uint_as_float(raw[j]), kLog2e, -base));
+      sum = fmaf(sum, exp2_fast(fmaf(largest, kLog2e, -base)), part);
+      largest = most;
+      if (target >= c && target < c + 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (target == c + j) picked = __uint_as_float(raw[j]);
+      }
+    }
+    if (inside && cols > 0) {
+      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.M + row] = make_float2(largest, sum);
+      if (target >= 0 && target < cols) p.picked[row] = picked;
+    }
+  } else if constexpr (EPI == kLogitGradient) {
+    const int64_t target = inside ? p.targets[row] - p.first_word - n0 : -1;
+    const float base = inside ? p.lse[row] * kLog2e : 0.f, factor = inside ? p.factor[row] : 0.f;
+    const int rows = min(32, p.M - m_warp);
+#pragma unroll
+    for (int c = 0; c < kWarpColumns; c += 64) {
+      uint32_t words[32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t raw[32];
+        tmem_ld_32x32(taddr + c + 32 * h, raw);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float p_j = exp2_fast(fmaf(__uint_as_float(raw[j]), kLog2e, -base));
+          raw[j] = __float_as_uint((target == c + 32 * h + j ? p_j - 1.f : p_j) * factor);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) words[16 * h + j] = pack16<T>(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
+      }
+      if (rows > 0 && c < cols)
+        store_lines(staging, words, reinterpret_cast<uint8_t*>(p.C) + (m_warp * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
+                    2 * min(64, cols - c), 2, true, lane);
+    }
+  } else {
+    const int rows = min(32, p.M - m_warp);
+    const float alpha = p.alpha ? *p.alpha : 1.f;
+    const bool to16 = p.C != nullptr;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.C) & 15) == 0 && (p.ldc & 7) == 0;
+#pragma unroll
+    for (int c = 0; c < kWarpColumns; c += 64) {
+      uint32_t words[32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t raw[32];
+        const int at = c + 32 * h;
+        tmem_ld_32x32(taddr + at, raw);
+        tmem_ld_wait();
+        if (p.add && inside && at < cols) {
+          const float* old = p.accumulator + row * p.ld_accumulator + n0 + at;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {               // (the accumulator's pitch is a multiple of 32)
+            const float4 v = *reinterpret_cast<const float4*>(old + j);
+            raw[j] = __float_as_uint(__uint_as_float(raw[j]) + v.x);
+            raw[j + 1] = __float_as_uint(__uint_as_float(raw[j + 1]) + v.y);
+            raw[j + 2] = __float_as_uint(__uint_as_float(raw[j + 2]) + v.z);
+            raw[j + 3] = __float_as_uint(__uint_as_float(raw[j + 3]) + v.w);
+          }
+        }
+        if (to16) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            words[16 * h + j] = pack16<T>(alpha * __uint_as_float(raw[2 * j]), alpha * __uint_as_float(raw[2 * j + 1]));
+        } else if (rows > 0 && at < cols) {
+          store_lines(staging, raw, reinterpret_cast<uint8_t*>(p.accumulator + m_warp * p.ld_accumulator + n0 + at),
+                      p.ld_accumulator * 4, rows, 128, 4, true, lane);
+        }
+      }
+      if (to16 && rows > 0 && c < cols)
+        store_lines(staging, words, reinterpret_cast<uint8_t*>(p.C) + (m_warp * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
+                    2 * min(64, cols - c), 2, wide, lane);
+    }
+  }
+}
+
+template <int EPI, bool A_K, bool B_K, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+              const __grid_constant__ Gemm16Problem prob, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = smem + kStages * kStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kWarpStaging);      // used in the leader CTA only
+  uint64_t* empty_bar = full_bar + kStages;         // each CTA its own: "my stage may be refilled"
+  uint64_t* acc_full = empty_bar + kStages;         // [2] each CTA its own: tensor core -> epilogue
+  uint64_t* acc_empty = acc_full + 2;               // [2] leader's only: epilogue warps of both CTAs -> tensor core
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int cta = static_cast<int>(cluster_cta_rank());
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_descriptor(&map_a);
+    tma_prefetch_descriptor(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * kTile);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();      // both CTAs' barriers exist before anything arrives on them remotely
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  wait_for_predecessor();
+  let_successor_start();
+
+  const Tiles tiles(prob.M, prob.N);
+  const int k_blocks = (prob.K + kBK - 1) / kBK;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer (each CTA its own rows; the bytes are credited to the leader) ----------------
+    int s = 0;
+    uint32_t parity = 1;
+    bool first_round = true, ok = true;
+    for (int t = cluster; t < tiles.count() && ok; t += clusters) {
+      int m0, n0;
+      tiles.place(t, m0, n0);
+      m0 += cta * kRows;
+      n0 += cta * kRows;
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!first_round && !mbar_wait_bounded(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) {
+          ok = false;
+          break;
+        }
+        uint8_t* stage = smem + s * kStageBytes;
+        if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
+        const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
+        if constexpr (A_K) {
+          tma_load_2d_pair(stage, &map_a, bar, kb * kBK, m0);
+        } else {
+          tma_load_2d_pair(stage, &map_a, bar, m0, kb * kBK);
+          tma_load_2d_pair(stage + kOperandBytes / 2, &map_a, bar, m0 + 64, kb * kBK);
+        }
+        if constexpr (B_K) {
+          tma_load_2d_pair(stage + kOperandBytes, &map_b, bar, kb * kBK, n0);
+        } else {
+          tma_load_2d_pair(stage + kOperandBytes, &map_b, bar, n0, kb * kBK);
+          tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, &map_b, bar, n0 + 64, kb * kBK);
+        }
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+          first_round = false;
+        }
+      }
+    }
+    if (*abort_flag) {
+      // give copies that are still in flight time to land before the CTA's shared memory is released
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1 && lane == 0 && cta == 0) {
+    // ---------------- MMA issuer ----------------
+    constexpr uint32_t kIdesc = (std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kTile, kTile) : umma_idesc_fp16(kTile, kTile)) |
+                                (A_K ? 0u : kUmmaMnMajorA) | (B_K ? 0u : kUmmaMnMajorB);
+    constexpr uint64_t kStepA = A_K ? 32 >> 4 : 2048 >> 4, kStepB = B_K ? 32 >> 4 : 2048 >> 4;      // 16 of K
+    int s = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    int it = 0;
+    for (int t = cluster; t < tiles.count() && ok; t += clusters, ++it) {
+      const int buf = it & 1;
+      if (it >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) break;
+      tc_fence_after_sync();
+      const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t stage = smem_u32(smem + s * kStageBytes);
+        const uint64_t a = A_K ? umma_desc_kmajor<128>(stage) : umma_desc_mn_major(stage);
+        const uint64_t b = B_K ? umma_desc_kmajor<128>(stage + kOperandBytes) : umma_desc_mn_major(stage + kOperandBytes);
+#pragma unroll
+        for (int k = 0; k < kBK / 16; ++k) umma_f16_ss_pair(acc, a + k * kStepA, b + k * kStepB, kIdesc, kb | k ? 1u : 0u);
+        umma_commit_pair(&empty_bar[s]);
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+        }
+      }
+      if (ok) umma_commit_pair(&acc_full[buf]);
+    }
+  } else if (warp >= 2) {
+    // ---------------- epilogue (each CTA its own 128 rows) ----------------
+    const int ew = warp - 2;
+    const int quarter = warp & 3;              // TMEM lane quarter this warp may read
+    const int col0 = (ew >> 2) * kWarpColumns;
+    const uint32_t drained = map_to_cta(smem_u32(&acc_empty[0]), 0);
+    int it = 0;
+    for (int t = cluster; t < tiles.count(); t += clusters, ++it) {
+      const int buf = it & 1;
+      int m0, n0;
+      tiles.place(t, m0, n0);
+      if (!mbar_wait_bounded(&acc_full[buf], (it >> 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) break;
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buf * kTile + col0);
+      epilogue_row<EPI, T>(prob, taddr, m0 + cta * kRows + quarter * 32, n0 + col0, staging + ew * kWarpStaging, lane);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(drained + static_cast<uint32_t>(buf * sizeof(uint64_t)));
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();      // nobody leaves while the other CTA may still touch its shared memory or TMEM
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 2 * kTile);
+  }
+}
+
+CUtensorMap map_of(bool bf16, const Matrix16& x, int64_t rows, int64_t K) {
+  const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return x.k_major ? encode_k_major(type, x.data, K, rows, 2 * x.ld, kBK, kRows, CU_TENSOR_MAP_SWIZZLE_128B)
+                   : encode_k_major(type, x.data, rows, K, 2 * x.ld, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int pairs_of_device() {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    throw std::runtime_error("gemm16: no device");
+  return sms / 2;
+}
+
+template <int EPI, bool A_K, bool B_K, typename T>
+void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream) {
+  static PerDeviceOnce configured;
+  allow_dynamic_smem(reinterpret_cast<const void*>(gemm16_kernel<EPI, A_K, B_K, T>), kSmemBytes, configured, "gemm16");
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  const CUtensorMap map_a = map_of(kBf16, a, p.M, p.K), map_b = map_of(kBf16, b, p.N, p.K);
+  const int64_t tiles = static_cast<int64_t>((p.M + kTile - 1) / kTile) * ((p.N + kTile - 1) / kTile);
+  if (tiles > (1 << 30)) throw std::invalid_argument("gemm16: too many tiles");
+  const int clusters = static_cast<int>(tiles < pairs_of_device() ? tiles : pairs_of_device());
+  cudaError_t err = launch_dependent(gemm16_kernel<EPI, A_K, B_K, T>, dim3(2 * clusters), dim3(kThreads), kSmemBytes, stream, map_a,
+                                     map_b, p, status);
+  if (err != cudaSuccess) throw std::runtime_error(std::string("gemm16 launch: ") + cudaGetErrorString(err));
+}
+
+template <typename T>
+void dispatch(Gemm16Epilogue epilogue, const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream) {
+  if (epilogue == kLogitStatistics && a.k_major && b.k_major) launch<kLogitStatistics, true, true, T>(a, b, p, status, stream);
+  else if (epilogue == kLogitGradient && a.k_major && b.k_major) launch<kLogitGradient, true, true, T>(a, b, p, status, stream);
+  else if (epilogue == kStore16 && a.k_major && !b.k_major) launch<kStore16, true, false, T>(a, b, p, status, stream);
+  else if (epilogue == kStore16 && !a.k_major && !b.k_major) launch<kStore16, false, false, T>(a, b, p, status, stream);
+  else throw std::invalid_argument("gemm16: no kernel for these orders of the operands");
+}
+
+}  // namespace
+
+void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status,
+            cudaStream_t stream) {
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0) throw std::invalid_argument("gemm16: empty product");
+  if (a.ld % 8 != 0 || b.ld % 8 != 0) throw std::invalid_argument("gemm16: operand pitches are multiples of 8 elements");
+  if (epilogue == kLogitGradient && (p.ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(p.C) & 15) != 0))
+    throw std::invalid_argument("gemm16: the logits' gradient needs 16-byte rows");
+  if (epilogue == kStore16 && (p.add || !p.C) && (!p.accumulator || p.ld_accumulator % 32 != 0 || p.ld_accumulator < p.N ||
+                                                  (reinterpret_cast<uintptr_t>(p.accumulator) & 15) != 0))
+    throw std::invalid_argument("gemm16: the accumulator's pitch is a multiple of 32 covering the columns");
+  if (bf16) dispatch<__nv_bfloat16>(epilogue, a, b, p, status, stream);
+  else dispatch<__half>(epilogue, a, b, p, status, stream);
+}
+
+}  // namespace soapb200

@@ -134,6 +134,19 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
+// The same with 32 columns.
+__device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Two fp32 values in one register pair, added and multiplied by one instruction, each rounded as fmaf and + round it.
@@ -171,6 +184,17 @@ __device__ __forceinline__ uint64_t umma_desc_kmajor(uint32_t smem_addr) {
   desc |= static_cast<uint64_t>((8 * RowBytes) >> 4) << 32;
   desc |= static_cast<uint64_t>(1) << 46;
   desc |= static_cast<uint64_t>(RowBytes == 128 ? 2 : (RowBytes == 64 ? 4 : 6)) << 61;   // SWIZZLE_128B / 64B / 32B
+  return desc;
+}
+// Operand tile of 16-bit elements whose M (or N) runs along the 128-byte swizzle rows, as a TMA box of 64 elements x 64 of K
+// writes it: 64 elements of M per row, rows of K 128 B apart, groups of eight of K 1024 B apart (the stride offset), the next 64
+// of M in the next box, 8192 B on (the leading offset).
+__device__ __forceinline__ uint64_t umma_desc_mn_major(uint32_t smem_addr) {
+  uint64_t desc = static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  desc |= static_cast<uint64_t>(8192 >> 4) << 16;
+  desc |= static_cast<uint64_t>(1024 >> 4) << 32;
+  desc |= static_cast<uint64_t>(1) << 46;
+  desc |= static_cast<uint64_t>(2) << 61;   // SWIZZLE_128B
   return desc;
 }
 // kind::tf32, fp32 accumulator, both operands K-major, no negation, dense.
@@ -259,5 +283,8 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
+
+// Instruction descriptor bits of operands that are M-major (A) or N-major (B) in shared memory.
+constexpr uint32_t kUmmaMnMajorA = 1u << 15, kUmmaMnMajorB = 1u << 16;
 
 }  // namespace soapb200
