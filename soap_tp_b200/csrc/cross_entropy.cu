@@ -3,20 +3,30 @@
 //   l_ij = h_i . w_j     lse_i = log sum_j exp l_ij     loss_i = lse_i - l_i,t_i
 //   d_ij = f_i (exp(l_ij - lse_i) - [j = t_i])          dH = alpha D W      dW = alpha D^T H
 //
-// Forward: one product (gemm16.cu) whose epilogue leaves, per token and 128 words, the largest logit and the sum of
-// exponentials relative to it; head_join_kernel joins these parts.  Backward: the logits once more, this time leaving D in 16 bits
-// for a bounded number of tokens at a time, then the two products that read D in both directions.
+// Tokens that do not count are left out from the start: the others' numbers, targets and hidden states are put one after another, every
+// product runs over those alone (their number stays on the device), and what the padding holds, NaN included, reaches nothing.
+//
+// The loss: one product (gemm16.cu) whose epilogue leaves, per token and 128 words, the largest logit and the sum of
+// exponentials relative to it; head_join_kernel joins these parts.  D goes through memory in 16 bits for a bounded number of tokens at a time, then
+// two products read it in both directions.  It comes about in one of two ways:
+//   * bf16 and one gradient of the loss for all tokens (mean, sum): the first product leaves the exponentials as well, one pass over them
+//     makes D of them once lse is known, and the gradients come with the loss, 6 N V K operations for N tokens.  The pass
+//     moves 4 N V bytes: 0.7 of 21 ms at 8192 x 4096 x 128256, where the product that it replaces takes 5.
+//   * fp16, whose gradients want the loss's scale before they are rounded, a gradient for each token, or a second backward pass: the logits
+//     are computed again once these are known, 8 N V K operations.
 //
 // What multiplies a row is split into a factor in [-1, 1] that goes into D and a number on the device that the products' epilogues
 // multiply by: mean's 1 / count never touches D, where -1 (the target of a token that the model does not know) is exact, and
 // fp16 keeps probabilities down to 2^-29 as normal numbers (D is stored times 2^15 there).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 
 #include "cross_entropy.h"
 #include "launch_util.h"
+#include "value16.cuh"
 
 namespace soapb200 {
 namespace {
@@ -29,109 +39,150 @@ void check(cudaError_t err, const char* what) {
   if (err != cudaSuccess) throw std::runtime_error(std::string(what) + " launch: " + cudaGetErrorString(err));
 }
 
-// 32 tokens a block, lanes along tokens, the parts dealt to 16 warps and joined in a fixed order.
-__global__ void __launch_bounds__(32 * kJoinSlices)
-head_join_kernel(const float2* __restrict__ parts, int count, int tokens, const int64_t* __restrict__ targets, int64_t first_word, int words,
-                 float* __restrict__ lse, float* __restrict__ picked) {
-  __shared__ float2 shared[kJoinSlices][32];
-  wait_for_predecessor();
-  let_successor_start();
-  const int token = blockIdx.x * 32 + threadIdx.x;
-  float largest = -INFINITY, sum = 0.f;
-  if (token < tokens) {
-#pragma unroll 4
-    for (int i = threadIdx.y; i < count; i += kJoinSlices) {
-      const float2 part = parts[static_cast<int64_t>(i) * tokens + token];
-      const float most = fmaxf(largest, part.x);
-      const float base = most == -INFINITY ? 0.f : most;
-      sum = sum * exp2f((largest - base) * kLog2e) + part.y * exp2f((part.x - base) * kLog2e);
-      largest = most;
-    }
-  }
-  shared[threadIdx.y][threadIdx.x] = make_float2(largest, sum);
-  __syncthreads();
-  if (threadIdx.y == 0 && token < tokens) {
-#pragma unroll
-    for (int s = 1; s < kJoinSlices; ++s) {
-      const float2 part = shared[s][threadIdx.x];
-      const float most = fmaxf(largest, part.x);
-      const float base = most == -INFINITY ? 0.f : most;
-      sum = sum * exp2f((largest - base) * kLog2e) + part.y * exp2f((part.x - base) * kLog2e);
-      largest = most;
-    }
-    lse[token] = logf(sum) + (largest == -INFINITY ? 0.f : largest);
-    const int64_t target = targets[token] - first_word;
-    if (target < 0 || target >= words) picked[token] = 0.f;
-  }
-}
-
-struct Targets {
-  const int64_t* at;
-  int64_t ignored, vocabulary;
-  __device__ __forceinline__ bool counts(int i) const { return at[i] != ignored; }
-  __device__ __forceinline__ bool known(int i) const { return at[i] >= 0 && at[i] < vocabulary; }
-};
-
-__global__ void head_token_losses_kernel(Targets targets, int tokens, const float* __restrict__ lse, const float* __restrict__ picked,
-                                         float* __restrict__ losses) {
-  wait_for_predecessor();
-  let_successor_start();
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < tokens) losses[i] = !targets.counts(i) ? 0.f : targets.known(i) ? lse[i] - picked[i] : nanf("");
-}
-
 template <typename V, typename Op>
 __device__ __forceinline__ V block_reduce(V v, Op op, V* shared) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    v = shared[threadIdx.x];
+  v = shared[threadIdx.x & 31];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (threadIdx.x == 0) shared[0] = v;
-  }
-  __syncthreads();
-  v = shared[0];
+  for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   __syncthreads();
   return v;
 }
 
-// One block: the sum does not depend on the order in which blocks end.
+// One block: a thread takes a run of neighbouring tokens, counts, learns how many come before, and writes.
 __global__ void __launch_bounds__(kSingleThreads)
-head_reduced_loss_kernel(Targets targets, int tokens, const float* __restrict__ lse, const float* __restrict__ picked, bool mean,
-                         float* __restrict__ loss, float* __restrict__ counted) {
-  __shared__ double shared[32];
+head_count_kernel(const int64_t* __restrict__ targets, int tokens, int64_t ignored, int64_t first_word, int words, int64_t vocabulary,
+                  int* __restrict__ count, int* __restrict__ where, int* __restrict__ column) {
+  __shared__ int warps[32];
   wait_for_predecessor();
   let_successor_start();
-  double sum = 0.0, count = 0.0;
-  for (int i = threadIdx.x; i < tokens; i += kSingleThreads) {
-    if (targets.counts(i)) {
-      count += 1.0;
-      sum += targets.known(i) ? lse[i] - picked[i] : nanf("");
-    }
+  const int each = (tokens + kSingleThreads - 1) / kSingleThreads;
+  const int begin = min(tokens, static_cast<int>(threadIdx.x) * each), end = min(tokens, begin + each);
+  int mine = 0;
+  for (int i = begin; i < end; ++i) mine += targets[i] != ignored;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += other;
   }
-  auto add = [](double a, double b) { return a + b; };
-  sum = block_reduce(sum, add, shared);
-  count = block_reduce(count, add, shared);
-  if (threadIdx.x == 0) {
-    *loss = static_cast<float>(mean ? (count > 0.0 ? sum / count : 0.0) : sum);
-    *counted = static_cast<float>(count);
+  if (lane == 31) warps[warp] = before;
+  __syncthreads();
+  if (warp == 0) {
+    int sum = warps[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += other;
+    }
+    warps[lane] = sum;
+  }
+  __syncthreads();
+  int at = before - mine + (warp ? warps[warp - 1] : 0);
+  for (int i = begin; i < end; ++i) {
+    const int64_t target = targets[i];
+    if (target == ignored) continue;
+    const int64_t here = target - first_word;
+    where[at] = i;
+    column[at++] = target < 0 || target >= vocabulary ? kUnknown : here < 0 || here >= words ? kElsewhere : static_cast<int>(here);
+  }
+  if (threadIdx.x == 0) *count = warps[31];
+}
+
+// Where not every token counts: the hidden states of those that do, one after another, zeros up to the next multiple of 64, and
+// zeros in the gradients of the others.  A warp takes a row.
+__global__ void head_gather_kernel(const uint16_t* __restrict__ hidden, int64_t ld, int tokens, int depth, const int64_t* __restrict__ targets, int64_t ignored,
+                                   const int* __restrict__ count, const int* __restrict__ where, uint16_t* __restrict__ packed, int64_t ld_packed,
+                                   uint16_t* __restrict__ d_hidden, int64_t ld_d) {
+  wait_for_predecessor();
+  let_successor_start();
+  const int counted = *count;
+  if (counted == tokens) return;
+  const int lane = threadIdx.x & 31;
+  const int rows_to_fill = min(tokens, (counted + 63) / 64 * 64);
+  for (int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); row < tokens; row += gridDim.x * (blockDim.x >> 5)) {
+    if (row < rows_to_fill) {
+      const uint16_t* from = row < counted ? hidden + where[row] * ld : nullptr;
+      uint16_t* to = packed + row * ld_packed;
+      for (int i = lane; i < depth / 8; i += 32)      // (both pitches are multiples of 8)
+        reinterpret_cast<uint4*>(to)[i] = from ? reinterpret_cast<const uint4*>(from)[i] : make_uint4(0, 0, 0, 0);
+      for (int i = depth / 8 * 8 + lane; i < depth; i += 32) to[i] = from ? from[i] : 0;
+    }
+    if (d_hidden && targets[row] == ignored)
+      for (int i = lane; i < depth; i += 32) d_hidden[row * ld_d + i] = 0;
   }
 }
 
+// 32 tokens a block, lanes along tokens, the parts dealt to 16 warps and joined in a fixed order.
+__global__ void __launch_bounds__(32 * kJoinSlices)
+head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number, const int* __restrict__ count, int first, int rows,
+                 const int* __restrict__ column, float* __restrict__ lse, float* __restrict__ picked) {
+  __shared__ float2 shared[kJoinSlices][32];
+  wait_for_predecessor();
+  let_successor_start();
+  const int token = blockIdx.x * 32 + threadIdx.x;
+  const bool here = token < min(rows, *count - first);
+  float largest = -INFINITY, sum = 0.f;
+  auto join = [&](const float2 part) {
+    const float most = fmaxf(largest, part.x);
+    const float base = most == -INFINITY ? 0.f : most;
+    sum = sum * exp2f((largest - base) * kLog2e) + part.y * exp2f((part.x - base) * kLog2e);
+    largest = most;
+  };
+  if (here) {
+#pragma unroll 4
+    for (int i = threadIdx.y; i < number; i += kJoinSlices) join(parts[i * ld_parts + token]);
+  }
+  shared[threadIdx.y][threadIdx.x] = make_float2(largest, sum);
+  __syncthreads();
+  if (threadIdx.y == 0 && here) {
+#pragma unroll
+    for (int s = 1; s < kJoinSlices; ++s) join(shared[s][threadIdx.x]);
+    lse[first + token] = logf(sum) + (largest == -INFINITY ? 0.f : largest);
+    if (column[first + token] < 0) picked[first + token] = 0.f;
+  }
+}
+
+__device__ __forceinline__ float token_loss(int column, float lse, float picked) { return column == kUnknown ? nanf("") : lse - picked; }
+
+// (the losses of tokens that do not count are cleared first)
+__global__ void head_token_losses_kernel(const int* __restrict__ count, const int* __restrict__ where, const int* __restrict__ column,
+                                         const float* __restrict__ lse, const float* __restrict__ picked, float* __restrict__ losses) {
+  wait_for_predecessor();
+  let_successor_start();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < *count) losses[where[i]] = token_loss(column[i], lse[i], picked[i]);
+}
+
+// One block: the sum does not depend on the order in which blocks end.
 __global__ void __launch_bounds__(kSingleThreads)
-head_factors_kernel(Targets targets, int tokens, int reduction, float stored, const float* __restrict__ grad_loss,
-                    const float* __restrict__ counted, float* __restrict__ factor, float* __restrict__ alpha) {
+head_reduced_loss_kernel(const int* __restrict__ count, const int* __restrict__ column, const float* __restrict__ lse,
+                         const float* __restrict__ picked, bool mean, float* __restrict__ loss) {
+  __shared__ double shared[32];
+  wait_for_predecessor();
+  let_successor_start();
+  const int counted = *count;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < counted; i += kSingleThreads) sum += token_loss(column[i], lse[i], picked[i]);
+  sum = block_reduce(sum, [](double a, double b) { return a + b; }, shared);
+  if (threadIdx.x == 0) *loss = static_cast<float>(mean && counted ? sum / counted : sum);
+}
+
+__global__ void __launch_bounds__(kSingleThreads)
+head_factors_kernel(const int* __restrict__ count, const int* __restrict__ where, const int* __restrict__ column, int reduction, float stored,
+                    const float* __restrict__ grad_loss, float* __restrict__ factor, float* __restrict__ alpha) {
   __shared__ float shared[32];
   wait_for_predecessor();
   let_successor_start();
+  const int counted = *count;
   float common = 1.f, relative = 1.f;      // the gradient is common * factor; factor = stored * relative * (the row's own)
   if (reduction == kLossNone) {
     float most = 0.f;
-    for (int i = threadIdx.x; i < tokens; i += kSingleThreads)
-      if (targets.counts(i)) most = fmaxf(most, fabsf(grad_loss[i]));
+    for (int i = threadIdx.x; i < counted; i += kSingleThreads) most = fmaxf(most, fabsf(grad_loss[where[i]]));
     most = block_reduce(most, [](float a, float b) { return fmaxf(a, b); }, shared);
     // a power of two, so that no factor is rounded; none where the largest is zero or not finite
     if (most > 0.f && most < INFINITY) {
@@ -140,81 +191,209 @@ head_factors_kernel(Targets targets, int tokens, int reduction, float stored, co
       relative = ldexpf(1.f, -exponent);
     }
   } else {
-    common = *grad_loss;
-    if (reduction == kLossMean) common = *counted > 0.f ? common / *counted : 0.f;
+    if (grad_loss) common = *grad_loss;
+    if (reduction == kLossMean) common = counted ? common / static_cast<float>(counted) : 0.f;
   }
-  for (int i = threadIdx.x; i < tokens; i += kSingleThreads) {
-    const float own = reduction == kLossNone ? grad_loss[i] : 1.f;
-    factor[i] = !targets.counts(i) ? 0.f : targets.known(i) ? stored * relative * own : nanf("");
+  for (int i = threadIdx.x; i < counted; i += kSingleThreads) {
+    const float own = reduction == kLossNone ? grad_loss[where[i]] : 1.f;
+    factor[i] = column[i] == kUnknown ? nanf("") : stored * relative * own;
   }
   if (threadIdx.x == 0) *alpha = common / stored;
 }
 
-Targets targets_of(const HeadProblem& p) { return Targets{p.targets, p.ignore_index, p.vocabulary}; }
+// A row of exponentials, relative to the largest of their parts, becomes the row of D.  Rows up to the next multiple of 64 are cleared: they
+// are read as part of K.
+constexpr int kRescaleThreads = 256, kRescaleRuns = 4;
+__global__ void __launch_bounds__(kRescaleThreads)
+head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, const int* __restrict__ count, int first, int rows,
+                    const float2* __restrict__ parts, int64_t ld_parts, const int* __restrict__ column, const float* __restrict__ lse,
+                    const float* __restrict__ picked, const float* __restrict__ factor) {
+  wait_for_predecessor();
+  let_successor_start();
+  const int row = blockIdx.y;
+  const int counted = min(rows, *count - first);
+  if (row >= min(rows, (counted + 63) / 64 * 64)) return;
+  const bool here = row < counted;
+  const float l = here ? lse[first + row] : 0.f, f = here ? factor[first + row] : 0.f;
+  const int target = here ? column[first + row] : -1;
+  __nv_bfloat16* line = logits + row * ld;
+  const int run0 = blockIdx.x * kRescaleThreads * kRescaleRuns + threadIdx.x;
+  const int runs = (words + 7) / 8;        // (the pitch is a multiple of 8)
+  Eight<__nv_bfloat16> e[kRescaleRuns];
+  float largest[kRescaleRuns];
+#pragma unroll
+  for (int i = 0; i < kRescaleRuns; ++i) {
+    const int run = run0 + i * kRescaleThreads;
+    if (here && run < runs) {
+      e[i].load(line + 8 * run);
+      largest[i] = parts[(run / (kLogitPart / 8)) * ld_parts + row].x;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRescaleRuns; ++i) {
+    const int run = run0 + i * kRescaleThreads;
+    if (run >= runs) break;
+    if (here) {
+      float v[8];
+      e[i].get(v);
+      const float by = exp2f((largest[i] - l) * kLog2e) * f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= by;
+      if (target >= 8 * run && target < 8 * run + 8) {
+        // from the target's logit itself: its probability, less one, is small where the model knows the word
+        const float d = expm1f(picked[first + row] - l) * f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (target == 8 * run + j) v[j] = d;
+      }
+      e[i].set(v);
+    } else {
+      e[i].clear();
+    }
+    e[i].store(line + 8 * run);
+  }
+}
+
+constexpr int kScaleThreads = 256;
+__global__ void __launch_bounds__(kScaleThreads)
+scale_gradients_kernel(const float* __restrict__ factor, __nv_bfloat16* __restrict__ a, int64_t count_a, __nv_bfloat16* __restrict__ b, int64_t count_b) {
+  wait_for_predecessor();
+  let_successor_start();
+  const float f = *factor;
+  if (f == 1.f) return;
+  const int64_t runs_a = (count_a + 7) / 8, runs = runs_a + (count_b + 7) / 8;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kScaleThreads + threadIdx.x; i < runs; i += static_cast<int64_t>(gridDim.x) * kScaleThreads) {
+    __nv_bfloat16* at = i < runs_a ? a + 8 * i : b + 8 * (i - runs_a);
+    const int valid = static_cast<int>(min(static_cast<int64_t>(8), i < runs_a ? count_a - 8 * i : count_b - 8 * (i - runs_a)));
+    float v[8];
+    read_eight(at, valid, true, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+    write_eight(at, valid, true, v);
+  }
+}
+
+int sms_of_device() {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    throw std::runtime_error("cross entropy: no device");
+  return sms;
+}
+
+Hidden16 hidden_of(const HeadProblem& p, int first) {
+  const int64_t at = static_cast<int64_t>(first);
+  return Hidden16{Matrix16{static_cast<const uint16_t*>(p.packed.data) + at * p.packed.ld, p.packed.ld, true},
+                  Matrix16{static_cast<const uint16_t*>(p.hidden.data) + at * p.hidden.ld, p.hidden.ld, true}, p.tokens};
+}
+
+Gemm16Problem logits_of(const HeadProblem& p, const LogitRows& r) {
+  if (r.rows < 1 || r.first < 0 || r.first + r.rows > p.tokens) throw std::invalid_argument("cross entropy: rows outside the tokens");
+  Gemm16Problem g{};
+  g.M = r.rows; g.N = p.words; g.K = p.depth;
+  g.count = p.count; g.first = r.first;
+  g.targets = p.column + r.first;
+  g.parts = r.parts; g.ld_parts = r.rows;
+  g.C = r.logits; g.ldc = r.ld_logits;
+  return g;
+}
 
 }  // namespace
 
-void head_statistics(const HeadProblem& p, float2* parts, float* lse, float* picked, int* status, cudaStream_t stream) {
-  Gemm16Problem g{};
-  g.M = p.tokens; g.N = p.words; g.K = p.depth;
-  g.targets = p.targets; g.first_word = p.first_word;
-  g.parts = parts; g.picked = picked;
-  gemm16(kLogitStatistics, p.bf16, p.hidden, p.weight, g, status, stream);
-  check(launch_dependent(head_join_kernel, dim3((p.tokens + 31) / 32), dim3(32, kJoinSlices), 0, stream, parts,
-                         (p.words + kLogitPart - 1) / kLogitPart, p.tokens, p.targets, p.first_word, p.words, lse, picked),
+void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaStream_t stream) {
+  check(launch_dependent(head_count_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.targets, p.tokens, p.ignore_index, p.first_word,
+                         p.words, p.vocabulary, p.count, p.where, p.column),
+        "head_count");
+  const int blocks = std::min((p.tokens + 7) / 8, 8 * sms_of_device());
+  check(launch_dependent(head_gather_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<const uint16_t*>(p.hidden.data), p.hidden.ld,
+                         p.tokens, p.depth, p.targets, p.ignore_index, p.count, p.where,
+                         static_cast<uint16_t*>(const_cast<void*>(p.packed.data)), p.packed.ld, static_cast<uint16_t*>(d_hidden), ld_hidden),
+        "head_gather");
+}
+
+void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float* picked, int* status, cudaStream_t stream) {
+  Gemm16Problem g = logits_of(p, r);
+  g.picked = picked + r.first;
+  const Hidden16 hidden = hidden_of(p, r.first);
+  gemm16(r.logits ? kLogitExponential : kLogitStatistics, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
+  check(launch_dependent(head_join_kernel, dim3((r.rows + 31) / 32), dim3(32, kJoinSlices), 0, stream, r.parts,
+                         static_cast<int64_t>(r.rows), (p.words + kLogitPart - 1) / kLogitPart, p.count, r.first, r.rows, p.column, lse, picked),
         "head_join");
 }
 
-void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, float* counted,
-                 cudaStream_t stream) {
-  if (reduction == kLossNone)
-    check(launch_dependent(head_token_losses_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, targets_of(p), p.tokens, lse,
-                           picked, loss),
+void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, cudaStream_t stream) {
+  if (reduction == kLossNone) {
+    const cudaError_t err = cudaMemsetAsync(loss, 0, sizeof(float) * p.tokens, stream);
+    if (err != cudaSuccess) throw std::runtime_error(std::string("head_losses: ") + cudaGetErrorString(err));
+    check(launch_dependent(head_token_losses_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p.count, p.where, p.column, lse, picked, loss),
           "head_token_losses");
-  else
-    check(launch_dependent(head_reduced_loss_kernel, dim3(1), dim3(kSingleThreads), 0, stream, targets_of(p), p.tokens, lse, picked,
-                           reduction == kLossMean, loss, counted),
+  } else {
+    check(launch_dependent(head_reduced_loss_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.count, p.column, lse, picked,
+                           reduction == kLossMean, loss),
           "head_reduced_loss");
+  }
 }
 
-void head_factors(const HeadProblem& p, LossReduction reduction, const float* grad_loss, const float* counted, float* factor,
-                  float* alpha, cudaStream_t stream) {
-  check(launch_dependent(head_factors_kernel, dim3(1), dim3(kSingleThreads), 0, stream, targets_of(p), p.tokens,
-                         static_cast<int>(reduction), p.bf16 ? 1.f : 32768.f, grad_loss, counted, factor, alpha),
+void head_factors(const HeadProblem& p, LossReduction reduction, const float* grad_loss, float* factor, float* alpha, cudaStream_t stream) {
+  check(launch_dependent(head_factors_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.count, p.where, p.column,
+                         static_cast<int>(reduction), p.bf16 ? 1.f : 32768.f, grad_loss, factor, alpha),
         "head_factors");
 }
 
-void head_gradients(const HeadProblem& p, const float* lse, const float* factor, const float* alpha, const HeadGradients& out, int* status,
-                    cudaStream_t stream) {
-  if (out.rows < 1) throw std::invalid_argument("head_gradients: no room for logits");
-  if (out.weight && p.tokens > out.rows && !out.sum) throw std::invalid_argument("head_gradients: several turns need a sum");
-  for (int first = 0; first < p.tokens; first += out.rows) {
-    const int rows = p.tokens - first < out.rows ? p.tokens - first : out.rows;
-    const Matrix16 hidden{static_cast<const uint16_t*>(p.hidden.data) + first * p.hidden.ld, p.hidden.ld, true};
-    Gemm16Problem g{};
-    g.M = rows; g.N = p.words; g.K = p.depth;
-    g.targets = p.targets + first; g.first_word = p.first_word;
-    g.lse = lse + first; g.factor = factor + first;
-    g.C = out.logits; g.ldc = out.ld_logits;
-    gemm16(kLogitGradient, p.bf16, hidden, p.weight, g, status, stream);
-    if (out.hidden) {
-      Gemm16Problem d{};
-      d.M = rows; d.N = p.depth; d.K = p.words;
-      d.C = static_cast<uint16_t*>(out.hidden) + first * out.ld_hidden; d.ldc = out.ld_hidden;
-      d.alpha = alpha;
-      gemm16(kStore16, p.bf16, Matrix16{out.logits, out.ld_logits, true}, Matrix16{p.weight.data, p.weight.ld, false}, d, status, stream);
-    }
-    if (out.weight) {
-      Gemm16Problem d{};
-      d.M = p.words; d.N = p.depth; d.K = rows;
-      d.alpha = alpha;
-      d.accumulator = out.sum; d.ld_accumulator = out.ld_sum; d.add = first > 0;
-      if (first + rows == p.tokens) {
-        d.C = out.weight; d.ldc = out.ld_weight;
-      }
-      gemm16(kStore16, p.bf16, Matrix16{out.logits, out.ld_logits, false}, Matrix16{hidden.data, hidden.ld, false}, d, status, stream);
-    }
+void head_rescale(const HeadProblem& p, const LogitRows& r, const float* lse, const float* picked, const float* factor, cudaStream_t stream) {
+  const Gemm16Problem g = logits_of(p, r);
+  constexpr int kWords = 8 * kRescaleThreads * kRescaleRuns;
+  // (the grid's second extent is at most 65535)
+  for (int begin = 0; begin < r.rows; begin += 65472) {
+    const int rows = std::min(r.rows - begin, 65472);
+    check(launch_dependent(head_rescale_kernel, dim3((p.words + kWords - 1) / kWords, rows), dim3(kRescaleThreads), 0, stream,
+                           static_cast<__nv_bfloat16*>(g.C) + begin * g.ldc, g.ldc, p.words, p.count, r.first + begin, rows, r.parts + begin,
+                           g.ld_parts, p.column, lse, picked, factor),
+          "head_rescale");
   }
+}
+
+void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const float* lse, const float* factor, int* status, cudaStream_t stream) {
+  Gemm16Problem g = logits_of(p, r);
+  g.lse = lse + r.first; g.factor = factor + r.first;
+  const Hidden16 hidden = hidden_of(p, r.first);
+  gemm16(kLogitGradient, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
+}
+
+void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha, const HeadGradients& out, int* status, cudaStream_t stream) {
+  const bool last = r.first + r.rows == p.tokens;
+  if (out.weight && !(r.first == 0 && last) && !out.sum) throw std::invalid_argument("head_gradients: several turns need a sum");
+  if (out.hidden) {
+    Gemm16Problem d{};
+    d.M = r.rows; d.N = p.depth; d.K = p.words;
+    d.count = p.count; d.first = r.first;
+    d.C = out.hidden; d.ldc = out.ld_hidden; d.where = p.where + r.first;
+    d.alpha = alpha;
+    gemm16(kStore16, p.bf16, Matrix16{r.logits, r.ld_logits, true}, Matrix16{p.weight.data, p.weight.ld, false}, d, status, stream);
+  }
+  if (out.weight) {
+    Gemm16Problem d{};
+    d.M = p.words; d.N = p.depth; d.K = r.rows;
+    d.count = p.count; d.first = r.first;
+    d.alpha = alpha;
+    d.accumulator = out.sum; d.ld_accumulator = out.ld_sum; d.add = r.first > 0;
+    if (last) {
+      d.C = out.weight; d.ldc = out.ld_weight;
+    }
+    Hidden16 hidden = hidden_of(p, r.first);
+    hidden.packed.k_major = hidden.all.k_major = false;
+    gemm16(kStore16, p.bf16, Matrix16{r.logits, r.ld_logits, false}, hidden.packed, d, status, stream, &hidden);
+  }
+}
+
+void scale_gradients(const float* factor, void* a, int64_t count_a, void* b, int64_t count_b, cudaStream_t stream) {
+  if ((reinterpret_cast<uintptr_t>(a) & 15) != 0 || (reinterpret_cast<uintptr_t>(b) & 15) != 0)
+    throw std::invalid_argument("scale_gradients: matrices lie on 16-byte boundaries");
+  const int64_t runs = (count_a + 7) / 8 + (count_b + 7) / 8;
+  if (runs == 0) return;
+  const int blocks = static_cast<int>(std::min<int64_t>((runs + kScaleThreads - 1) / kScaleThreads, 8 * sms_of_device()));
+  check(launch_dependent(scale_gradients_kernel, dim3(blocks), dim3(kScaleThreads), 0, stream, factor, static_cast<__nv_bfloat16*>(a), count_a,
+                         static_cast<__nv_bfloat16*>(b), count_b),
+        "scale_gradients");
 }
 
 }  // namespace soapb200

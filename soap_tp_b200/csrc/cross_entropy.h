@@ -17,35 +17,55 @@ struct HeadProblem {
   bool bf16;
   const int64_t* targets;
   int64_t ignore_index, first_word, vocabulary;
+  // The tokens that count, one after another: how many there are, which token each is, the column that is its target here (kElsewhere: another
+  // rank's, kUnknown: none's), and their hidden states, unless all tokens count.
+  int* count;               // [1]
+  int* where;               // [tokens]
+  int* column;              // [tokens]
+  Matrix16 packed;          // [tokens][depth]
 };
+constexpr int kElsewhere = -1, kUnknown = -2;
 
-// lse[i] = log sum_j exp(l_ij) over this rank's words, picked[i] = l_i,t_i where the target is one of them and 0 elsewhere.
-// `parts`: ceil(words / 128) x tokens pairs.
-void head_statistics(const HeadProblem& p, float2* parts, float* lse, float* picked, int* status, cudaStream_t stream);
+// Fills count, where, column and packed; with `d_hidden`, clears the rows of the tokens that do not count.
+void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaStream_t stream);
 
-// losses[i] = lse - picked; 0 for tokens that do not count, NaN for targets outside the vocabulary.  With a reduction the
-// result goes to `loss`, and how many tokens count to `counted`.
-void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, float* counted,
-                 cudaStream_t stream);
+// For tokens first .. first + rows of those that count: lse[i] = log sum_j exp(l_ij) over this rank's words, picked[i] = l_i,t_i where the
+// target is one of them and 0 elsewhere.  `parts`: ceil(words / 128) x rows pairs.  With `logits` (bf16) the exponentials stay
+// there, each relative to the largest of its part.
+struct LogitRows {
+  int first, rows;
+  void* logits;
+  int64_t ld_logits;
+  float2* parts;
+};
+void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float* picked, int* status, cudaStream_t stream);
 
-// What the gradient of the loss multiplies row i by: factor[i] * *alpha.  `grad_loss` has one value per token, or one.
-void head_factors(const HeadProblem& p, LossReduction reduction, const float* grad_loss, const float* counted, float* factor,
-                  float* alpha, cudaStream_t stream);
+// losses = lse - picked by token; 0 for tokens that do not count, NaN for targets outside the vocabulary.  With a reduction the result
+// goes to `loss`.
+void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, cudaStream_t stream);
 
-// Gradients of the hidden states and the weight (either may be null), `rows` tokens at a time through `logits`, rows x pitch 16-bit values.
-// `sum`: words x ld_sum floats, needed where the tokens take more than one turn.
+// What the gradient of the loss multiplies the row of a token that counts by: factor[i] * *alpha.  `grad_loss` has one value per token,
+// or one; null: one.
+void head_factors(const HeadProblem& p, LossReduction reduction, const float* grad_loss, float* factor, float* alpha, cudaStream_t stream);
+
+// The exponentials that head_statistics left become the logits' gradient, factor (exp(l - lse) - [target]).
+void head_rescale(const HeadProblem& p, const LogitRows& r, const float* lse, const float* picked, const float* factor, cudaStream_t stream);
+// The logits' gradient from the logits anew.
+void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const float* lse, const float* factor, int* status, cudaStream_t stream);
+
+// Gradients of the hidden states and the weight (either may be null) from the logits' gradient of these rows.  The weight's is summed over
+// the turns in `sum`, words x ld_sum floats, where one does not take all tokens.
 struct HeadGradients {
   void* hidden;
   int64_t ld_hidden;
   void* weight;
   int64_t ld_weight;
-  void* logits;
-  int64_t ld_logits;
-  int rows;
   float* sum;
   int64_t ld_sum;
 };
-void head_gradients(const HeadProblem& p, const float* lse, const float* factor, const float* alpha, const HeadGradients& g, int* status,
-                    cudaStream_t stream);
+void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha, const HeadGradients& g, int* status, cudaStream_t stream);
+
+// Two contiguous bf16 matrices times *factor, in place; nothing where it is one.
+void scale_gradients(const float* factor, void* a, int64_t count_a, void* b, int64_t count_b, cudaStream_t stream);
 
 }  // namespace soapb200

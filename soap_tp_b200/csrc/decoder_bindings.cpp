@@ -70,53 +70,90 @@ HeadProblem head_problem(Reader& in) {
   p.bf16 = in.next() != 0;
   p.targets = in.pointer<int64_t>();
   p.ignore_index = in.next(); p.first_word = in.next(); p.vocabulary = in.next();
+  p.count = in.pointer<int>(); p.where = p.count + 1; p.column = p.where + p.tokens;      // 1 + 2 * tokens integers
+  p.packed.data = in.pointer<void>(); p.packed.ld = in.next(); p.packed.k_major = true;
   return p;
+}
+
+LogitRows logit_rows(Reader& in) {
+  LogitRows r{};
+  r.first = in.size(); r.rows = in.size();
+  r.logits = in.pointer<void>(); r.ld_logits = in.next();
+  r.parts = in.pointer<float2>();
+  return r;
 }
 }  // namespace
 
 void register_decoder(py::module_& m) {
-  m.def("head_statistics", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& buffers) {
-    Reader first(problem), in(buffers);
+  // Each call: the problem, then what this step adds (addresses, pitches, sizes), the status word where it is needed, the stream.
+  m.def("head_prepare", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& more) {
+    Reader first(problem), in(more);
     const HeadProblem p = head_problem(first);
     first.finish();
-    auto* parts = in.pointer<float2>(); auto* lse = in.pointer<float>(); auto* picked = in.pointer<float>();
+    auto* d_hidden = in.pointer<void>();
+    const int64_t ld = in.next();
+    auto stream = in.stream();
+    in.finish();
+    head_prepare(p, d_hidden, ld, stream);
+  });
+  m.def("head_statistics", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& more) {
+    Reader first(problem), in(more);
+    const HeadProblem p = head_problem(first);
+    first.finish();
+    const LogitRows r = logit_rows(in);
+    auto* lse = in.pointer<float>(); auto* picked = in.pointer<float>();
     auto* status = in.pointer<int>(); auto stream = in.stream();
     in.finish();
-    head_statistics(p, parts, lse, picked, status, stream);
+    head_statistics(p, r, lse, picked, status, stream);
   });
-  m.def("head_losses", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& buffers) {
-    Reader first(problem), in(buffers);
+  m.def("head_losses", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& more) {
+    Reader first(problem), in(more);
     const HeadProblem p = head_problem(first);
     first.finish();
     auto* lse = in.pointer<float>(); auto* picked = in.pointer<float>();
     const auto reduction = static_cast<LossReduction>(in.next());
-    auto* loss = in.pointer<float>(); auto* counted = in.pointer<float>(); auto stream = in.stream();
+    auto* loss = in.pointer<float>(); auto stream = in.stream();
     in.finish();
-    head_losses(p, lse, picked, reduction, loss, counted, stream);
+    head_losses(p, lse, picked, reduction, loss, stream);
   });
-  m.def("head_factors", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& buffers) {
-    Reader first(problem), in(buffers);
+  m.def("head_factors", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& more) {
+    Reader first(problem), in(more);
     const HeadProblem p = head_problem(first);
     first.finish();
     const auto reduction = static_cast<LossReduction>(in.next());
-    auto* grad_loss = in.pointer<float>(); auto* counted = in.pointer<float>();
-    auto* factor = in.pointer<float>(); auto* alpha = in.pointer<float>(); auto stream = in.stream();
+    auto* grad_loss = in.pointer<float>(); auto* factor = in.pointer<float>(); auto* alpha = in.pointer<float>();
+    auto stream = in.stream();
     in.finish();
-    head_factors(p, reduction, grad_loss, counted, factor, alpha, stream);
+    head_factors(p, reduction, grad_loss, factor, alpha, stream);
   });
-  m.def("head_gradients", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& buffers) {
-    Reader first(problem), in(buffers);
+  // The gradients of one turn.  With `picked` the logits are the exponentials that head_statistics left, otherwise they are computed anew.
+  m.def("head_gradients", [](const std::vector<int64_t>& problem, const std::vector<int64_t>& more) {
+    Reader first(problem), in(more);
     const HeadProblem p = head_problem(first);
     first.finish();
-    auto* lse = in.pointer<float>(); auto* factor = in.pointer<float>(); auto* alpha = in.pointer<float>();
+    const LogitRows r = logit_rows(in);
+    auto* lse = in.pointer<float>(); auto* picked = in.pointer<float>();
+    auto* factor = in.pointer<float>(); auto* alpha = in.pointer<float>();
     HeadGradients g{};
     g.hidden = in.pointer<void>(); g.ld_hidden = in.next();
     g.weight = in.pointer<void>(); g.ld_weight = in.next();
-    g.logits = in.pointer<void>(); g.ld_logits = in.next(); g.rows = in.size();
     g.sum = in.pointer<float>(); g.ld_sum = in.next();
     auto* status = in.pointer<int>(); auto stream = in.stream();
     in.finish();
-    head_gradients(p, lse, factor, alpha, g, status, stream);
+    if (picked) head_rescale(p, r, lse, picked, factor, stream);
+    else head_logit_gradient(p, r, lse, factor, status, stream);
+    head_gradients(p, r, alpha, g, status, stream);
+  });
+  m.def("scale_gradients", [](const std::vector<int64_t>& values) {
+    Reader in(values);
+    auto* factor = in.pointer<float>();
+    auto* a = in.pointer<void>();
+    const int64_t count_a = in.next();
+    auto* b = in.pointer<void>();
+    const int64_t count_b = in.next();
+    auto stream = in.stream();
+    in.finish();
+    scale_gradients(factor, a, count_a, b, count_b, stream);
   });
   // A plain product, C[m, n] = sum_k A(m, k) B(n, k), B with N along its rows and A in either order (tests, kernel cases).
   m.def("gemm16_store", [](bool bf16, bool a_k_major, const std::vector<int64_t>& values) {

@@ -3,14 +3,16 @@
 // A persistent kernel of clusters of two CTAs, one CTA per SM; a pair takes 256 x 256 tiles one after another:
 //   warp 0, one lane : TMA producer - this CTA's 128 rows of A and its 128 of the tile's 256 rows of B, 64 of K, per stage of 32 KB
 //   warp 1, one lane : MMA issuer (leader CTA) - M 256 x N 256 x K 16, cta_group::2
-//   warps 2..9       : epilogue - each a quarter of the CTA's 128 rows and half of the columns
+//   warps 4..11      : epilogue - each a quarter of the CTA's 128 rows and half of the columns, 128 sums a thread; their two warpgroups
+//                      take the registers that the first one (two of whose warps are idle) gives back
 // The accumulator takes 256 of TMEM's 512 columns, so that the epilogue of a tile runs beside the products of the next.
 // Operands whose M or N runs along memory's rows go in as they lie (kUmmaMnMajorA, kUmmaMnMajorB): the gradients' products
 // read the logits' gradient in both directions, and no matrix is transposed.
 //
-// The accumulator is drained once, after the whole of K.  The tensor core truncates as it adds, 2^-24 of the running sum per 16 of K on
-// average: at most 3e-5 of a logit's own size at K = 8192, and 5e-4 of a gradient's over 128256 words, a quarter of what its
-// rounding to bf16 costs.
+// The tensor core truncates as it adds: 2^-24 of the running sum per 16 of K on average.  Logits are drained from TMEM into sums in registers
+// (round to nearest) every 256 of K, or 512 for the first two drains of a tile, while the previous tile's epilogue still runs: a loss is then
+// off by some 5e-7 of itself where one sum over K = 4096 was off by 2e-6.  Gradients are drained once: 5e-4 of one over 128256
+// words at most, a quarter of what its rounding to bf16 costs.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,7 +37,10 @@ constexpr int kOperandBytes = kRows * kBK * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kStages = 6;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kFirstEpiWarp = 4;
+constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
+// 384 threads are launched with 168 registers each, 64512 together; 128 * 40 + 256 * 224 = 62464.
+constexpr int kFewRegisters = 40, kManyRegisters = 224;
 constexpr int kWarpStaging = 32 * 128;           // 32 rows of 128 bytes
 constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kWarpStaging + 1024 + 256;
 constexpr int kWarpColumns = kTile / 2;          // of the tile, per epilogue thread
@@ -74,9 +79,10 @@ struct Tiles {
 };
 
 // 32 rows of 128 bytes, one per lane, to 32 rows of a matrix: staged in shared memory (16-byte words swizzled by row, so that
-// neither side has bank conflicts) and stored with whole 128-byte lines.  `valid` bytes of each row are inside the matrix.
-__device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&words)[32], uint8_t* first, int64_t pitch, int rows,
-                                            int valid, int element, bool wide, int lane) {
+// neither side has bank conflicts) and stored with whole 128-byte lines.  Row i is row where[first + i] of `base`, or first + i;
+// `valid` bytes of each row are inside the matrix.
+__device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&words)[32], uint8_t* base, int64_t pitch, const int* where,
+                                            int first, int rows, int valid, int element, bool wide, int lane) {
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     *reinterpret_cast<uint4*>(staging + lane * 128 + ((c ^ (lane & 7)) << 4)) =
@@ -88,7 +94,7 @@ __device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&w
     const int row = 4 * i + (lane >> 3);
     const uint4 v = *reinterpret_cast<const uint4*>(staging + row * 128 + ((chunk ^ (row & 7)) << 4));
     if (row < rows) {
-      uint8_t* dst = first + row * pitch + chunk * 16;
+      uint8_t* dst = base + (where ? where[first + row] : first + row) * pitch + chunk * 16;
       const int left = valid - chunk * 16;
       if (wide && left >= 16) {
         *reinterpret_cast<uint4*>(dst) = v;
@@ -109,115 +115,132 @@ __device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&w
   __syncwarp();
 }
 
-// An epilogue thread's row of the tile: `taddr` is the first of its 128 columns.
+// Lines of 64 16-bit values whose row i goes to row where[i] of a matrix.
+template <typename T>
+__device__ __forceinline__ void store_values(uint8_t* staging, const uint32_t (&words)[32], const Gemm16Problem& p, int m_warp, int column,
+                                             int rows, int cols, bool wide, int lane) {
+  store_lines(staging, words, reinterpret_cast<uint8_t*>(p.C) + static_cast<int64_t>(column) * 2, p.ldc * 2, p.where, m_warp, rows, 2 * min(64, cols), 2, wide, lane);
+}
+
+// An epilogue thread's 128 logits of one token.
 template <int EPI, typename T>
-__device__ __forceinline__ void epilogue_row(const Gemm16Problem& p, uint32_t taddr, int m_warp, int n0, uint8_t* staging, int lane) {
+__device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, float (&v)[kWarpColumns], int M, int m_warp, int n0, uint8_t* staging, int lane) {
   const int row = m_warp + lane;
-  const bool inside = row < p.M;
+  const bool inside = row < M;
   const int cols = min(kWarpColumns, p.N - n0);           // of this thread's part; may be negative
-  if constexpr (EPI == kLogitStatistics) {
-    const int64_t target = inside ? p.targets[row] - p.first_word - n0 : -1;
-    float largest = -INFINITY, sum = 0.f, picked = 0.f;
-#pragma unroll
-    for (int c = 0; c < kWarpColumns; c += 32) {
-      uint32_t raw[32];
-      tmem_ld_32x32(taddr + c, raw);
-      tmem_ld_wait();
-      if (c + 32 > cols) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j >= cols) raw[j] = __float_as_uint(-INFINITY);
-      }
-      float most = __uint_as_float(raw[0]);
-#pragma unroll
-      for (int j = 1; j < 32; ++j) most = fmaxf(most, __uint_as_float(raw[j]));
-      most = fmaxf(most, largest);
-      // (a row of no finite logit is taken relative to zero, so that its sum is zero, or NaN where a logit is)
-      const float base = most == -INFINITY ? 0.f : most * kLog2e;
-      float part = 0.f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) part += exp2_fast(fmaf(__uint_as_float(raw[j]), kLog2e, -base));
-      sum = fmaf(sum, exp2_fast(fmaf(largest, kLog2e, -base)), part);
-      largest = most;
-      if (target >= c && target < c + 32) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (target == c + j) picked = __uint_as_float(raw[j]);
-      }
-    }
-    if (inside && cols > 0) {
-      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.M + row] = make_float2(largest, sum);
-      if (target >= 0 && target < cols) p.picked[row] = picked;
-    }
-  } else if constexpr (EPI == kLogitGradient) {
-    const int64_t target = inside ? p.targets[row] - p.first_word - n0 : -1;
+  // (the gradient's rows up to the next multiple of 64 are cleared: they are read as part of K)
+  const int rows = min(32, (EPI == kLogitGradient ? min(p.M, (M + kBK - 1) / kBK * kBK) : M) - m_warp);
+  const int target = inside ? p.targets[row] - n0 : -1;
+  if constexpr (EPI == kLogitGradient) {
     const float base = inside ? p.lse[row] * kLog2e : 0.f, factor = inside ? p.factor[row] : 0.f;
-    const int rows = min(32, p.M - m_warp);
 #pragma unroll
     for (int c = 0; c < kWarpColumns; c += 64) {
       uint32_t words[32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t raw[32];
-        tmem_ld_32x32(taddr + c + 32 * h, raw);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float p_j = exp2_fast(fmaf(__uint_as_float(raw[j]), kLog2e, -base));
-          raw[j] = __float_as_uint((target == c + 32 * h + j ? p_j - 1.f : p_j) * factor);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) words[16 * h + j] = pack16<T>(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
+      for (int j = 0; j < 64; ++j) {
+        const float e = exp2_fast(fmaf(v[c + j], kLog2e, -base));
+        v[c + j] = inside ? (target == c + j ? e - 1.f : e) * factor : 0.f;
       }
-      if (rows > 0 && c < cols)
-        store_lines(staging, words, reinterpret_cast<uint8_t*>(p.C) + (m_warp * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
-                    2 * min(64, cols - c), 2, true, lane);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) words[j] = pack16<T>(v[c + 2 * j], v[c + 2 * j + 1]);
+      if (rows > 0 && c < cols) store_values<T>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
     }
   } else {
-    const int rows = min(32, p.M - m_warp);
-    const float alpha = p.alpha ? *p.alpha : 1.f;
-    const bool to16 = p.C != nullptr;
-    const bool wide = (reinterpret_cast<uintptr_t>(p.C) & 15) == 0 && (p.ldc & 7) == 0;
+    if (cols < kWarpColumns) {
 #pragma unroll
-    for (int c = 0; c < kWarpColumns; c += 64) {
-      uint32_t words[32];
+      for (int j = 0; j < kWarpColumns; ++j)
+        if (j >= cols) v[j] = -INFINITY;
+    }
+    if (inside && target >= 0 && target < cols) {
+      float picked = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t raw[32];
-        const int at = c + 32 * h;
-        tmem_ld_32x32(taddr + at, raw);
-        tmem_ld_wait();
-        if (p.add && inside && at < cols) {
-          const float* old = p.accumulator + row * p.ld_accumulator + n0 + at;
+      for (int j = 0; j < kWarpColumns; ++j)
+        if (target == j) picked = v[j];
+      p.picked[row] = picked;
+    }
+    float most[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {               // (the accumulator's pitch is a multiple of 32)
-            const float4 v = *reinterpret_cast<const float4*>(old + j);
-            raw[j] = __float_as_uint(__uint_as_float(raw[j]) + v.x);
-            raw[j + 1] = __float_as_uint(__uint_as_float(raw[j + 1]) + v.y);
-            raw[j + 2] = __float_as_uint(__uint_as_float(raw[j + 2]) + v.z);
-            raw[j + 3] = __float_as_uint(__uint_as_float(raw[j + 3]) + v.w);
-          }
-        }
-        if (to16) {
+    for (int j = 4; j < kWarpColumns; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
+    const float largest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    // (a row of no finite logit is taken relative to zero, so that its sum is zero, or NaN where a logit is)
+    const float base = largest == -INFINITY ? 0.f : largest * kLog2e;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            words[16 * h + j] = pack16<T>(alpha * __uint_as_float(raw[2 * j]), alpha * __uint_as_float(raw[2 * j + 1]));
-        } else if (rows > 0 && at < cols) {
-          store_lines(staging, raw, reinterpret_cast<uint8_t*>(p.accumulator + m_warp * p.ld_accumulator + n0 + at),
-                      p.ld_accumulator * 4, rows, 128, 4, true, lane);
-        }
+    for (int j = 0; j < kWarpColumns; ++j) {
+      v[j] = exp2_fast(fmaf(v[j], kLog2e, -base));
+      sum[j & 3] += v[j];
+    }
+    if (inside && cols > 0)
+      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.ld_parts + row] = make_float2(largest, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if constexpr (EPI == kLogitExponential) {
+#pragma unroll
+      for (int c = 0; c < kWarpColumns; c += 64) {
+        uint32_t words[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) words[j] = pack16<T>(v[c + 2 * j], v[c + 2 * j + 1]);
+        if (rows > 0 && c < cols) store_values<T>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
       }
-      if (to16 && rows > 0 && c < cols)
-        store_lines(staging, words, reinterpret_cast<uint8_t*>(p.C) + (m_warp * p.ldc + n0 + c) * 2, p.ldc * 2, rows,
-                    2 * min(64, cols - c), 2, wide, lane);
     }
   }
 }
 
+// An epilogue thread's row of a product; `taddr` is the first of its 128 columns.  `empty`: nothing was added up.
+template <typename T>
+__device__ __forceinline__ void product_epilogue(const Gemm16Problem& p, uint32_t taddr, bool empty, int M, int m_warp, int n0, uint8_t* staging, int lane) {
+  const int row = m_warp + lane;
+  const bool inside = row < M;
+  const int cols = min(kWarpColumns, p.N - n0);
+  const int rows = min(32, M - m_warp);
+  const float alpha = p.alpha ? *p.alpha : 1.f;
+  const bool to16 = p.C != nullptr;
+  const bool wide = (reinterpret_cast<uintptr_t>(p.C) & 15) == 0 && (p.ldc & 7) == 0;
+#pragma unroll
+  for (int c = 0; c < kWarpColumns; c += 64) {
+    uint32_t words[32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t raw[32];
+      const int at = c + 32 * h;
+      tmem_ld_32x32(taddr + at, raw);
+      tmem_ld_wait();
+      if (empty) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) raw[j] = 0;
+      }
+      if (p.add && inside && at < cols) {
+        const float* old = p.accumulator + row * p.ld_accumulator + n0 + at;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {               // (the accumulator's pitch is a multiple of 32)
+          const float4 v = *reinterpret_cast<const float4*>(old + j);
+          raw[j] = __float_as_uint(__uint_as_float(raw[j]) + v.x);
+          raw[j + 1] = __float_as_uint(__uint_as_float(raw[j + 1]) + v.y);
+          raw[j + 2] = __float_as_uint(__uint_as_float(raw[j + 2]) + v.z);
+          raw[j + 3] = __float_as_uint(__uint_as_float(raw[j + 3]) + v.w);
+        }
+      }
+      if (to16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          words[16 * h + j] = pack16<T>(alpha * __uint_as_float(raw[2 * j]), alpha * __uint_as_float(raw[2 * j + 1]));
+      } else if (rows > 0 && at < cols) {
+        store_lines(staging, raw, reinterpret_cast<uint8_t*>(p.accumulator + n0 + at), p.ld_accumulator * 4, nullptr, m_warp, rows, 128, 4, true, lane);
+      }
+    }
+    if (to16 && rows > 0 && c < cols) store_values<T>(staging, words, p, m_warp, n0 + c, rows, cols - c, wide, lane);
+  }
+}
+
+// K-blocks that the accumulator takes before its drain number `d` of a tile.
+template <bool LOGITS>
+__device__ __forceinline__ int drain_blocks(int d, int left) {
+  return LOGITS ? min(left, d < 2 ? 8 : 4) : left;
+}
+
 template <int EPI, bool A_K, bool B_K, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              const __grid_constant__ Gemm16Problem prob, int* status) {
+gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_all,
+              int all_tokens, const __grid_constant__ Gemm16Problem prob, int* status) {
+  constexpr bool kLogits = EPI != kStore16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + kStages * kStageBytes;
@@ -259,101 +282,150 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
   wait_for_predecessor();
   let_successor_start();
 
-  const Tiles tiles(prob.M, prob.N);
-  const int k_blocks = (prob.K + kBK - 1) / kBK;
+  int M = prob.M, K = prob.K;
+  const CUtensorMap *source_a = &map_a, *source_b = &map_b;
+  if (prob.count) {
+    const int count = *prob.count;
+    int& tokens = A_K ? M : K;
+    tokens = max(0, min(tokens, count - prob.first));
+    if (count == all_tokens) (kLogits ? source_a : source_b) = &map_all;
+  }
+  const Tiles tiles(M, prob.N);
+  const int k_blocks = (K + kBK - 1) / kBK;
 
-  if (warp == 0 && lane == 0) {
-    // ---------------- TMA producer (each CTA its own rows; the bytes are credited to the leader) ----------------
-    int s = 0;
-    uint32_t parity = 1;
-    bool first_round = true, ok = true;
-    for (int t = cluster; t < tiles.count() && ok; t += clusters) {
-      int m0, n0;
-      tiles.place(t, m0, n0);
-      m0 += cta * kRows;
-      n0 += cta * kRows;
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!first_round && !mbar_wait_bounded(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) {
-          ok = false;
-          break;
+  if (warp < kFirstEpiWarp) {
+    give_registers_back<kFewRegisters>();
+    if (warp == 0 && lane == 0) {
+      // ---------------- TMA producer (each CTA its own rows; the bytes are credited to the leader) ----------------
+      int s = 0;
+      uint32_t parity = 1;
+      bool first_round = true, ok = true;
+      for (int t = cluster; t < tiles.count() && ok; t += clusters) {
+        int m0, n0;
+        tiles.place(t, m0, n0);
+        m0 += cta * kRows;
+        n0 += cta * kRows;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!first_round && !mbar_wait_bounded(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) {
+            ok = false;
+            break;
+          }
+          uint8_t* stage = smem + s * kStageBytes;
+          if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
+          const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
+          if constexpr (A_K) {
+            tma_load_2d_pair(stage, source_a, bar, kb * kBK, m0);
+          } else {
+            tma_load_2d_pair(stage, source_a, bar, m0, kb * kBK);
+            tma_load_2d_pair(stage + kOperandBytes / 2, source_a, bar, m0 + 64, kb * kBK);
+          }
+          if constexpr (B_K) {
+            tma_load_2d_pair(stage + kOperandBytes, source_b, bar, kb * kBK, n0);
+          } else {
+            tma_load_2d_pair(stage + kOperandBytes, source_b, bar, n0, kb * kBK);
+            tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, source_b, bar, n0 + 64, kb * kBK);
+          }
+          if (++s == kStages) {
+            s = 0;
+            parity ^= 1;
+            first_round = false;
+          }
         }
-        uint8_t* stage = smem + s * kStageBytes;
-        if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
-        const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
-        if constexpr (A_K) {
-          tma_load_2d_pair(stage, &map_a, bar, kb * kBK, m0);
-        } else {
-          tma_load_2d_pair(stage, &map_a, bar, m0, kb * kBK);
-          tma_load_2d_pair(stage + kOperandBytes / 2, &map_a, bar, m0 + 64, kb * kBK);
-        }
-        if constexpr (B_K) {
-          tma_load_2d_pair(stage + kOperandBytes, &map_b, bar, kb * kBK, n0);
-        } else {
-          tma_load_2d_pair(stage + kOperandBytes, &map_b, bar, n0, kb * kBK);
-          tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, &map_b, bar, n0 + 64, kb * kBK);
-        }
-        if (++s == kStages) {
-          s = 0;
-          parity ^= 1;
-          first_round = false;
+      }
+      if (*abort_flag) {
+        // give copies that are still in flight time to land before the CTA's shared memory is released
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+      }
+    } else if (warp == 1 && lane == 0 && cta == 0) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t kIdesc = (std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kTile, kTile) : umma_idesc_fp16(kTile, kTile)) |
+                                  (A_K ? 0u : kUmmaMnMajorA) | (B_K ? 0u : kUmmaMnMajorB);
+      constexpr uint64_t kStepA = A_K ? 32 >> 4 : 2048 >> 4, kStepB = B_K ? 32 >> 4 : 2048 >> 4;      // 16 of K
+      int s = 0;
+      uint32_t parity = 0;
+      bool ok = true;
+      int it = 0;                                // drains so far
+      for (int t = cluster; t < tiles.count() && ok; t += clusters) {
+        for (int d = 0, kb = 0; kb < k_blocks && ok; ++d, ++it) {
+          const int buf = it & 1;
+          if (it >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
+          const int blocks = drain_blocks<kLogits>(d, k_blocks - kb);
+          for (int i = 0; i < blocks; ++i, ++kb) {
+            if (!mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t stage = smem_u32(smem + s * kStageBytes);
+            const uint64_t a = A_K ? umma_desc_kmajor<128>(stage) : umma_desc_mn_major(stage);
+            const uint64_t b = B_K ? umma_desc_kmajor<128>(stage + kOperandBytes) : umma_desc_mn_major(stage + kOperandBytes);
+  #pragma unroll
+            for (int k = 0; k < kBK / 16; ++k) umma_f16_ss_pair(acc, a + k * kStepA, b + k * kStepB, kIdesc, i | k ? 1u : 0u);
+            umma_commit_pair(&empty_bar[s]);
+            if (++s == kStages) {
+              s = 0;
+              parity ^= 1;
+            }
+          }
+          if (ok) umma_commit_pair(&acc_full[buf]);
         }
       }
     }
-    if (*abort_flag) {
-      // give copies that are still in flight time to land before the CTA's shared memory is released
-      for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    }
-  } else if (warp == 1 && lane == 0 && cta == 0) {
-    // ---------------- MMA issuer ----------------
-    constexpr uint32_t kIdesc = (std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kTile, kTile) : umma_idesc_fp16(kTile, kTile)) |
-                                (A_K ? 0u : kUmmaMnMajorA) | (B_K ? 0u : kUmmaMnMajorB);
-    constexpr uint64_t kStepA = A_K ? 32 >> 4 : 2048 >> 4, kStepB = B_K ? 32 >> 4 : 2048 >> 4;      // 16 of K
-    int s = 0;
-    uint32_t parity = 0;
-    bool ok = true;
-    int it = 0;
-    for (int t = cluster; t < tiles.count() && ok; t += clusters, ++it) {
-      const int buf = it & 1;
-      if (it >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) break;
-      tc_fence_after_sync();
-      const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t stage = smem_u32(smem + s * kStageBytes);
-        const uint64_t a = A_K ? umma_desc_kmajor<128>(stage) : umma_desc_mn_major(stage);
-        const uint64_t b = B_K ? umma_desc_kmajor<128>(stage + kOperandBytes) : umma_desc_mn_major(stage + kOperandBytes);
-#pragma unroll
-        for (int k = 0; k < kBK / 16; ++k) umma_f16_ss_pair(acc, a + k * kStepA, b + k * kStepB, kIdesc, kb | k ? 1u : 0u);
-        umma_commit_pair(&empty_bar[s]);
-        if (++s == kStages) {
-          s = 0;
-          parity ^= 1;
-        }
-      }
-      if (ok) umma_commit_pair(&acc_full[buf]);
-    }
-  } else if (warp >= 2) {
+  } else {
+    take_registers<kManyRegisters>();
     // ---------------- epilogue (each CTA its own 128 rows) ----------------
-    const int ew = warp - 2;
+    const int ew = warp - kFirstEpiWarp;
     const int quarter = warp & 3;              // TMEM lane quarter this warp may read
     const int col0 = (ew >> 2) * kWarpColumns;
     const uint32_t drained = map_to_cta(smem_u32(&acc_empty[0]), 0);
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(col0);
     int it = 0;
-    for (int t = cluster; t < tiles.count(); t += clusters, ++it) {
-      const int buf = it & 1;
-      int m0, n0;
-      tiles.place(t, m0, n0);
-      if (!mbar_wait_bounded(&acc_full[buf], (it >> 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) break;
+    auto filled = [&]() {
+      if (!mbar_wait_bounded(&acc_full[it & 1], (it >> 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) return false;
       tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buf * kTile + col0);
-      epilogue_row<EPI, T>(prob, taddr, m0 + cta * kRows + quarter * 32, n0 + col0, staging + ew * kWarpStaging, lane);
+      return true;
+    };
+    auto release = [&]() {
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(drained + static_cast<uint32_t>(buf * sizeof(uint64_t)));
+      if (lane == 0) mbar_arrive_cluster(drained + static_cast<uint32_t>((it & 1) * sizeof(uint64_t)));
+      ++it;
+    };
+    for (int t = cluster; t < tiles.count(); t += clusters) {
+      int m0, n0;
+      tiles.place(t, m0, n0);
+      const int m_warp = m0 + cta * kRows + quarter * 32;
+      if constexpr (kLogits) {
+        float v[kWarpColumns];
+        bool ok = true;
+        for (int d = 0, kb = 0; kb < k_blocks; ++d) {
+          kb += drain_blocks<true>(d, k_blocks - kb);
+          ok = filled();
+          if (!ok) break;
+          const uint32_t from = taddr + static_cast<uint32_t>((it & 1) * kTile);
+#pragma unroll
+          for (int c = 0; c < kWarpColumns; c += 32) {
+            uint32_t raw[32];
+            tmem_ld_32x32(from + c, raw);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[c + j] = d ? v[c + j] + __uint_as_float(raw[j]) : __uint_as_float(raw[j]);
+          }
+          release();
+        }
+        if (!ok) break;
+        logits_epilogue<EPI, T>(prob, v, M, m_warp, n0 + col0, staging + ew * kWarpStaging, lane);
+      } else {
+        const bool empty = k_blocks == 0;
+        if (!empty && !filled()) break;
+        product_epilogue<T>(prob, taddr + static_cast<uint32_t>((it & 1) * kTile), empty, M, m_warp, n0 + col0, staging + ew * kWarpStaging, lane);
+        if (!empty) release();
+      }
     }
   }
 
@@ -380,41 +452,51 @@ int pairs_of_device() {
 }
 
 template <int EPI, bool A_K, bool B_K, typename T>
-void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream) {
+void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream, const Hidden16* hidden) {
   static PerDeviceOnce configured;
   allow_dynamic_smem(reinterpret_cast<const void*>(gemm16_kernel<EPI, A_K, B_K, T>), kSmemBytes, configured, "gemm16");
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   const CUtensorMap map_a = map_of(kBf16, a, p.M, p.K), map_b = map_of(kBf16, b, p.N, p.K);
+  const CUtensorMap map_all = !hidden ? map_a : EPI != kStore16 ? map_of(kBf16, hidden->all, p.M, p.K) : map_of(kBf16, hidden->all, p.N, p.K);
   const int64_t tiles = static_cast<int64_t>((p.M + kTile - 1) / kTile) * ((p.N + kTile - 1) / kTile);
   if (tiles > (1 << 30)) throw std::invalid_argument("gemm16: too many tiles");
   const int clusters = static_cast<int>(tiles < pairs_of_device() ? tiles : pairs_of_device());
   cudaError_t err = launch_dependent(gemm16_kernel<EPI, A_K, B_K, T>, dim3(2 * clusters), dim3(kThreads), kSmemBytes, stream, map_a,
-                                     map_b, p, status);
+                                     map_b, map_all, hidden ? hidden->tokens : -1, p, status);
   if (err != cudaSuccess) throw std::runtime_error(std::string("gemm16 launch: ") + cudaGetErrorString(err));
 }
 
 template <typename T>
-void dispatch(Gemm16Epilogue epilogue, const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream) {
-  if (epilogue == kLogitStatistics && a.k_major && b.k_major) launch<kLogitStatistics, true, true, T>(a, b, p, status, stream);
-  else if (epilogue == kLogitGradient && a.k_major && b.k_major) launch<kLogitGradient, true, true, T>(a, b, p, status, stream);
-  else if (epilogue == kStore16 && a.k_major && !b.k_major) launch<kStore16, true, false, T>(a, b, p, status, stream);
-  else if (epilogue == kStore16 && !a.k_major && !b.k_major) launch<kStore16, false, false, T>(a, b, p, status, stream);
+void dispatch(Gemm16Epilogue epilogue, const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream,
+              const Hidden16* hidden) {
+  const bool logits = a.k_major && b.k_major;
+  if (epilogue == kLogitStatistics && logits) launch<kLogitStatistics, true, true, T>(a, b, p, status, stream, hidden);
+  else if (epilogue == kLogitGradient && logits) launch<kLogitGradient, true, true, T>(a, b, p, status, stream, hidden);
+  else if (epilogue == kStore16 && a.k_major && !b.k_major && !hidden) launch<kStore16, true, false, T>(a, b, p, status, stream, hidden);
+  else if (epilogue == kStore16 && !a.k_major && !b.k_major) launch<kStore16, false, false, T>(a, b, p, status, stream, hidden);
   else throw std::invalid_argument("gemm16: no kernel for these orders of the operands");
 }
 
 }  // namespace
 
 void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status,
-            cudaStream_t stream) {
+            cudaStream_t stream, const Hidden16* hidden) {
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) throw std::invalid_argument("gemm16: empty product");
-  if (a.ld % 8 != 0 || b.ld % 8 != 0) throw std::invalid_argument("gemm16: operand pitches are multiples of 8 elements");
-  if (epilogue == kLogitGradient && (p.ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(p.C) & 15) != 0))
+  if (a.ld % 8 != 0 || b.ld % 8 != 0 || (hidden && hidden->all.ld % 8 != 0))
+    throw std::invalid_argument("gemm16: operand pitches are multiples of 8 elements");
+  if ((epilogue == kLogitGradient || epilogue == kLogitExponential) && (p.ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(p.C) & 15) != 0))
     throw std::invalid_argument("gemm16: the logits' gradient needs 16-byte rows");
   if (epilogue == kStore16 && (p.add || !p.C) && (!p.accumulator || p.ld_accumulator % 32 != 0 || p.ld_accumulator < p.N ||
                                                   (reinterpret_cast<uintptr_t>(p.accumulator) & 15) != 0))
     throw std::invalid_argument("gemm16: the accumulator's pitch is a multiple of 32 covering the columns");
-  if (bf16) dispatch<__nv_bfloat16>(epilogue, a, b, p, status, stream);
-  else dispatch<__half>(epilogue, a, b, p, status, stream);
+  if (epilogue == kLogitExponential) {
+    if (!bf16 || !a.k_major || !b.k_major) throw std::invalid_argument("gemm16: exponentials are kept in bf16, of K-major operands");
+    launch<kLogitExponential, true, true, __nv_bfloat16>(a, b, p, status, stream, hidden);
+  } else if (bf16) {
+    dispatch<__nv_bfloat16>(epilogue, a, b, p, status, stream, hidden);
+  } else {
+    dispatch<__half>(epilogue, a, b, p, status, stream, hidden);
+  }
 }
 
 }  // namespace soapb200

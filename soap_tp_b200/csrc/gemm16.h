@@ -16,33 +16,47 @@ struct Matrix16 {
 
 enum Gemm16Epilogue : int {
   kLogitStatistics = 0,     // largest logit and sum of exponentials per row and 128 columns, and the logit of each row's target
-  kLogitGradient = 1,       // softmax minus target, times the row's factor, as a 16-bit matrix
-  kStore16 = 2,             // the product itself
+  kLogitExponential = 1,    // the same, and the exponentials themselves, relative to the largest of their part, as a 16-bit matrix
+  kLogitGradient = 2,       // softmax minus target, times the row's factor, as a 16-bit matrix
+  kStore16 = 3,             // the product itself
 };
 
 constexpr int kLogitPart = 128;      // columns that share one partial maximum and sum
 
 struct Gemm16Problem {
   int M, N, K;
-  // logits: row i is a token, column j a word; the token's target counts from this matrix's first column
-  const int64_t* targets;
-  int64_t first_word;
-  float2* parts;            // [ceil(N / kLogitPart)][M]: largest logit, sum of exp(logit - largest)
+  // How many tokens there are is known on the device: `*count` in all, of which this product starts with number `first`.  They are
+  // A's rows (logits, and kStore16 with A K-major), or K.  Null: M and K hold as they are.
+  const int* count;
+  int first;
+  // logits: row i is a token, column j a word
+  const int* targets;       // [M]: the column that is the token's target; negative where none of them is
+  float2* parts;            // [ceil(N / kLogitPart)][ld_parts]: largest logit, sum of exp(logit - largest)
+  int64_t ld_parts;
   float* picked;            // [M]: the target's logit, written where the target is a column
   const float* lse;         // [M]
   const float* factor;      // [M]
-  // kLogitGradient, kStore16: 16-bit result [M][ldc]
+  // 16-bit result [M][ldc]
   void* C;
   int64_t ldc;
-  // kStore16: alpha * (product + accumulator); without `C` the sum goes back into the accumulator [M][ld_accumulator]
+  // kStore16: alpha * (product + accumulator), row i of it in row where[i] of C; without `C` the sum goes back into the accumulator
+  const int* where;         // null: rows stay where they are
   const float* alpha;       // on the device; null: 1
-  float* accumulator;
+  float* accumulator;       // [M][ld_accumulator]
   int64_t ld_accumulator;
   bool add;                 // whether the accumulator holds something
 };
 
+// The hidden states in two places: the tokens that count one after another, and all of them (`all`, of `tokens` rows), which is where
+// they are read from when every token counts.
+struct Hidden16 {
+  Matrix16 packed, all;
+  int tokens;
+};
+
 // acc[m, n] = sum_k A(m, k) B(n, k) and its epilogue.  `bf16`: both operands and the 16-bit result are bf16, otherwise fp16.
+// `hidden` (or null) stands for the operand that the tokens' states are: A of logits, B of kStore16 otherwise.
 void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix16& b, const Gemm16Problem& problem, int* status,
-            cudaStream_t stream);
+            cudaStream_t stream, const Hidden16* hidden = nullptr);
 
 }  // namespace soapb200

@@ -284,6 +284,17 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// Registers of this warpgroup's threads from here on; all four warps take part.  What the block was launched with is what there is
+// to share out.
+template <int N>
+__device__ __forceinline__ void give_registers_back() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Instruction descriptor bits of operands that are M-major (A) or N-major (B) in shared memory.
 constexpr uint32_t kUmmaMnMajorA = 1u << 15, kUmmaMnMajorB = 1u << 16;
 

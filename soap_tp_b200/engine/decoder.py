@@ -30,80 +30,93 @@ def _rows16(x: Tensor) -> Tensor:
     return padded
 
 
-class Head(NamedTuple):
-    """One call's hidden states, this rank's words and the targets, ready for the kernels."""
+class Head:
+    """One call's hidden states, this rank's words and the targets, ready for the kernels (``csrc/cross_entropy.h``)."""
 
-    hidden: Tensor
-    weight: Tensor
-    targets: Tensor
-    ignore_index: int
-    first_word: int
-    vocabulary: int
+    def __init__(self, hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int, first_word: int, vocabulary: int) -> None:
+        self.hidden, self.weight, self.targets = _rows16(hidden), _rows16(weight), targets.to(torch.int64).contiguous()
+        self.tokens, self.depth, self.words = hidden.shape[0], hidden.shape[1], weight.shape[0]
+        self.device, self.dtype = hidden.device, hidden.dtype
+        # how many tokens count, which they are and their targets' columns; their hidden states, used unless all count
+        self.numbers_of = torch.empty(1 + 2 * self.tokens, dtype=torch.int32, device=self.device)
+        self.packed = torch.empty((self.tokens, k.round_up(self.depth, 8)), dtype=self.dtype, device=self.device)
+        self.problem = [self.hidden.data_ptr(), self.hidden.stride(0), self.weight.data_ptr(), self.weight.stride(0), self.tokens, self.depth,
+                        self.words, int(self.dtype == torch.bfloat16), self.targets.data_ptr(), ignore_index, first_word, vocabulary,
+                        self.numbers_of.data_ptr(), self.packed.data_ptr(), self.packed.shape[1]]
+        self.status = k.status_word(self.device).data_ptr()
 
-    @staticmethod
-    def of(hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int, first_word: int, vocabulary: int) -> "Head":
-        return Head(_rows16(hidden), _rows16(weight), targets.to(torch.int64).contiguous(), ignore_index, first_word, vocabulary)
+    def prepare(self, d_hidden: Optional[Tensor] = None) -> None:
+        """Finds the tokens that count; the rows of ``d_hidden`` that belong to the others are cleared."""
+        _C.head_prepare(self.problem, [0 if d_hidden is None else d_hidden.data_ptr(), self.depth, k._stream()])
+        k._count("head_count_kernel")
+        k._count("head_gather_kernel")
 
-    @property
-    def device(self) -> torch.device:
-        return self.hidden.device
+    def turns(self, workspace_bytes: int):
+        """Tokens a turn, and the pitch of their logits in 16 bits: as many as the workspace holds, 256 at least."""
+        pitch = k.round_up(self.words, 64)
+        return min(self.tokens, max(256, workspace_bytes // (2 * pitch) // 256 * 256)), pitch
 
-    def numbers(self) -> list:
-        return [self.hidden.data_ptr(), self.hidden.stride(0), self.weight.data_ptr(), self.weight.stride(0), self.hidden.shape[0],
-                self.hidden.shape[1], self.weight.shape[0], int(self.hidden.dtype == torch.bfloat16), self.targets.data_ptr(),
-                self.ignore_index, self.first_word, self.vocabulary]
+    def parts(self, rows: int) -> Tensor:
+        return torch.empty((-(-self.words // LOGIT_PART), rows, 2), dtype=torch.float32, device=self.device)
 
-
-def head_statistics(head: Head) -> Tuple[Tensor, Tensor]:
-    """Log-sum-exp over this rank's words, and the target's logit where this rank has it (0 elsewhere), per token."""
-    tokens, words = head.hidden.shape[0], head.weight.shape[0]
-    parts = torch.empty((-(-words // LOGIT_PART), tokens, 2), dtype=torch.float32, device=head.device)
-    lse, picked = torch.empty((2, tokens), dtype=torch.float32, device=head.device)
-    _C.head_statistics(head.numbers(), [parts.data_ptr(), lse.data_ptr(), picked.data_ptr(), k.status_word(head.device).data_ptr(),
-                                        k._stream()])
-    k._count("gemm16_kernel")
-    k._count("head_join_kernel")
-    return lse, picked
-
-
-def head_losses(head: Head, lse: Tensor, picked: Tensor, reduction: str) -> Tuple[Tensor, Optional[Tensor]]:
-    """The loss, and with a reduction the number of tokens that count."""
-    counted = None
-    if reduction == "none":
-        loss = torch.empty_like(lse)
-    else:
-        loss, counted = torch.empty(2, dtype=torch.float32, device=head.device)
-    _C.head_losses(head.numbers(), [lse.data_ptr(), picked.data_ptr(), REDUCTIONS[reduction], loss.data_ptr(),
-                                    0 if counted is None else counted.data_ptr(), k._stream()])
-    k._count("head_losses_kernel")
-    return loss, counted
-
-
-def head_gradients(head: Head, lse: Tensor, reduction: str, grad_loss: Tensor, counted: Optional[Tensor], want_hidden: bool,
-                   want_weight: bool, workspace_bytes: int) -> Tuple[Optional[Tensor], Optional[Tensor]]:
-    """Gradients of the hidden states and of the weight; the softmax of ``workspace_bytes`` at a time is in memory."""
-    tokens, depth = head.hidden.shape
-    words = head.weight.shape[0]
-    factor = torch.empty(tokens + 1, dtype=torch.float32, device=head.device)
-    alpha = factor[tokens:]
-    grad_loss = grad_loss.to(torch.float32).contiguous()
-    _C.head_factors(head.numbers(), [REDUCTIONS[reduction], grad_loss.data_ptr(), 0 if counted is None else counted.data_ptr(),
-                                     factor.data_ptr(), alpha.data_ptr(), k._stream()])
-    pitch = k.round_up(words, 64)
-    rows = min(tokens, max(256, workspace_bytes // (2 * pitch) // 256 * 256))
-    logits = torch.empty((rows, pitch), dtype=head.hidden.dtype, device=head.device)
-    d_hidden = torch.empty((tokens, depth), dtype=head.hidden.dtype, device=head.device) if want_hidden else None
-    d_weight = torch.empty((words, depth), dtype=head.hidden.dtype, device=head.device) if want_weight else None
-    total = torch.empty((words, k.round_up(depth, 32)), dtype=torch.float32, device=head.device) if want_weight and rows < tokens else None
-    _C.head_gradients(head.numbers(), [
-        lse.data_ptr(), factor.data_ptr(), alpha.data_ptr(),
-        d_hidden.data_ptr() if want_hidden else 0, depth, d_weight.data_ptr() if want_weight else 0, depth,
-        logits.data_ptr(), pitch, rows, 0 if total is None else total.data_ptr(), 0 if total is None else total.stride(0),
-        k.status_word(head.device).data_ptr(), k._stream()])
-    k._count("head_factors_kernel")
-    for _ in range(-(-tokens // rows) * (1 + want_hidden + want_weight)):
+    def statistics(self, first: int, rows: int, parts: Tensor, lse: Tensor, picked: Tensor, logits: Optional[Tensor] = None) -> None:
+        """Log-sum-exp over this rank's words and the target's logit where this rank has it (0 elsewhere), of ``rows`` of the tokens
+        that count; the exponentials stay in ``logits``."""
+        _C.head_statistics(self.problem, [first, rows, 0 if logits is None else logits.data_ptr(), 0 if logits is None else logits.shape[1],
+                                          parts.data_ptr(), lse.data_ptr(), picked.data_ptr(), self.status, k._stream()])
         k._count("gemm16_kernel")
-    return d_hidden, d_weight
+        k._count("head_join_kernel")
+
+    def loss(self, lse: Tensor, picked: Tensor, reduction: str) -> Tensor:
+        loss = torch.empty(self.tokens if reduction == "none" else (), dtype=torch.float32, device=self.device)
+        _C.head_losses(self.problem, [lse.data_ptr(), picked.data_ptr(), REDUCTIONS[reduction], loss.data_ptr(), k._stream()])
+        k._count("head_losses_kernel")
+        return loss
+
+
+class HeadGradients:
+    """Gradients of a head's hidden states and weight (those that are wanted), made turn by turn from the tokens' softmax."""
+
+    def __init__(self, head: Head, want_hidden: bool, want_weight: bool, workspace_bytes: int) -> None:
+        self.head = head
+        self.rows, pitch = head.turns(workspace_bytes)
+        device, dtype = head.device, head.dtype
+        self.logits = torch.empty((self.rows, pitch), dtype=dtype, device=device)
+        self.hidden = torch.empty((head.tokens, head.depth), dtype=dtype, device=device) if want_hidden else None
+        self.weight = torch.empty((head.words, head.depth), dtype=dtype, device=device) if want_weight else None
+        several = want_weight and self.rows < head.tokens
+        self.sum = torch.empty((head.words, k.round_up(head.depth, 32)), dtype=torch.float32, device=device) if several else None
+        self.factor = torch.empty(1 + head.tokens, dtype=torch.float32, device=device)      # alpha, then a factor for each token
+
+    def turns(self):
+        for first in range(0, self.head.tokens, self.rows):
+            yield first, min(self.rows, self.head.tokens - first)
+
+    def factors(self, reduction: str, grad_loss: Optional[Tensor]) -> None:
+        alpha = self.factor.data_ptr()
+        _C.head_factors(self.head.problem, [REDUCTIONS[reduction], 0 if grad_loss is None else grad_loss.data_ptr(), alpha + 4, alpha, k._stream()])
+        k._count("head_factors_kernel")
+
+    def add(self, first: int, rows: int, lse: Tensor, parts: Optional[Tensor] = None, picked: Optional[Tensor] = None) -> None:
+        """One turn: from the exponentials that ``Head.statistics`` left in ``logits``, with their ``parts`` and ``picked``, or anew."""
+        head, alpha = self.head, self.factor.data_ptr()
+        _C.head_gradients(head.problem, [
+            first, rows, self.logits.data_ptr(), self.logits.shape[1], 0 if parts is None else parts.data_ptr(), lse.data_ptr(),
+            0 if picked is None else picked.data_ptr(), alpha + 4, alpha,
+            0 if self.hidden is None else self.hidden.data_ptr(), head.depth, 0 if self.weight is None else self.weight.data_ptr(), head.depth,
+            0 if self.sum is None else self.sum.data_ptr(), 0 if self.sum is None else self.sum.shape[1], head.status, k._stream()])
+        k._count("head_rescale_kernel" if parts is not None else "gemm16_kernel")
+        for wanted in (self.hidden, self.weight):
+            if wanted is not None:
+                k._count("gemm16_kernel")
+
+
+def scale_gradients(factor: Tensor, a: Optional[Tensor], b: Optional[Tensor]) -> None:
+    """Contiguous bf16 gradients times ``factor`` (one fp32 value), in place; nothing is moved where it is one."""
+    _C.scale_gradients([factor.data_ptr(), 0 if a is None else a.data_ptr(), 0 if a is None else a.numel(),
+                        0 if b is None else b.data_ptr(), 0 if b is None else b.numel(), k._stream()])
+    k._count("scale_gradients_kernel")
+    k.mark_written(a, b)
 
 
 VALUE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}

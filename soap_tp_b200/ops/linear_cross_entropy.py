@@ -1,8 +1,12 @@
 """Softmax cross entropy over a large vocabulary straight from the hidden states, without the logits.
 
 ``loss_i = log sum_j exp(h_i . w_j) - h_i . w_{t_i}``.  The head's product, the softmax and the loss are one pass whose logits stay in
-the tensor cores' accumulators; the gradients recompute them a bounded number of tokens at a time.  A head of 128256 words on 32768
-tokens would otherwise keep 16 GB of fp32 logits and as much again of their softmax for the backward pass.
+the tensor cores' accumulators; for the gradients the softmax of a bounded number of tokens at a time is in memory, in 16 bits.  A head of 128256
+words on 32768 tokens would otherwise keep 16 GB of fp32 logits and as much again of their softmax for the backward pass.
+
+On CUDA, bf16 and reduced to one number, the gradients are made together with the loss and the backward pass multiplies them by its
+own gradient (which moves nothing where that is one); so a loss whose gradients nobody wants belongs under ``torch.no_grad()``.  In the other
+cases the backward pass computes the logits again.
 
 With ``group`` the weight is this rank's equal slice of the vocabulary, in rank order, as ``ColumnParallelLinear`` stores a head:
 log-sum-exp and the target's logit are joined over the group, and the gradient of the (replicated) hidden states is summed over it.
@@ -50,12 +54,12 @@ def _world(group) -> int:
     return 1 if group is None else dist.get_world_size(group)
 
 
-def _join(lse: Tensor, picked: Tensor, group) -> Tensor:
-    """Log-sum-exp over all ranks' words; ``picked`` becomes the target's logit on every rank."""
+def _join(lse: Tensor, picked: Tensor, group) -> None:
+    """``lse`` becomes that over all ranks' words, ``picked`` the target's logit on every rank (both in place)."""
     every = [torch.empty_like(lse) for _ in range(_world(group))]
-    dist.all_gather(every, lse.contiguous(), group=group)
+    dist.all_gather(every, lse, group=group)
     dist.all_reduce(picked, group=group)
-    return torch.logsumexp(torch.stack(every), dim=0)
+    lse.copy_(torch.logsumexp(torch.stack(every), dim=0))
 
 
 def _wide(dtype: torch.dtype) -> torch.dtype:
@@ -95,50 +99,94 @@ class _HostHead:
         return d @ self.weight, d.t() @ self.hidden
 
 
+def _device_loss(ctx, hidden, weight, targets, reduction, ignore_index, group, workspace_bytes, want_hidden, want_weight):
+    """The loss and each counted token's log-sum-exp; where the gradients can come with it they are left in ``ctx.gradients``."""
+    from ..engine import decoder
+
+    head = decoder.Head(hidden, weight, targets, ignore_index, ctx.first_word, ctx.vocabulary)
+    lse, picked = torch.empty((2, head.tokens), dtype=torch.float32, device=head.device)
+    shared = _world(group) > 1
+    # bf16 only: fp16 gradients are rounded after the loss's scale, which the backward pass brings, has been multiplied in
+    if (want_hidden or want_weight) and reduction != "none" and head.dtype == torch.bfloat16:
+        gradients = decoder.HeadGradients(head, want_hidden, want_weight, workspace_bytes)
+        head.prepare(gradients.hidden)
+        gradients.factors(reduction, None)
+        parts = head.parts(gradients.rows)
+        for first, rows in gradients.turns():
+            head.statistics(first, rows, parts, lse, picked, gradients.logits)
+            if shared:
+                _join(lse[first:first + rows], picked[first:first + rows], group)
+            gradients.add(first, rows, lse, parts, picked)
+        ctx.gradients = (gradients.hidden, gradients.weight)
+    else:
+        head.prepare()
+        head.statistics(0, head.tokens, head.parts(head.tokens), lse, picked)
+        if shared:
+            _join(lse, picked, group)
+    return head.loss(lse, picked, reduction), lse
+
+
+def _device_gradients(ctx, grad_loss, hidden, weight, targets, lse, want_hidden, want_weight):
+    from ..engine import decoder
+
+    head = decoder.Head(hidden, weight, targets, ctx.ignore_index, ctx.first_word, ctx.vocabulary)
+    gradients = decoder.HeadGradients(head, want_hidden, want_weight, ctx.workspace_bytes)
+    head.prepare(gradients.hidden)
+    gradients.factors(ctx.reduction, grad_loss.to(torch.float32).contiguous())
+    for first, rows in gradients.turns():
+        gradients.add(first, rows, lse)
+    return gradients.hidden, gradients.weight
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, reduction, ignore_index, group, workspace_bytes):
         words = weight.shape[0]
-        world = _world(group)
-        first_word = 0 if group is None else dist.get_rank(group) * words
-        ctx.arguments = (reduction, ignore_index, first_word, words * world, group, workspace_bytes)
+        ctx.first_word = 0 if group is None else dist.get_rank(group) * words
+        ctx.vocabulary = words * _world(group)
+        ctx.reduction, ctx.ignore_index, ctx.group, ctx.workspace_bytes = reduction, ignore_index, group, workspace_bytes
+        ctx.gradients = None
+        shape = targets.shape
+        hidden, targets = hidden.detach().reshape(-1, hidden.shape[-1]), targets.reshape(-1)
         if hidden.is_cuda:
-            from ..engine import decoder
-
             with torch.cuda.device(hidden.device):
-                head = decoder.Head.of(hidden, weight, targets, ignore_index, first_word, words * world)
-                lse, picked = decoder.head_statistics(head)
-                if world > 1:
-                    lse = _join(lse, picked, group)
-                loss, counted = decoder.head_losses(head, lse, picked, reduction)
+                ctx.captured = torch.cuda.is_current_stream_capturing()
+                loss, lse = _device_loss(ctx, hidden, weight, targets, reduction, ignore_index, group, workspace_bytes,
+                                         *ctx.needs_input_grad[:2])
+            counted = None
         else:
-            head = _HostHead(hidden, weight, targets, ignore_index, first_word, words * world)
+            head = _HostHead(hidden, weight, targets, ignore_index, ctx.first_word, ctx.vocabulary)
             lse, picked = head.statistics()
-            if world > 1:
-                lse = _join(lse, picked, group)
+            if _world(group) > 1:
+                _join(lse, picked, group)
             loss, counted = head.losses(lse, picked, reduction)
         ctx.save_for_backward(hidden, weight, targets, lse, counted)
-        return loss
+        ctx.shape = (*shape, hidden.shape[-1])
+        return loss.view(shape) if reduction == "none" else loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
         hidden, weight, targets, lse, counted = ctx.saved_tensors
-        reduction, ignore_index, first_word, vocabulary, group, workspace_bytes = ctx.arguments
         want_hidden, want_weight = ctx.needs_input_grad[:2]
         if hidden.is_cuda:
-            from ..engine import decoder
-
             with torch.cuda.device(hidden.device):
-                head = decoder.Head.of(hidden, weight, targets, ignore_index, first_word, vocabulary)
-                d_hidden, d_weight = decoder.head_gradients(head, lse, reduction, grad_loss, counted, want_hidden, want_weight,
-                                                            workspace_bytes)
+                made, ctx.gradients = ctx.gradients, None
+                # handed over once: they are the caller's from then on.  A graph of the backward pass alone would scale them again at every replay.
+                if made is not None and ctx.captured == torch.cuda.is_current_stream_capturing():
+                    from ..engine import decoder
+
+                    decoder.scale_gradients(grad_loss.to(torch.float32), *made)
+                    d_hidden, d_weight = made
+                else:
+                    d_hidden, d_weight = _device_gradients(ctx, grad_loss, hidden, weight, targets, lse, want_hidden, want_weight)
         else:
-            head = _HostHead(hidden, weight, targets, ignore_index, first_word, vocabulary)
-            d_hidden, d_weight = (g.to(hidden.dtype) for g in head.gradients(lse, reduction, grad_loss, counted))
-        if want_hidden and _world(group) > 1:
-            dist.all_reduce(d_hidden, group=group)
-        return d_hidden if want_hidden else None, d_weight if want_weight else None, None, None, None, None, None
+            head = _HostHead(hidden, weight, targets, ctx.ignore_index, ctx.first_word, ctx.vocabulary)
+            d_hidden, d_weight = (g.to(hidden.dtype) for g in head.gradients(lse, ctx.reduction, grad_loss.reshape(-1) if
+                                                                             ctx.reduction == "none" else grad_loss, counted))
+        if want_hidden and _world(ctx.group) > 1:
+            dist.all_reduce(d_hidden, group=ctx.group)
+        return d_hidden.view(ctx.shape) if want_hidden else None, d_weight if want_weight else None, None, None, None, None, None
 
 
 def linear_cross_entropy(
@@ -160,12 +208,10 @@ def linear_cross_entropy(
     (256 tokens' at least) and, where the tokens need more than one turn, the weight's gradient in fp32.
     """
     _validate(hidden, weight, targets, reduction, workspace_bytes)
-    flat = hidden.reshape(-1, hidden.shape[-1])
-    if flat.shape[0] == 0:
-        loss = (flat.sum() + weight[:0].sum()).to(_wide(hidden.dtype))
+    if targets.numel() == 0:
+        loss = (hidden.sum() + weight[:0].sum()).to(_wide(hidden.dtype))
         return loss.expand(targets.shape) if reduction == "none" else loss
-    loss = _LinearCrossEntropy.apply(flat, weight, targets.reshape(-1), reduction, ignore_index, group, workspace_bytes)
-    return loss.view(targets.shape) if reduction == "none" else loss
+    return _LinearCrossEntropy.apply(hidden, weight, targets, reduction, ignore_index, group, workspace_bytes)
 
 
 __all__ = ["linear_cross_entropy"]

@@ -3,6 +3,8 @@
 ``u`` is half a step of the result's type (``eps / 2``); every bound is the rounding of the result, the roundings of what it is computed from in
 16 bits, and the errors of fp32 arithmetic, each times the magnitudes it acts on.
 """
+import math
+
 import torch
 
 IGNORED = -100
@@ -19,6 +21,8 @@ def head_exact(hidden, weight, targets, reduction, grad_loss=None, ignore_index=
     A logit is a sum of products that the tensor core adds with truncation, 2^-23 of the sum of magnitudes for each of the K / 16 additions at most:
     ``e`` bounds it.  exp, log and the joining of partial sums err by 2^-20 of one more.  The logits' gradient d has 16 bits (fp16: 2^-25 of
     its largest possible value, times 2^-15, below its normal numbers); its products add up with K / 16 truncated additions again.
+    bf16 gradients of a reduced loss are made from exponentials that were rounded once already (the target's entry is not), so that d has
+    two roundings, and an upstream gradient that is not a power of two rounds the results once more.
     """
     dtype = hidden.dtype
     u = half_step(dtype)
@@ -42,14 +46,16 @@ def head_exact(hidden, weight, targets, reduction, grad_loss=None, ignore_index=
     d[torch.arange(len(at), device=at.device), at] -= 1.0
     # a probability errs by its logit's and its lse's error, its rounding by u of what is stored
     # (and below 2^-126, the smallest normal fp32 number, it is taken as zero: exp(x) < 2^-126 errs by itself, at most 2^-126)
-    e_d = (p * (2 * e.unsqueeze(1) + 2.0 ** -19) + (u + 4 * F32) * d.abs() + 2.0 ** -126) * factor.abs()
+    with_loss = dtype == torch.bfloat16 and reduction != "none"
+    e_d = (p * (2 * e.unsqueeze(1) + 2.0 ** -19 + (u if with_loss else 0.0)) + (u + 4 * F32) * d.abs() + 2.0 ** -126) * factor.abs()
     if dtype == torch.float16:
         e_d = e_d + 2.0 ** -39 * factor.abs().max()
     d = d * factor
     d_hidden, d_weight = d @ w, d.t() @ h
 
     def bound(result, a, e_a, b, k):
-        return u * result.abs() + (e_a + (k // 16 + 2) * 2.0 ** -23 * a.abs()) @ b.abs() * (1 + u) + smallest(dtype)
+        roundings = 2 if with_loss and abs(math.log2(abs(upstream))) % 1 else 1
+        return roundings * u * result.abs() + (e_a + (k // 16 + 2) * 2.0 ** -23 * a.abs()) @ b.abs() * (1 + u) + smallest(dtype)
 
     e_hidden = bound(d_hidden, d, e_d, w, w.shape[0])
     e_weight = bound(d_weight, d.t(), e_d.t(), h, h.shape[0])

@@ -146,6 +146,47 @@ def test_cross_entropy_of_unusual_targets():
     _check_head(hidden, weight, torch.full_like(targets, 299))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("ignored", [0.02, 0.9, 0.99])
+def test_cross_entropy_leaves_padding_out(dtype, ignored):
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    hidden, weight, targets = _head(700, 60, 500, dtype, ignored=ignored)
+    targets[3], targets[5] = 17, IGNORED
+    spoilt = hidden.detach().clone()
+    spoilt[targets == IGNORED] = float("nan")
+    for reduction in ("mean", "none"):
+        _, expected = _check_head(hidden, weight, targets, reduction, workspace_bytes=1)
+        up = torch.rand(700, generator=torch.Generator("cuda").manual_seed(9), device="cuda") - 0.3 if reduction == "none" else None
+        leaf = spoilt.clone().requires_grad_()
+        loss = linear_cross_entropy(leaf, weight, targets, reduction=reduction, workspace_bytes=1)
+        for got, want in zip(torch.autograd.grad(loss, (leaf, weight), up), expected):
+            assert torch.equal(got, want)
+        assert not expected[0][targets == IGNORED].any()
+
+
+def test_cross_entropy_backward_pass_captured_alone():
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    hidden, weight, targets = _head(100, 64, 300, BF16)
+    up = torch.tensor(0.5, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(linear_cross_entropy(hidden, weight, targets), (hidden, weight), up)
+        loss = linear_cross_entropy(hidden, weight, targets)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grads = torch.autograd.grad(loss, (hidden, weight), up)
+    exact = head_exact(hidden, weight, targets, "mean", up)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        within(grads[0], exact[1])
+        within(grads[1], exact[2])
+
+
 def test_cross_entropy_of_large_logits():
     hidden, weight, targets = _head(64, 64, 300, BF16)
     big = (hidden.detach() * 40).requires_grad_()
