@@ -6,7 +6,7 @@
 // Tokens that do not count are left out from the start: the others' numbers, targets and hidden states are put one after another, every
 // product runs over those alone (their number stays on the device), and what the padding holds, NaN included, reaches nothing.
 //
-// The loss: one product (gemm16.cu) whose epilogue leaves, per token and 128 words, the largest logit and the sum of
+// The loss: one product (gemm16.cu) whose epilogue leaves, per token and 64 words, the largest logit and the sum of
 // exponentials relative to it; head_join_kernel joins these parts.  D goes through memory in 16 bits for a bounded number of tokens at a time, then
 // two products read it in both directions.  It comes about in one of two ways:
 //   * bf16 and one gradient of the loss for all tokens (mean, sum): the first product leaves the exponentials as well, one pass over them
@@ -55,10 +55,11 @@ __device__ __forceinline__ V block_reduce(V v, Op op, V* shared) {
 // One block: a thread takes a run of neighbouring tokens, counts, learns how many come before, and writes.
 __global__ void __launch_bounds__(kSingleThreads)
 head_count_kernel(const int64_t* __restrict__ targets, int tokens, int64_t ignored, int64_t first_word, int words, int64_t vocabulary,
-                  int* __restrict__ count, int* __restrict__ where, int* __restrict__ column) {
+                  int* __restrict__ count, int* __restrict__ where, int* __restrict__ column, int* __restrict__ split_counters) {
   __shared__ int warps[32];
   wait_for_predecessor();
   let_successor_start();
+  for (int i = threadIdx.x; i < kSplitCounters; i += kSingleThreads) split_counters[i] = 0;
   const int each = (tokens + kSingleThreads - 1) / kSingleThreads;
   const int begin = min(tokens, static_cast<int>(threadIdx.x) * each), end = min(tokens, begin + each);
   int mine = 0;
@@ -118,14 +119,21 @@ __global__ void head_gather_kernel(const uint16_t* __restrict__ hidden, int64_t 
 }
 
 // 32 tokens a block, lanes along tokens, the parts dealt to 16 warps and joined in a fixed order.
+//
+// The target's logit is then computed anew in fp32, a warp to a token: where the tensor core's truncation makes all large logits a little too small
+// (5e-6 of themselves at K = 4096), a loss, which is a difference from the target's, would be off by 2e-6 of its own size.
+template <typename T>
 __global__ void __launch_bounds__(32 * kJoinSlices)
 head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number, const int* __restrict__ count, int first, int rows,
-                 const int* __restrict__ column, float* __restrict__ lse, float* __restrict__ picked) {
+                 const int* __restrict__ column, const T* __restrict__ all, int64_t ld_all, int tokens, const T* __restrict__ packed, int64_t ld_packed,
+                 const T* __restrict__ weight, int64_t ld_weight, int depth, float* __restrict__ lse, float* __restrict__ picked) {
   __shared__ float2 shared[kJoinSlices][32];
+  __shared__ float exact[32];
   wait_for_predecessor();
   let_successor_start();
+  const int counted = *count;
   const int token = blockIdx.x * 32 + threadIdx.x;
-  const bool here = token < min(rows, *count - first);
+  const bool here = token < min(rows, counted - first);
   float largest = -INFINITY, sum = 0.f;
   auto join = [&](const float2 part) {
     const float most = fmaxf(largest, part.x);
@@ -138,12 +146,41 @@ head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number,
     for (int i = threadIdx.y; i < number; i += kJoinSlices) join(parts[i * ld_parts + token]);
   }
   shared[threadIdx.y][threadIdx.x] = make_float2(largest, sum);
+#pragma unroll
+  for (int i = 0; i < 32 / kJoinSlices; ++i) {
+    const int which = threadIdx.y + i * kJoinSlices, other = blockIdx.x * 32 + which;
+    const int word = other < min(rows, counted - first) ? column[first + other] : -1;
+    if (word < 0) continue;                // (the whole warp)
+    const T* h = counted == tokens ? all + (first + other) * ld_all : packed + (first + other) * ld_packed;
+    const T* w = weight + word * ld_weight;
+    float dot = 0.f;
+    for (int run = threadIdx.x; run < depth / 8; run += 32) {      // (rows lie on 16-byte boundaries)
+      Eight<T> a, b;
+      a.load(h + 8 * run);
+      b.load(w + 8 * run);
+      float u[8], v[8];
+      a.get(u);
+      b.get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot = fmaf(u[j], v[j], dot);
+    }
+    for (int j = depth / 8 * 8 + threadIdx.x; j < depth; j += 32) dot = fmaf(to_float(h[j]), to_float(w[j]), dot);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (threadIdx.x == 0) exact[which] = dot;
+  }
   __syncthreads();
   if (threadIdx.y == 0 && here) {
 #pragma unroll
     for (int s = 1; s < kJoinSlices; ++s) join(shared[s][threadIdx.x]);
-    lse[first + token] = logf(sum) + (largest == -INFINITY ? 0.f : largest);
-    if (column[first + token] < 0) picked[first + token] = 0.f;
+    const float base = largest == -INFINITY ? 0.f : largest;
+    float target = 0.f;
+    if (column[first + token] >= 0) {
+      target = exact[threadIdx.x];
+      sum = sum - exp2f((picked[first + token] - base) * kLog2e) + exp2f((target - base) * kLog2e);
+    }
+    lse[first + token] = logf(sum) + base;
+    picked[first + token] = target;
   }
 }
 
@@ -301,7 +338,7 @@ Gemm16Problem logits_of(const HeadProblem& p, const LogitRows& r) {
 
 void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaStream_t stream) {
   check(launch_dependent(head_count_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.targets, p.tokens, p.ignore_index, p.first_word,
-                         p.words, p.vocabulary, p.count, p.where, p.column),
+                         p.words, p.vocabulary, p.count, p.where, p.column, p.split_counters),
         "head_count");
   const int blocks = std::min((p.tokens + 7) / 8, 8 * sms_of_device());
   check(launch_dependent(head_gather_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<const uint16_t*>(p.hidden.data), p.hidden.ld,
@@ -315,9 +352,16 @@ void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float
   g.picked = picked + r.first;
   const Hidden16 hidden = hidden_of(p, r.first);
   gemm16(r.logits ? kLogitExponential : kLogitStatistics, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
-  check(launch_dependent(head_join_kernel, dim3((r.rows + 31) / 32), dim3(32, kJoinSlices), 0, stream, r.parts,
-                         static_cast<int64_t>(r.rows), (p.words + kLogitPart - 1) / kLogitPart, p.count, r.first, r.rows, p.column, lse, picked),
-        "head_join");
+  auto join = [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    check(launch_dependent(head_join_kernel<T>, dim3((r.rows + 31) / 32), dim3(32, kJoinSlices), 0, stream, r.parts,
+                           static_cast<int64_t>(r.rows), (p.words + kLogitPart - 1) / kLogitPart, p.count, r.first, r.rows, p.column,
+                           static_cast<const T*>(p.hidden.data), p.hidden.ld, p.tokens, static_cast<const T*>(p.packed.data), p.packed.ld,
+                           static_cast<const T*>(p.weight.data), p.weight.ld, p.depth, lse, picked),
+          "head_join");
+  };
+  if (p.bf16) join(static_cast<__nv_bfloat16*>(nullptr));
+  else join(static_cast<__half*>(nullptr));
 }
 
 void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, cudaStream_t stream) {
@@ -368,6 +412,7 @@ void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha
     d.count = p.count; d.first = r.first;
     d.C = out.hidden; d.ldc = out.ld_hidden; d.where = p.where + r.first;
     d.alpha = alpha;
+    d.split_parts = out.split_parts; d.split_counters = p.split_counters;
     gemm16(kStore16, p.bf16, Matrix16{r.logits, r.ld_logits, true}, Matrix16{p.weight.data, p.weight.ld, false}, d, status, stream);
   }
   if (out.weight) {
@@ -376,6 +421,7 @@ void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha
     d.count = p.count; d.first = r.first;
     d.alpha = alpha;
     d.accumulator = out.sum; d.ld_accumulator = out.ld_sum; d.add = r.first > 0;
+    d.split_parts = out.split_parts; d.split_counters = p.split_counters;
     if (last) {
       d.C = out.weight; d.ldc = out.ld_weight;
     }

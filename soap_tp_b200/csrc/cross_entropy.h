@@ -22,15 +22,16 @@ struct HeadProblem {
   int* count;               // [1]
   int* where;               // [tokens]
   int* column;              // [tokens]
+  int* split_counters;      // [kSplitCounters], cleared with them
   Matrix16 packed;          // [tokens][depth]
 };
 constexpr int kElsewhere = -1, kUnknown = -2;
 
-// Fills count, where, column and packed; with `d_hidden`, clears the rows of the tokens that do not count.
+// Fills count, where, column, split_counters and packed; with `d_hidden`, clears the rows of the tokens that do not count.
 void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaStream_t stream);
 
 // For tokens first .. first + rows of those that count: lse[i] = log sum_j exp(l_ij) over this rank's words, picked[i] = l_i,t_i where the
-// target is one of them and 0 elsewhere.  `parts`: ceil(words / 128) x rows pairs.  With `logits` (bf16) the exponentials stay
+// target is one of them and 0 elsewhere.  `parts`: ceil(words / kLogitPart) x rows pairs.  With `logits` (bf16) the exponentials stay
 // there, each relative to the largest of its part.
 struct LogitRows {
   int first, rows;
@@ -62,6 +63,7 @@ struct HeadGradients {
   int64_t ld_weight;
   float* sum;
   int64_t ld_sum;
+  float* split_parts;       // kSplitScratch floats
 };
 void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha, const HeadGradients& g, int* status, cudaStream_t stream);
 

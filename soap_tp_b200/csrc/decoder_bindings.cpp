@@ -70,7 +70,8 @@ HeadProblem head_problem(Reader& in) {
   p.bf16 = in.next() != 0;
   p.targets = in.pointer<int64_t>();
   p.ignore_index = in.next(); p.first_word = in.next(); p.vocabulary = in.next();
-  p.count = in.pointer<int>(); p.where = p.count + 1; p.column = p.where + p.tokens;      // 1 + 2 * tokens integers
+  p.count = in.pointer<int>(); p.where = p.count + 1; p.column = p.where + p.tokens;
+  p.split_counters = p.column + p.tokens;      // 1 + 2 * tokens + kSplitCounters integers
   p.packed.data = in.pointer<void>(); p.packed.ld = in.next(); p.packed.k_major = true;
   return p;
 }
@@ -138,6 +139,7 @@ void register_decoder(py::module_& m) {
     g.hidden = in.pointer<void>(); g.ld_hidden = in.next();
     g.weight = in.pointer<void>(); g.ld_weight = in.next();
     g.sum = in.pointer<float>(); g.ld_sum = in.next();
+    g.split_parts = in.pointer<float>();
     auto* status = in.pointer<int>(); auto stream = in.stream();
     in.finish();
     if (picked) head_rescale(p, r, lse, picked, factor, stream);
@@ -163,6 +165,7 @@ void register_decoder(py::module_& m) {
     Gemm16Problem p{};
     p.M = in.size(); p.N = in.size(); p.K = in.size();
     p.C = in.pointer<void>(); p.ldc = in.next();
+    p.split_parts = in.pointer<float>(); p.split_counters = in.pointer<int>();
     auto* status = in.pointer<int>(); auto stream = in.stream();
     in.finish();
     gemm16(kStore16, bf16, a, b, p, status, stream);
@@ -240,4 +243,7 @@ void register_decoder(py::module_& m) {
   });
   m.def("residual_norm_blocks", &residual_norm_blocks);
   m.attr("SCALE_GROUP") = kScaleGroup;
+  m.attr("LOGIT_PART") = kLogitPart;
+  m.attr("SPLIT_COUNTERS") = kSplitCounters;
+  m.attr("SPLIT_SCRATCH") = kSplitScratch;
 }

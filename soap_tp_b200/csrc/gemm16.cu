@@ -3,21 +3,22 @@
 // A persistent kernel of clusters of two CTAs, one CTA per SM; a pair takes 256 x 256 tiles one after another:
 //   warp 0, one lane : TMA producer - this CTA's 128 rows of A and its 128 of the tile's 256 rows of B, 64 of K, per stage of 32 KB
 //   warp 1, one lane : MMA issuer (leader CTA) - M 256 x N 256 x K 16, cta_group::2
-//   warps 4..11      : epilogue - each a quarter of the CTA's 128 rows and half of the columns, 128 sums a thread; their two warpgroups
-//                      take the registers that the first one (two of whose warps are idle) gives back
+//   warps 4..        : epilogue - each a quarter of the CTA's 128 rows; logits: sixteen warps of 64 columns, products: eight of 128.  Their
+//                      warpgroups take the registers that the first one (two of whose warps are idle) gives back
 // The accumulator takes 256 of TMEM's 512 columns, so that the epilogue of a tile runs beside the products of the next.
 // Operands whose M or N runs along memory's rows go in as they lie (kUmmaMnMajorA, kUmmaMnMajorB): the gradients' products
 // read the logits' gradient in both directions, and no matrix is transposed.
 //
-// The tensor core truncates as it adds: 2^-24 of the running sum per 16 of K on average.  Logits are drained from TMEM into sums in registers
-// (round to nearest) every 256 of K, or 512 for the first two drains of a tile, while the previous tile's epilogue still runs: a loss is then
-// off by some 5e-7 of itself where one sum over K = 4096 was off by 2e-6.  Gradients are drained once: 5e-4 of one over 128256
-// words at most, a quarter of what its rounding to bf16 costs.
+// The tensor core truncates as it adds: some 2^-24 of the running sum per 16 of K.  Logits are drained from TMEM into sums in registers (round
+// to nearest) every 2048 of K, gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
+// Draining every 256 of K costs 150 of 690 thousand cycles at 4096 x 16032 x 4096: handing the accumulator over takes the tensor core about
+// 700 cycles, whatever the epilogue does meanwhile.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -36,15 +37,21 @@ constexpr int kBK = 64;                          // one 128-byte swizzle row of 
 constexpr int kOperandBytes = kRows * kBK * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kStages = 6;
-constexpr int kEpiWarps = 8;
+constexpr int kStagingBytes = 32 * 1024;
+constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
 constexpr int kFirstEpiWarp = 4;
-constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
-// 384 threads are launched with 168 registers each, 64512 together; 128 * 40 + 256 * 224 = 62464.
-constexpr int kFewRegisters = 40, kManyRegisters = 224;
-constexpr int kWarpStaging = 32 * 128;           // 32 rows of 128 bytes
-constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kWarpStaging + 1024 + 256;
-constexpr int kWarpColumns = kTile / 2;          // of the tile, per epilogue thread
-static_assert(kWarpColumns == kLogitPart, "an epilogue thread's columns are one part of its row");
+// What the two kinds of epilogue have.  `kFew` and `kMany`: registers of a thread of the first warpgroup and of the others, once shared
+// out; together they are what the block is launched with, 640 * 96 or (less than) 384 * 168.
+template <bool LOGITS>
+struct Epi {
+  static constexpr int kWarps = LOGITS ? 16 : 8;
+  static constexpr int kThreads = 32 * (kFirstEpiWarp + kWarps);
+  static constexpr int kColumns = kTile / (kWarps / 4);      // of the tile, per thread
+  static constexpr int kStaging = kStagingBytes / kWarps;    // 32 rows of 64 or 128 bytes
+  static constexpr int kFew = LOGITS ? 32 : 40, kMany = LOGITS ? 112 : 224;
+};
+static_assert(Epi<true>::kColumns == kLogitPart, "an epilogue thread's logits are one part of its row");
+static_assert(128 * 32 + 512 * 112 <= 640 * 96 && 128 * 40 + 256 * 224 <= 384 * 168, "registers to share out");
 constexpr int kGroup = 8;                        // tile rows that share their tiles of B in L2 while they sweep the columns
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -78,21 +85,25 @@ struct Tiles {
   }
 };
 
-// 32 rows of 128 bytes, one per lane, to 32 rows of a matrix: staged in shared memory (16-byte words swizzled by row, so that
-// neither side has bank conflicts) and stored with whole 128-byte lines.  Row i is row where[first + i] of `base`, or first + i;
+// 32 rows of LINE bytes, one per lane, to 32 rows of a matrix: staged in shared memory (16-byte words swizzled by row, so that
+// neither side has bank conflicts) and stored LINE bytes at a time.  Row i is row where[first + i] of `base`, or first + i;
 // `valid` bytes of each row are inside the matrix.
-__device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&words)[32], uint8_t* base, int64_t pitch, const int* where,
+template <int LINE>
+__device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&words)[LINE / 4], uint8_t* base, int64_t pitch, const int* where,
                                             int first, int rows, int valid, int element, bool wide, int lane) {
+  constexpr int kChunks = LINE / 16;                   // of a row
+  const int turn = kChunks == 8 ? lane : lane >> 1;    // (eight lanes that store together hit all banks)
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    *reinterpret_cast<uint4*>(staging + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+  for (int c = 0; c < kChunks; ++c)
+    *reinterpret_cast<uint4*>(staging + lane * LINE + ((c ^ (turn & (kChunks - 1))) << 4)) =
         make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2], words[4 * c + 3]);
   __syncwarp();
-  const int chunk = lane & 7;
+  const int chunk = lane & (kChunks - 1);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = 4 * i + (lane >> 3);
-    const uint4 v = *reinterpret_cast<const uint4*>(staging + row * 128 + ((chunk ^ (row & 7)) << 4));
+  for (int i = 0; i < kChunks; ++i) {
+    const int row = (32 / kChunks) * i + lane / kChunks;
+    const int row_turn = kChunks == 8 ? row : row >> 1;
+    const uint4 v = *reinterpret_cast<const uint4*>(staging + row * LINE + ((chunk ^ (row_turn & (kChunks - 1))) << 4));
     if (row < rows) {
       uint8_t* dst = base + (where ? where[first + row] : first + row) * pitch + chunk * 16;
       const int left = valid - chunk * 16;
@@ -115,98 +126,102 @@ __device__ __forceinline__ void store_lines(uint8_t* staging, const uint32_t (&w
   __syncwarp();
 }
 
-// Lines of 64 16-bit values whose row i goes to row where[i] of a matrix.
-template <typename T>
-__device__ __forceinline__ void store_values(uint8_t* staging, const uint32_t (&words)[32], const Gemm16Problem& p, int m_warp, int column,
+// 32 rows of 16-bit values, from `column` of C on.
+template <int LINE>
+__device__ __forceinline__ void store_values(uint8_t* staging, const uint32_t (&words)[LINE / 4], const Gemm16Problem& p, int m_warp, int column,
                                              int rows, int cols, bool wide, int lane) {
-  store_lines(staging, words, reinterpret_cast<uint8_t*>(p.C) + static_cast<int64_t>(column) * 2, p.ldc * 2, p.where, m_warp, rows, 2 * min(64, cols), 2, wide, lane);
+  store_lines<LINE>(staging, words, reinterpret_cast<uint8_t*>(p.C) + static_cast<int64_t>(column) * 2, p.ldc * 2, p.where, m_warp, rows,
+                    min(LINE, 2 * cols), 2, wide, lane);
 }
 
-// An epilogue thread's 128 logits of one token.
+// An epilogue thread's logits of one token, as pairs of neighbouring columns.
 template <int EPI, typename T>
-__device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, float (&v)[kWarpColumns], int M, int m_warp, int n0, uint8_t* staging, int lane) {
+__device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t (&sums)[kLogitPart / 2], int M, int m_warp, int n0,
+                                                uint8_t* staging, int lane) {
   const int row = m_warp + lane;
   const bool inside = row < M;
-  const int cols = min(kWarpColumns, p.N - n0);           // of this thread's part; may be negative
+  const int cols = min(kLogitPart, p.N - n0);             // of this thread's part; may be negative
   // (the gradient's rows up to the next multiple of 64 are cleared: they are read as part of K)
   const int rows = min(32, (EPI == kLogitGradient ? min(p.M, (M + kBK - 1) / kBK * kBK) : M) - m_warp);
   const int target = inside ? p.targets[row] - n0 : -1;
-  if constexpr (EPI == kLogitGradient) {
-    const float base = inside ? p.lse[row] * kLog2e : 0.f, factor = inside ? p.factor[row] : 0.f;
+  const uint64_t scale = pack_floats(kLog2e, kLog2e);
+  auto store = [&](auto value) {                          // value(j): the 16-bit result's column j
 #pragma unroll
-    for (int c = 0; c < kWarpColumns; c += 64) {
-      uint32_t words[32];
+    for (int c = 0; c < kLogitPart; c += 32) {
+      uint32_t words[16];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) {
-        const float e = exp2_fast(fmaf(v[c + j], kLog2e, -base));
-        v[c + j] = inside ? (target == c + j ? e - 1.f : e) * factor : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 32; ++j) words[j] = pack16<T>(v[c + 2 * j], v[c + 2 * j + 1]);
-      if (rows > 0 && c < cols) store_values<T>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
+      for (int j = 0; j < 16; ++j) words[j] = pack16<T>(value(c + 2 * j), value(c + 2 * j + 1));
+      if (rows > 0 && c < cols) store_values<64>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
     }
-  } else {
-    if (cols < kWarpColumns) {
+  };
+  // sums become the exponents of two that their exponentials are
+  auto exponents = [&](float base) {
+    const uint64_t shift = pack_floats(-base, -base);
 #pragma unroll
-      for (int j = 0; j < kWarpColumns; ++j)
-        if (j >= cols) v[j] = -INFINITY;
+    for (int j = 0; j < kLogitPart / 2; ++j) {
+      uint64_t v = shift;
+      fma_pair(v, sums[j], scale);
+      sums[j] = v;
+    }
+  };
+  auto value = [&](int j) { return pair_element(sums[j / 2], j & 1); };
+  if constexpr (EPI == kLogitGradient) {
+    const float factor = inside ? p.factor[row] : 0.f;
+    exponents(inside ? p.lse[row] * kLog2e : 0.f);
+    store([&](int j) {
+      const float e = exp2_fast(value(j));
+      return inside ? (target == j ? e - 1.f : e) * factor : 0.f;
+    });
+  } else {
+    if (cols < kLogitPart) {
+#pragma unroll
+      for (int j = 0; j < kLogitPart; j += 2)
+        sums[j / 2] = pack_floats(j < cols ? value(j) : -INFINITY, j + 1 < cols ? value(j + 1) : -INFINITY);
     }
     if (inside && target >= 0 && target < cols) {
       float picked = 0.f;
 #pragma unroll
-      for (int j = 0; j < kWarpColumns; ++j)
-        if (target == j) picked = v[j];
+      for (int j = 0; j < kLogitPart; ++j)
+        if (target == j) picked = value(j);
       p.picked[row] = picked;
     }
-    float most[4] = {v[0], v[1], v[2], v[3]};
+    float most[4] = {value(0), value(1), value(2), value(3)};
 #pragma unroll
-    for (int j = 4; j < kWarpColumns; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
+    for (int j = 4; j < kLogitPart; ++j) most[j & 3] = fmaxf(most[j & 3], value(j));
     const float largest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
     // (a row of no finite logit is taken relative to zero, so that its sum is zero, or NaN where a logit is)
-    const float base = largest == -INFINITY ? 0.f : largest * kLog2e;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    exponents(largest == -INFINITY ? 0.f : largest * kLog2e);
+    uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < kWarpColumns; ++j) {
-      v[j] = exp2_fast(fmaf(v[j], kLog2e, -base));
-      sum[j & 3] += v[j];
+    for (int j = 0; j < kLogitPart; j += 2) {
+      sums[j / 2] = pack_floats(exp2_fast(value(j)), exp2_fast(value(j + 1)));
+      add_pair(sum[(j >> 1) & 1], sums[j / 2]);
     }
+    add_pair(sum[0], sum[1]);
     if (inside && cols > 0)
-      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.ld_parts + row] = make_float2(largest, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-    if constexpr (EPI == kLogitExponential) {
-#pragma unroll
-      for (int c = 0; c < kWarpColumns; c += 64) {
-        uint32_t words[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) words[j] = pack16<T>(v[c + 2 * j], v[c + 2 * j + 1]);
-        if (rows > 0 && c < cols) store_values<T>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
-      }
-    }
+      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.ld_parts + row] = make_float2(largest, pair_element(sum[0], 0) + pair_element(sum[0], 1));
+    if constexpr (EPI == kLogitExponential) store(value);
   }
 }
 
-// An epilogue thread's row of a product; `taddr` is the first of its 128 columns.  `empty`: nothing was added up.
-template <typename T>
-__device__ __forceinline__ void product_epilogue(const Gemm16Problem& p, uint32_t taddr, bool empty, int M, int m_warp, int n0, uint8_t* staging, int lane) {
+// An epilogue thread's row of a product.  values(at, raw): its 32 sums from column `at` of its 128 on.
+template <typename T, typename Values>
+__device__ __forceinline__ void product_epilogue(const Gemm16Problem& p, int M, int m_warp, int n0, uint8_t* staging, int lane, Values values) {
   const int row = m_warp + lane;
   const bool inside = row < M;
-  const int cols = min(kWarpColumns, p.N - n0);
+  const int cols = min(Epi<false>::kColumns, p.N - n0);
   const int rows = min(32, M - m_warp);
   const float alpha = p.alpha ? *p.alpha : 1.f;
   const bool to16 = p.C != nullptr;
   const bool wide = (reinterpret_cast<uintptr_t>(p.C) & 15) == 0 && (p.ldc & 7) == 0;
 #pragma unroll
-  for (int c = 0; c < kWarpColumns; c += 64) {
+  for (int c = 0; c < Epi<false>::kColumns; c += 64) {
     uint32_t words[32];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t raw[32];
       const int at = c + 32 * h;
-      tmem_ld_32x32(taddr + at, raw);
-      tmem_ld_wait();
-      if (empty) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) raw[j] = 0;
-      }
+      values(at, raw);
       if (p.add && inside && at < cols) {
         const float* old = p.accumulator + row * p.ld_accumulator + n0 + at;
 #pragma unroll
@@ -223,28 +238,62 @@ __device__ __forceinline__ void product_epilogue(const Gemm16Problem& p, uint32_
         for (int j = 0; j < 16; ++j)
           words[16 * h + j] = pack16<T>(alpha * __uint_as_float(raw[2 * j]), alpha * __uint_as_float(raw[2 * j + 1]));
       } else if (rows > 0 && at < cols) {
-        store_lines(staging, raw, reinterpret_cast<uint8_t*>(p.accumulator + n0 + at), p.ld_accumulator * 4, nullptr, m_warp, rows, 128, 4, true, lane);
+        store_lines<128>(staging, raw, reinterpret_cast<uint8_t*>(p.accumulator + n0 + at), p.ld_accumulator * 4, nullptr, m_warp, rows, 128, 4, true, lane);
       }
     }
-    if (to16 && rows > 0 && c < cols) store_values<T>(staging, words, p, m_warp, n0 + c, rows, cols - c, wide, lane);
+    if (to16 && rows > 0 && c < cols) store_values<128>(staging, words, p, m_warp, n0 + c, rows, cols - c, wide, lane);
   }
 }
 
-// K-blocks that the accumulator takes before its drain number `d` of a tile.
+// What a pair does one after another: whole tiles, and where the last round has fewer tiles than there are pairs, parts of tiles' K, so
+// that no pair is idle while others take a whole tile.  (A head's gradient of 4096 x 4096 hidden states is 256 tiles, 3.46 rounds of 74 pairs.)
+struct Units {
+  int tiles, whole, split, k_blocks;
+  __device__ __forceinline__ Units(int tiles_, int k_blocks_, int pairs, bool may_split) : tiles(tiles_), whole(tiles_), split(1), k_blocks(k_blocks_) {
+    const int rest = tiles % pairs;
+    if (may_split && rest) {
+      split = max(1, min(min(pairs, kSplitUnits) / rest, min(kMostSplit, k_blocks / kLeastBlocks)));
+      if (split > 1) whole = tiles - rest;
+    }
+  }
+  __device__ __forceinline__ int count() const { return whole + (tiles - whole) * split; }
+  // tile, and first and last k-block, of a unit; its number among the parts of the split tiles, or -1
+  __device__ __forceinline__ void place(int unit, int& tile, int& begin, int& end, int& part) const {
+    tile = unit;
+    begin = 0;
+    end = k_blocks;
+    part = -1;
+    if (unit >= whole) {
+      part = unit - whole;
+      tile = whole + part / split;
+      const int64_t which = part % split;
+      begin = static_cast<int>(which * k_blocks / split);
+      end = static_cast<int>((which + 1) * k_blocks / split);
+    }
+  }
+  static constexpr int kLeastBlocks = 8;      // of a part: its sums go through memory once more
+  static constexpr int kMostSplit = 16;
+};
+
+// K-blocks that the accumulator takes before it is drained, `left` of them remaining.
+constexpr int kDrainBlocks = 2048 / kBK;
 template <bool LOGITS>
-__device__ __forceinline__ int drain_blocks(int d, int left) {
-  return LOGITS ? min(left, d < 2 ? 8 : 4) : left;
+__device__ __forceinline__ int drain_blocks(int left) {
+  if (!LOGITS || left <= kDrainBlocks) return left;
+  const int drains = (left + kDrainBlocks - 1) / kDrainBlocks;      // of about the same size
+  return (left + drains - 1) / drains;
 }
 
 template <int EPI, bool A_K, bool B_K, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Epi<EPI != kStore16>::kThreads, 1)
 gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_all,
               int all_tokens, const __grid_constant__ Gemm16Problem prob, int* status) {
   constexpr bool kLogits = EPI != kStore16;
+  using E = Epi<kLogits>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + kStages * kStageBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kWarpStaging);      // used in the leader CTA only
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + kStagingBytes);      // used in the leader CTA only
   uint64_t* empty_bar = full_bar + kStages;         // each CTA its own: "my stage may be refilled"
   uint64_t* acc_full = empty_bar + kStages;         // [2] each CTA its own: tensor core -> epilogue
   uint64_t* acc_empty = acc_full + 2;               // [2] leader's only: epilogue warps of both CTAs -> tensor core
@@ -263,7 +312,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * kEpiWarps);
+      mbar_init(&acc_empty[b], 2 * E::kWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -292,20 +341,22 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
   }
   const Tiles tiles(M, prob.N);
   const int k_blocks = (K + kBK - 1) / kBK;
+  const Units units(tiles.count(), k_blocks, clusters, !kLogits && prob.split_parts);
 
   if (warp < kFirstEpiWarp) {
-    give_registers_back<kFewRegisters>();
+    give_registers_back<E::kFew>();
     if (warp == 0 && lane == 0) {
       // ---------------- TMA producer (each CTA its own rows; the bytes are credited to the leader) ----------------
       int s = 0;
       uint32_t parity = 1;
       bool first_round = true, ok = true;
-      for (int t = cluster; t < tiles.count() && ok; t += clusters) {
-        int m0, n0;
-        tiles.place(t, m0, n0);
+      for (int u = cluster; u < units.count() && ok; u += clusters) {
+        int m0, n0, tile, begin, end, part;
+        units.place(u, tile, begin, end, part);
+        tiles.place(tile, m0, n0);
         m0 += cta * kRows;
         n0 += cta * kRows;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = begin; kb < end; ++kb) {
           if (!first_round && !mbar_wait_bounded(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) {
             ok = false;
             break;
@@ -345,18 +396,23 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
       uint32_t parity = 0;
       bool ok = true;
       int it = 0;                                // drains so far
-      for (int t = cluster; t < tiles.count() && ok; t += clusters) {
-        for (int d = 0, kb = 0; kb < k_blocks && ok; ++d, ++it) {
+      // Whether the next k-block's operands and the next accumulator are there is looked up while this k-block's products are still being
+      // issued: a wait, however short, drains the tensor core's queue of a few products.
+      bool loaded = false, drained = false;
+      for (int u = cluster; u < units.count() && ok; u += clusters) {
+        int tile, begin, end, part;
+        units.place(u, tile, begin, end, part);
+        for (int kb = begin; kb < end && ok; ++it) {
           const int buf = it & 1;
-          if (it >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
+          if (it >= 2 && !drained && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
           const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
-          const int blocks = drain_blocks<kLogits>(d, k_blocks - kb);
+          const int blocks = drain_blocks<kLogits>(end - kb);
           for (int i = 0; i < blocks; ++i, ++kb) {
-            if (!mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
+            if (!loaded && !mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
               ok = false;
               break;
             }
@@ -365,7 +421,14 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             const uint64_t a = A_K ? umma_desc_kmajor<128>(stage) : umma_desc_mn_major(stage);
             const uint64_t b = B_K ? umma_desc_kmajor<128>(stage + kOperandBytes) : umma_desc_mn_major(stage + kOperandBytes);
   #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) umma_f16_ss_pair(acc, a + k * kStepA, b + k * kStepB, kIdesc, i | k ? 1u : 0u);
+            for (int k = 0; k < kBK / 16; ++k) {
+              umma_f16_ss_pair(acc, a + k * kStepA, b + k * kStepB, kIdesc, i | k ? 1u : 0u);
+              if (k == 1) {
+                const int next = s + 1 == kStages ? 0 : s + 1;
+                loaded = mbar_test(&full_bar[next], next ? parity : parity ^ 1);
+                drained = it >= 1 && mbar_test(&acc_empty[buf ^ 1], (((it + 1) >> 1) - 1) & 1);
+              }
+            }
             umma_commit_pair(&empty_bar[s]);
             if (++s == kStages) {
               s = 0;
@@ -377,11 +440,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
       }
     }
   } else {
-    take_registers<kManyRegisters>();
+    take_registers<E::kMany>();
     // ---------------- epilogue (each CTA its own 128 rows) ----------------
     const int ew = warp - kFirstEpiWarp;
     const int quarter = warp & 3;              // TMEM lane quarter this warp may read
-    const int col0 = (ew >> 2) * kWarpColumns;
+    const int col0 = (ew >> 2) * E::kColumns;
+    uint8_t* mine = staging + ew * E::kStaging;
     const uint32_t drained = map_to_cta(smem_u32(&acc_empty[0]), 0);
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(col0);
     int it = 0;
@@ -396,35 +460,86 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
       if (lane == 0) mbar_arrive_cluster(drained + static_cast<uint32_t>((it & 1) * sizeof(uint64_t)));
       ++it;
     };
-    for (int t = cluster; t < tiles.count(); t += clusters) {
-      int m0, n0;
-      tiles.place(t, m0, n0);
+    for (int u = cluster; u < units.count(); u += clusters) {
+      int m0, n0, tile, begin, end, part;
+      units.place(u, tile, begin, end, part);
+      tiles.place(tile, m0, n0);
       const int m_warp = m0 + cta * kRows + quarter * 32;
       if constexpr (kLogits) {
-        float v[kWarpColumns];
+        uint64_t sums[kLogitPart / 2];         // pairs of neighbouring columns
+#pragma unroll
+        for (int j = 0; j < kLogitPart / 2; ++j) sums[j] = 0;
         bool ok = true;
-        for (int d = 0, kb = 0; kb < k_blocks; ++d) {
-          kb += drain_blocks<true>(d, k_blocks - kb);
+        for (int kb = 0; kb < k_blocks;) {
+          kb += drain_blocks<true>(k_blocks - kb);
           ok = filled();
           if (!ok) break;
           const uint32_t from = taddr + static_cast<uint32_t>((it & 1) * kTile);
 #pragma unroll
-          for (int c = 0; c < kWarpColumns; c += 32) {
-            uint32_t raw[32];
-            tmem_ld_32x32(from + c, raw);
+          for (int c = 0; c < kLogitPart; c += 16) {
+            uint32_t raw[16];
+            tmem_ld_32x16(from + c, raw);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[c + j] = d ? v[c + j] + __uint_as_float(raw[j]) : __uint_as_float(raw[j]);
+            for (int j = 0; j < 8; ++j) add_pair(sums[c / 2 + j], pack_pair(raw[2 * j], raw[2 * j + 1]));
           }
           release();
         }
         if (!ok) break;
-        logits_epilogue<EPI, T>(prob, v, M, m_warp, n0 + col0, staging + ew * kWarpStaging, lane);
+        logits_epilogue<EPI, T>(prob, sums, M, m_warp, n0 + col0, mine, lane);
       } else {
-        const bool empty = k_blocks == 0;
+        const bool empty = k_blocks == 0;      // (nothing was added up)
         if (!empty && !filled()) break;
-        product_epilogue<T>(prob, taddr + static_cast<uint32_t>((it & 1) * kTile), empty, M, m_warp, n0 + col0, staging + ew * kWarpStaging, lane);
-        if (!empty) release();
+        const uint32_t from = taddr + static_cast<uint32_t>((it & 1) * kTile);
+        auto accumulated = [&](int at, uint32_t (&raw)[32]) {
+          tmem_ld_32x32(from + at, raw);
+          tmem_ld_wait();
+          if (empty) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) raw[j] = 0;
+          }
+        };
+        if (part < 0) {
+          product_epilogue<T>(prob, M, m_warp, n0 + col0, mine, lane, accumulated);
+          if (!empty) release();
+        } else {
+          // This part's sums, 256 x 256 of them a part; the warp that is the last to leave its region of the tile adds the parts up in order.
+          const int row = cta * kRows + quarter * 32;
+          const int first = (tile - units.whole) * units.split;
+#pragma unroll
+          for (int at = 0; at < E::kColumns; at += 32) {
+            uint32_t raw[32];
+            accumulated(at, raw);
+            store_lines<128>(mine, raw, reinterpret_cast<uint8_t*>(prob.split_parts + part * int64_t{kTile * kTile} + col0 + at), kTile * 4, nullptr,
+                             row, 32, 128, 4, true, lane);
+          }
+          release();
+          __threadfence();
+          __syncwarp();
+          int* counter = prob.split_counters + ((tile - units.whole) * 2 + cta) * E::kWarps + ew;
+          int before = 0;
+          if (lane == 0) before = atomicAdd(counter, 1);
+          before = __shfl_sync(0xffffffffu, before, 0);
+          if (before == units.split - 1) {
+            if (lane == 0) *counter = 0;
+            __threadfence();
+            product_epilogue<T>(prob, M, m_warp, n0 + col0, mine, lane, [&](int at, uint32_t (&raw)[32]) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) raw[j] = 0;
+              for (int i = 0; i < units.split; ++i) {
+                const float* from_part = prob.split_parts + (first + i) * int64_t{kTile * kTile} + (row + lane) * kTile + col0 + at;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                  const float4 v = __ldcg(reinterpret_cast<const float4*>(from_part + j));
+                  raw[j] = __float_as_uint(__uint_as_float(raw[j]) + v.x);
+                  raw[j + 1] = __float_as_uint(__uint_as_float(raw[j + 1]) + v.y);
+                  raw[j + 2] = __float_as_uint(__uint_as_float(raw[j + 2]) + v.z);
+                  raw[j + 3] = __float_as_uint(__uint_as_float(raw[j + 3]) + v.w);
+                }
+              }
+            });
+          }
+        }
       }
     }
   }
@@ -460,8 +575,10 @@ void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* s
   const CUtensorMap map_all = !hidden ? map_a : EPI != kStore16 ? map_of(kBf16, hidden->all, p.M, p.K) : map_of(kBf16, hidden->all, p.N, p.K);
   const int64_t tiles = static_cast<int64_t>((p.M + kTile - 1) / kTile) * ((p.N + kTile - 1) / kTile);
   if (tiles > (1 << 30)) throw std::invalid_argument("gemm16: too many tiles");
-  const int clusters = static_cast<int>(tiles < pairs_of_device() ? tiles : pairs_of_device());
-  cudaError_t err = launch_dependent(gemm16_kernel<EPI, A_K, B_K, T>, dim3(2 * clusters), dim3(kThreads), kSmemBytes, stream, map_a,
+  // (where tokens are left out there may be fewer tiles in the end than here, and more parts of one)
+  const int64_t parts = p.split_parts ? std::max(1, std::min(Units::kMostSplit, (p.K + kBK - 1) / kBK / Units::kLeastBlocks)) : 1;
+  const int clusters = static_cast<int>(std::min<int64_t>(tiles * parts, pairs_of_device()));
+  cudaError_t err = launch_dependent(gemm16_kernel<EPI, A_K, B_K, T>, dim3(2 * clusters), dim3(Epi<EPI != kStore16>::kThreads), kSmemBytes, stream, map_a,
                                      map_b, map_all, hidden ? hidden->tokens : -1, p, status);
   if (err != cudaSuccess) throw std::runtime_error(std::string("gemm16 launch: ") + cudaGetErrorString(err));
 }
@@ -489,6 +606,8 @@ void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix1
   if (epilogue == kStore16 && (p.add || !p.C) && (!p.accumulator || p.ld_accumulator % 32 != 0 || p.ld_accumulator < p.N ||
                                                   (reinterpret_cast<uintptr_t>(p.accumulator) & 15) != 0))
     throw std::invalid_argument("gemm16: the accumulator's pitch is a multiple of 32 covering the columns");
+  if ((p.split_parts == nullptr) != (p.split_counters == nullptr) || (reinterpret_cast<uintptr_t>(p.split_parts) & 15) != 0)
+    throw std::invalid_argument("gemm16: split tiles need aligned room for their parts and counters");
   if (epilogue == kLogitExponential) {
     if (!bf16 || !a.k_major || !b.k_major) throw std::invalid_argument("gemm16: exponentials are kept in bf16, of K-major operands");
     launch<kLogitExponential, true, true, __nv_bfloat16>(a, b, p, status, stream, hidden);

@@ -15,13 +15,13 @@ struct Matrix16 {
 };
 
 enum Gemm16Epilogue : int {
-  kLogitStatistics = 0,     // largest logit and sum of exponentials per row and 128 columns, and the logit of each row's target
+  kLogitStatistics = 0,     // largest logit and sum of exponentials per row and 64 columns, and the logit of each row's target
   kLogitExponential = 1,    // the same, and the exponentials themselves, relative to the largest of their part, as a 16-bit matrix
   kLogitGradient = 2,       // softmax minus target, times the row's factor, as a 16-bit matrix
   kStore16 = 3,             // the product itself
 };
 
-constexpr int kLogitPart = 128;      // columns that share one partial maximum and sum
+constexpr int kLogitPart = 64;      // columns that share one partial maximum and sum
 
 struct Gemm16Problem {
   int M, N, K;
@@ -45,7 +45,14 @@ struct Gemm16Problem {
   float* accumulator;       // [M][ld_accumulator]
   int64_t ld_accumulator;
   bool add;                 // whether the accumulator holds something
+  // kStore16: where tiles whose K is split leave their parts (kSplitScratch floats), and how many have (kSplitCounters zeros, left as
+  // zeros); null: no tile is split
+  float* split_parts;
+  int* split_counters;
 };
+constexpr int kSplitUnits = 80;                       // parts of tiles at most: one for each CTA pair of the device
+constexpr int64_t kSplitScratch = kSplitUnits * int64_t{256} * 256;
+constexpr int kSplitCounters = kSplitUnits * 16;
 
 // The hidden states in two places: the tokens that count one after another, and all of them (`all`, of `tokens` rows), which is where
 // they are read from when every token counts.

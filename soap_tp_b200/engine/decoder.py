@@ -15,7 +15,7 @@ from . import kernels as k
 from .kernels import _C
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-LOGIT_PART = 128          # words that share one partial maximum and sum
+LOGIT_PART, SPLIT_COUNTERS, SPLIT_SCRATCH = _C.LOGIT_PART, _C.SPLIT_COUNTERS, _C.SPLIT_SCRATCH
 
 
 def _rows16(x: Tensor) -> Tensor:
@@ -38,7 +38,7 @@ class Head:
         self.tokens, self.depth, self.words = hidden.shape[0], hidden.shape[1], weight.shape[0]
         self.device, self.dtype = hidden.device, hidden.dtype
         # how many tokens count, which they are and their targets' columns; their hidden states, used unless all count
-        self.numbers_of = torch.empty(1 + 2 * self.tokens, dtype=torch.int32, device=self.device)
+        self.numbers_of = torch.empty(1 + 2 * self.tokens + SPLIT_COUNTERS, dtype=torch.int32, device=self.device)
         self.packed = torch.empty((self.tokens, k.round_up(self.depth, 8)), dtype=self.dtype, device=self.device)
         self.problem = [self.hidden.data_ptr(), self.hidden.stride(0), self.weight.data_ptr(), self.weight.stride(0), self.tokens, self.depth,
                         self.words, int(self.dtype == torch.bfloat16), self.targets.data_ptr(), ignore_index, first_word, vocabulary,
@@ -87,6 +87,7 @@ class HeadGradients:
         several = want_weight and self.rows < head.tokens
         self.sum = torch.empty((head.words, k.round_up(head.depth, 32)), dtype=torch.float32, device=device) if several else None
         self.factor = torch.empty(1 + head.tokens, dtype=torch.float32, device=device)      # alpha, then a factor for each token
+        self.split_parts = torch.empty(SPLIT_SCRATCH, dtype=torch.float32, device=device)
 
     def turns(self):
         for first in range(0, self.head.tokens, self.rows):
@@ -104,7 +105,8 @@ class HeadGradients:
             first, rows, self.logits.data_ptr(), self.logits.shape[1], 0 if parts is None else parts.data_ptr(), lse.data_ptr(),
             0 if picked is None else picked.data_ptr(), alpha + 4, alpha,
             0 if self.hidden is None else self.hidden.data_ptr(), head.depth, 0 if self.weight is None else self.weight.data_ptr(), head.depth,
-            0 if self.sum is None else self.sum.data_ptr(), 0 if self.sum is None else self.sum.shape[1], head.status, k._stream()])
+            0 if self.sum is None else self.sum.data_ptr(), 0 if self.sum is None else self.sum.shape[1],
+            self.split_parts.data_ptr(), head.status, k._stream()])
         k._count("head_rescale_kernel" if parts is not None else "gemm16_kernel")
         for wanted in (self.hidden, self.weight):
             if wanted is not None:

@@ -24,8 +24,10 @@ def _no_timeouts():
 # ---- products on 16-bit operands ----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("k_major", [True, False])
-@pytest.mark.parametrize("m,n,k", [(1, 8, 1), (128, 256, 64), (256, 256, 128), (130, 72, 200), (513, 300, 65), (300, 1000, 2000), (2600, 2300, 96)])
-def test_gemm16(m, n, k, k_major, dtype):
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 1), (128, 256, 64), (256, 256, 128), (130, 72, 200), (513, 300, 65), (300, 1000, 2000), (2600, 2300, 1096),
+                                   (100, 700, 30000)])
+def test_gemm16(m, n, k, k_major, dtype, split):
     from soap_tp_b200.engine import kernels
 
     def padded(rows, cols, seed):
@@ -34,13 +36,16 @@ def test_gemm16(m, n, k, k_major, dtype):
     a = padded(m, k, 1) if k_major else padded(k, m, 1)
     b = padded(k, n, 2)
     c = torch.full((m + 1, n + 3), 7.0, dtype=dtype, device="cuda")
+    parts = torch.full((kernels._C.SPLIT_SCRATCH,), float("nan"), device="cuda")
+    counters = torch.zeros(kernels._C.SPLIT_COUNTERS, dtype=torch.int32, device="cuda")
     kernels._C.gemm16_store(dtype == BF16, k_major, [a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), m, n, k, c.data_ptr(), c.stride(0),
+                                                     parts.data_ptr() if split else 0, counters.data_ptr() if split else 0,
                                                      kernels.status_word(a.device).data_ptr(), kernels._stream()])
     x = a.double() if k_major else a.double().t()
     exact = x @ b.double()
     bound = half_step(dtype) * exact.abs() + (k // 16 + 2) * 2.0 ** -23 * (x.abs() @ b.double().abs()) + smallest(dtype)
     within(c[:m, :n], (exact, bound))
-    assert bool((c[m] == 7).all()) and bool((c[:, n:] == 7).all())
+    assert bool((c[m] == 7).all()) and bool((c[:, n:] == 7).all()) and not counters.any()
 
 
 # ---- cross entropy ------------------------------------------------------------------------------------------------------
