@@ -15,7 +15,6 @@
 #include <vector>
 
 #include "comm.h"
-#include "decoder.h"
 #include "elementwise.h"
 #include "gemm.h"
 #include "gemm_half.h"
@@ -497,5 +496,4 @@ PYBIND11_MODULE(_C, m) {
   m.attr("QR_MAX_ROWS") = kQrMaxRows;
 
   register_comm(m);
-  register_decoder(m);
 }

@@ -65,11 +65,17 @@ __device__ __forceinline__ float group_scale(const float (&v)[8]) {
   return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(most) / 127.f, kSmallestScale);
 }
 
+// 16-bit values are multiplied by the reciprocal, whose rounding can move what lies within 2^-16 of a step from a tie to the other side;
+// fp32 values, which come back exactly but for their step, are divided.
+template <typename T>
 __device__ __forceinline__ uint2 quantise(const float (&v)[8], float scale) {
-  const float inverse = 1.f / scale;       // the quotient's rounding moves ties and values next to them by a step at most
+  const float inverse = 1.f / scale;
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i / 4] |= (static_cast<uint32_t>(__float2int_rn(v[i] * inverse)) & 0xffu) << (8 * (i & 3));
+  for (int i = 0; i < 8; ++i) {
+    const float quotient = std::is_same<T, float>::value ? v[i] / scale : v[i] * inverse;
+    w[i / 4] |= (static_cast<uint32_t>(__float2int_rn(quotient)) & 0xffu) << (8 * (i & 3));
+  }
   return make_uint2(w[0], w[1]);
 }
 
@@ -79,10 +85,11 @@ __device__ __forceinline__ void dequantise(uint2 q, float scale, float (&v)[8]) 
   for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i & 3)))) * scale;
 }
 
+template <typename T>
 __device__ __forceinline__ void keep(const Kept8& kept, const Shape& shape, const Place& p, bool here, int lane8, const float (&v)[8]) {
   const float scale = group_scale(v);
   if (!here) return;
-  if (p.valid > 0) *reinterpret_cast<uint2*>(kept.values + p.row * kept.pitch + p.column) = quantise(v, scale);
+  if (p.valid > 0) *reinterpret_cast<uint2*>(kept.values + p.row * kept.pitch + p.column) = quantise<T>(v, scale);
   if (lane8 == 0) kept.scales[p.row * shape.groups + p.group] = scale;
 }
 
@@ -109,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x
   const bool here = shape.place(first_group(), lane8, p);
   float v[8];
   read_eight(x + p.row * ld + p.column, here ? p.valid : 0, wide, v);
-  keep(kept, shape, p, here, lane8, v);
+  keep<T>(kept, shape, p, here, lane8, v);
 }
 
 template <typename T>
@@ -137,8 +144,8 @@ swiglu8_forward_kernel(const T* __restrict__ gate, int64_t ld_gate, const T* __r
   read_eight(gate + p.row * ld_gate + p.column, valid, wide, g);
   read_eight(up + p.row * ld_up + p.column, valid, wide, u);
   if (KEEP) {
-    keep(gate8, shape, p, here, lane8, g);
-    keep(up8, shape, p, here, lane8, u);
+    keep<T>(gate8, shape, p, here, lane8, g);
+    keep<T>(up8, shape, p, here, lane8, u);
   }
   if (valid <= 0) return;
 #pragma unroll

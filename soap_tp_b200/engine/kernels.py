@@ -38,6 +38,7 @@ STATUS_MESSAGES = {
 }
 
 LAUNCH_COUNTS: Dict[str, int] = {}
+LAUNCHES_ELSEWHERE: list = []      # functions that return how many kernels other native modules have launched
 
 
 def _count(name: str) -> None:
@@ -46,7 +47,7 @@ def _count(name: str) -> None:
 
 def total_launches() -> int:
     """Number of kernels of this library launched by this process so far."""
-    return sum(LAUNCH_COUNTS.values())
+    return sum(LAUNCH_COUNTS.values()) + sum(launches() for launches in LAUNCHES_ELSEWHERE)
 
 
 class SoapKernelError(RuntimeError):

@@ -12,6 +12,8 @@ Results of the forward pass are those of exact activations; gradients are those 
 """
 from __future__ import annotations
 
+import functools
+import math
 from typing import Callable, Iterable, NamedTuple, Tuple
 
 import torch
@@ -36,6 +38,17 @@ class Packed8(NamedTuple):
         return self.values.numel() + 4 * self.scales.numel()
 
 
+@functools.cache
+def _native():
+    from ..engine import decoder
+
+    return decoder.native
+
+
+def _on_device(x: Tensor) -> bool:
+    return x.is_cuda and x.numel() > 0
+
+
 def _check_values(name: str, x: Tensor) -> None:
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name} must be (..., features), got {tuple(x.shape)}.")
@@ -57,43 +70,30 @@ def _host_unpack(values: Tensor, scales: Tensor, dim: int, dtype: torch.dtype) -
     return (values[:, :dim].float() * scales.repeat_interleave(GROUP, dim=1)[:, :dim]).to(dtype)
 
 
-def _pack(x: Tensor) -> Tuple[Tensor, Tensor]:
-    if x.is_cuda and x.numel() > 0:
-        from ..engine import decoder
-
-        with torch.cuda.device(x.device):
-            return decoder.pack8(x)
-    return _host_pack(x)
-
-
-def _unpack(values: Tensor, scales: Tensor, dim: int, dtype: torch.dtype) -> Tensor:
-    if values.is_cuda and values.numel() > 0:
-        from ..engine import decoder
-
-        with torch.cuda.device(values.device):
-            return decoder.unpack8(decoder.Kept8(values, scales), dim, dtype)
-    return _host_unpack(values, scales, dim, dtype)
-
-
-@torch.no_grad()
 def pack8(x: Tensor) -> Packed8:
-    """``x`` (..., features) in 8 bits."""
+    """``x`` (..., features) in 8 bits; no gradients."""
     _check_values("x", x)
-    return Packed8(*_pack(x.reshape(-1, x.shape[-1])), x.shape, x.dtype)
+    if _on_device(x):
+        values, scales = _native().pack8(x)
+    else:
+        values, scales = _host_pack(x.detach().reshape(-1, x.shape[-1]))
+    return Packed8(values, scales, x.shape, x.dtype)
 
 
-@torch.no_grad()
 def unpack8(packed: Packed8) -> Tensor:
     """The values that ``packed`` stands for, in the dtype it was made from."""
-    rows, dim = packed.values.shape[0], packed.shape[-1]
-    groups = -(-dim // GROUP)
-    if packed.shape.numel() != rows * dim or packed.values.shape != (rows, -(-dim // 8) * 8) or packed.scales.shape != (rows, groups):
-        raise ValueError(f"values {tuple(packed.values.shape)} and scales {tuple(packed.scales.shape)} do not hold a tensor of shape {tuple(packed.shape)}.")
-    if packed.values.dtype != torch.int8 or packed.scales.dtype != torch.float32 or packed.dtype not in DTYPES:
-        raise TypeError(f"values are int8 and scales float32, got {packed.values.dtype} and {packed.scales.dtype} for {packed.dtype}.")
-    if packed.values.device != packed.scales.device:
-        raise ValueError(f"values and scales must be on one device, got {packed.values.device} and {packed.scales.device}.")
-    return _unpack(packed.values.contiguous(), packed.scales.contiguous(), dim, packed.dtype).view(packed.shape)
+    values, scales, shape, dtype = packed
+    rows, dim = values.shape[0], shape[-1]
+    if math.prod(shape) != rows * dim or values.shape != (rows, -(-dim // 8) * 8) or scales.shape != (rows, -(-dim // GROUP)):
+        raise ValueError(f"values {tuple(values.shape)} and scales {tuple(scales.shape)} do not hold a tensor of shape {tuple(shape)}.")
+    if values.dtype != torch.int8 or scales.dtype != torch.float32 or dtype not in DTYPES:
+        raise TypeError(f"values are int8 and scales float32, got {values.dtype} and {scales.dtype} for {dtype}.")
+    if values.device != scales.device:
+        raise ValueError(f"values and scales must be on one device, got {values.device} and {scales.device}.")
+    values, scales = values.contiguous(), scales.contiguous()
+    if _on_device(values):
+        return _native().unpack8(values, scales, shape, dtype)
+    return _host_unpack(values, scales, dim, dtype).view(shape)
 
 
 class _Checkpoint8(torch.autograd.Function):
@@ -151,64 +151,42 @@ def _check_swiglu(gate: Tensor, up: Tensor) -> None:
         raise ValueError(f"gate and up must match, got {tuple(gate.shape)} {gate.dtype} {gate.device} and {tuple(up.shape)} {up.dtype} {up.device}.")
 
 
-def _swiglu_forward(gate: Tensor, up: Tensor, keep: bool):
-    if gate.is_cuda and gate.numel() > 0:
-        from ..engine import decoder
-
-        with torch.cuda.device(gate.device):
-            y, gate8, up8 = decoder.swiglu8_forward(gate, up, keep)
-        return y, (*gate8, *up8) if keep else ()
-    return (F.silu(gate.float()) * up.float()).to(gate.dtype), (*_host_pack(gate), *_host_pack(up)) if keep else ()
+def _host_swiglu(gate: Tensor, up: Tensor) -> Tensor:
+    return (F.silu(gate.float()) * up.float()).to(gate.dtype)
 
 
-def _swiglu_backward(grad: Tensor, kept, with_y: bool):
-    if grad.is_cuda and grad.numel() > 0:
-        from ..engine import decoder
-
-        with torch.cuda.device(grad.device):
-            return decoder.swiglu8_backward(grad, decoder.Kept8(*kept[:2]), decoder.Kept8(*kept[2:]), with_y)
+def _host_swiglu_gradients(grad: Tensor, kept) -> Tuple[Tensor, Tensor, Tensor]:
+    """Gradients of gate and up, and the activation, at the kept values."""
     dim = grad.shape[1]
     g, u = _host_unpack(kept[0], kept[1], dim, torch.float32), _host_unpack(kept[2], kept[3], dim, torch.float32)
     s, d = torch.sigmoid(g), grad.float()
-    return ((d * u * s * (1.0 + g * (1.0 - s))).to(grad.dtype), (d * g * s).to(grad.dtype), (g * s * u).to(grad.dtype) if with_y else None)
+    return (d * u * s * (1.0 + g * (1.0 - s))).to(grad.dtype), (d * g * s).to(grad.dtype), (g * s * u).to(grad.dtype)
 
 
 class _SwiGLU8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate, up):
-        y, kept = _swiglu_forward(gate, up, keep=True)
-        ctx.save_for_backward(*kept)
-        return y
+    """CPU tensors: with a weight, the linear layer behind it too."""
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        return _swiglu_backward(grad, ctx.saved_tensors, with_y=False)[:2]
-
-
-class _SwiGLULinear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, weight):
-        y, kept = _swiglu_forward(gate, up, keep=True)
-        ctx.save_for_backward(weight, *kept)
-        return F.linear(y, weight)
+        ctx.save_for_backward(weight, *_host_pack(gate), *_host_pack(up))
+        y = _host_swiglu(gate, up)
+        return y if weight is None else F.linear(y, weight)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         weight, *kept = ctx.saved_tensors
-        want_weight = ctx.needs_input_grad[2]
-        d_gate, d_up, y = _swiglu_backward(grad @ weight, kept, with_y=want_weight)
-        return d_gate, d_up, grad.t() @ y if want_weight else None
+        d_gate, d_up, y = _host_swiglu_gradients(grad if weight is None else grad @ weight, kept)
+        return d_gate, d_up, grad.t() @ y if ctx.needs_input_grad[2] else None
 
 
 def swiglu8(gate: Tensor, up: Tensor) -> Tensor:
     """``silu(gate) * up``; the backward pass works from both kept in 8 bits.  Differentiable once."""
     _check_swiglu(gate, up)
-    flat = (gate.reshape(-1, gate.shape[-1]), up.reshape(-1, up.shape[-1]))
-    if not torch.is_grad_enabled() or not (gate.requires_grad or up.requires_grad):
-        return _swiglu_forward(*flat, keep=False)[0].view(gate.shape)
-    return _SwiGLU8.apply(*flat).view(gate.shape)
+    if _on_device(gate):
+        return _native().swiglu8(gate, up)
+    dim = gate.shape[-1]
+    return _SwiGLU8.apply(gate.reshape(-1, dim), up.reshape(-1, dim), None).view(gate.shape)
 
 
 def swiglu_linear8(gate: Tensor, up: Tensor, weight: Tensor) -> Tensor:
@@ -216,12 +194,10 @@ def swiglu_linear8(gate: Tensor, up: Tensor, weight: Tensor) -> Tensor:
     _check_swiglu(gate, up)
     if weight.ndim != 2 or weight.shape[1] != gate.shape[-1] or weight.dtype != gate.dtype or weight.device != gate.device:
         raise ValueError(f"weight must be (out, {gate.shape[-1]}) {gate.dtype} on {gate.device}, got {tuple(weight.shape)} {weight.dtype} on {weight.device}.")
-    flat = (gate.reshape(-1, gate.shape[-1]), up.reshape(-1, up.shape[-1]))
-    if not torch.is_grad_enabled() or not (gate.requires_grad or up.requires_grad or weight.requires_grad):
-        out = F.linear(_swiglu_forward(*flat, keep=False)[0], weight)
-    else:
-        out = _SwiGLULinear8.apply(*flat, weight)
-    return out.view(*gate.shape[:-1], weight.shape[0])
+    if _on_device(gate):
+        return _native().swiglu_linear8(gate, up, weight)
+    dim = gate.shape[-1]
+    return _SwiGLU8.apply(gate.reshape(-1, dim), up.reshape(-1, dim), weight).view(*gate.shape[:-1], weight.shape[0])
 
 
 __all__ = ["Packed8", "checkpoint8", "pack8", "swiglu8", "swiglu_linear8", "unpack8"]

@@ -13,6 +13,7 @@ log-sum-exp and the target's logit are joined over the group, and the gradient o
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -23,30 +24,42 @@ from torch.autograd.function import once_differentiable
 REDUCTIONS = ("none", "sum", "mean")
 
 
+_ON_CUDA = (torch.bfloat16, torch.float16)
+_ON_CPU = (torch.bfloat16, torch.float16, torch.float32, torch.float64)
+
+
+@functools.cache
+def _native():
+    from ..engine import decoder
+
+    return decoder
+
+
 def _validate(hidden: Tensor, weight: Tensor, targets: Tensor, reduction: str, workspace_bytes: int) -> None:
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {REDUCTIONS}, got {reduction!r}.")
-    if hidden.ndim < 1 or weight.ndim != 2:
-        raise ValueError(f"hidden must be (..., depth) and weight (words, depth), got {tuple(hidden.shape)} and {tuple(weight.shape)}.")
-    if hidden.shape[-1] != weight.shape[1]:
-        raise ValueError(f"hidden has depth {hidden.shape[-1]} and weight {weight.shape[1]}.")
-    if targets.shape != hidden.shape[:-1]:
-        raise ValueError(f"targets must have shape {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}.")
+    shape, words = hidden.shape, weight.shape
+    if len(shape) < 1 or len(words) != 2:
+        raise ValueError(f"hidden must be (..., depth) and weight (words, depth), got {tuple(shape)} and {tuple(words)}.")
+    if shape[-1] != words[1]:
+        raise ValueError(f"hidden has depth {shape[-1]} and weight {words[1]}.")
+    if targets.shape != shape[:-1]:
+        raise ValueError(f"targets must have shape {tuple(shape[:-1])}, got {tuple(targets.shape)}.")
     if targets.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"targets must be int64 or int32, got {targets.dtype}.")
     if hidden.dtype != weight.dtype:
         raise TypeError(f"hidden and weight must have one dtype, got {hidden.dtype} and {weight.dtype}.")
-    if weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"weight must not be empty, got {tuple(weight.shape)}.")
-    if hidden.device != weight.device or hidden.device != targets.device:
-        raise ValueError(f"hidden, weight and targets must be on one device, got {hidden.device}, {weight.device} and {targets.device}.")
-    allowed = (torch.bfloat16, torch.float16) if hidden.is_cuda else (torch.bfloat16, torch.float16, torch.float32, torch.float64)
+    if words[0] < 1 or words[1] < 1:
+        raise ValueError(f"weight must not be empty, got {tuple(words)}.")
+    device = hidden.device
+    if device != weight.device or device != targets.device:
+        raise ValueError(f"hidden, weight and targets must be on one device, got {device}, {weight.device} and {targets.device}.")
+    allowed = _ON_CUDA if hidden.is_cuda else _ON_CPU
     if hidden.dtype not in allowed:
-        raise TypeError(f"on {hidden.device.type} hidden and weight must be one of {allowed}, got {hidden.dtype}.")
+        raise TypeError(f"on {device.type} hidden and weight must be one of {allowed}, got {hidden.dtype}.")
     if workspace_bytes < 1:
         raise ValueError(f"workspace_bytes must be positive, got {workspace_bytes}.")
-    largest = 2**31 - 1
-    if weight.shape[0] > largest or weight.shape[1] > largest or targets.numel() > largest:
+    if max(words[0], words[1], targets.numel()) >= 2**31:
         raise ValueError("tokens, words and depth must each be below 2**31.")
 
 
@@ -54,7 +67,7 @@ def _world(group) -> int:
     return 1 if group is None else dist.get_world_size(group)
 
 
-def _join(lse: Tensor, picked: Tensor, group) -> None:
+def _join(group, lse: Tensor, picked: Tensor) -> None:
     """``lse`` becomes that over all ranks' words, ``picked`` the target's logit on every rank (both in place)."""
     every = [torch.empty_like(lse) for _ in range(_world(group))]
     dist.all_gather(every, lse, group=group)
@@ -99,94 +112,51 @@ class _HostHead:
         return d @ self.weight, d.t() @ self.hidden
 
 
-def _device_loss(ctx, hidden, weight, targets, reduction, ignore_index, group, workspace_bytes, want_hidden, want_weight):
-    """The loss and each counted token's log-sum-exp; where the gradients can come with it they are left in ``ctx.gradients``."""
-    from ..engine import decoder
-
-    head = decoder.Head(hidden, weight, targets, ignore_index, ctx.first_word, ctx.vocabulary)
-    lse, picked = torch.empty((2, head.tokens), dtype=torch.float32, device=head.device)
-    shared = _world(group) > 1
-    # bf16 only: fp16 gradients are rounded after the loss's scale, which the backward pass brings, has been multiplied in
-    if (want_hidden or want_weight) and reduction != "none" and head.dtype == torch.bfloat16:
-        gradients = decoder.HeadGradients(head, want_hidden, want_weight, workspace_bytes)
-        head.prepare(gradients.hidden)
-        gradients.factors(reduction, None)
-        parts = head.parts(gradients.rows)
-        for first, rows in gradients.turns():
-            head.statistics(first, rows, parts, lse, picked, gradients.logits)
-            if shared:
-                _join(lse[first:first + rows], picked[first:first + rows], group)
-            gradients.add(first, rows, lse, parts, picked)
-        ctx.gradients = (gradients.hidden, gradients.weight)
-    else:
-        head.prepare()
-        head.statistics(0, head.tokens, head.parts(head.tokens), lse, picked)
-        if shared:
-            _join(lse, picked, group)
-    return head.loss(lse, picked, reduction), lse
-
-
-def _device_gradients(ctx, grad_loss, hidden, weight, targets, lse, want_hidden, want_weight):
-    from ..engine import decoder
-
-    head = decoder.Head(hidden, weight, targets, ctx.ignore_index, ctx.first_word, ctx.vocabulary)
-    gradients = decoder.HeadGradients(head, want_hidden, want_weight, ctx.workspace_bytes)
-    head.prepare(gradients.hidden)
-    gradients.factors(ctx.reduction, grad_loss.to(torch.float32).contiguous())
-    for first, rows in gradients.turns():
-        gradients.add(first, rows, lse)
-    return gradients.hidden, gradients.weight
-
-
 class _LinearCrossEntropy(torch.autograd.Function):
+    """CPU tensors."""
+
     @staticmethod
-    def forward(ctx, hidden, weight, targets, reduction, ignore_index, group, workspace_bytes):
-        words = weight.shape[0]
-        ctx.first_word = 0 if group is None else dist.get_rank(group) * words
-        ctx.vocabulary = words * _world(group)
-        ctx.reduction, ctx.ignore_index, ctx.group, ctx.workspace_bytes = reduction, ignore_index, group, workspace_bytes
-        ctx.gradients = None
+    def forward(ctx, hidden, weight, targets, reduction, ignore_index, group):
+        words, world = weight.shape[0], _world(group)
+        first_word = 0 if group is None else dist.get_rank(group) * words
+        ctx.arguments = (ignore_index, first_word, words * world)
+        ctx.reduction, ctx.shape = reduction, hidden.shape
         shape = targets.shape
         hidden, targets = hidden.detach().reshape(-1, hidden.shape[-1]), targets.reshape(-1)
-        if hidden.is_cuda:
-            with torch.cuda.device(hidden.device):
-                ctx.captured = torch.cuda.is_current_stream_capturing()
-                loss, lse = _device_loss(ctx, hidden, weight, targets, reduction, ignore_index, group, workspace_bytes,
-                                         *ctx.needs_input_grad[:2])
-            counted = None
-        else:
-            head = _HostHead(hidden, weight, targets, ignore_index, ctx.first_word, ctx.vocabulary)
-            lse, picked = head.statistics()
-            if _world(group) > 1:
-                _join(lse, picked, group)
-            loss, counted = head.losses(lse, picked, reduction)
+        head = _HostHead(hidden, weight, targets, *ctx.arguments)
+        lse, picked = head.statistics()
+        if world > 1:
+            _join(group, lse, picked)
+        loss, counted = head.losses(lse, picked, reduction)
         ctx.save_for_backward(hidden, weight, targets, lse, counted)
-        ctx.shape = (*shape, hidden.shape[-1])
         return loss.view(shape) if reduction == "none" else loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
         hidden, weight, targets, lse, counted = ctx.saved_tensors
-        want_hidden, want_weight = ctx.needs_input_grad[:2]
-        if hidden.is_cuda:
-            with torch.cuda.device(hidden.device):
-                made, ctx.gradients = ctx.gradients, None
-                # handed over once: they are the caller's from then on.  A graph of the backward pass alone would scale them again at every replay.
-                if made is not None and ctx.captured == torch.cuda.is_current_stream_capturing():
-                    from ..engine import decoder
+        head = _HostHead(hidden, weight, targets, *ctx.arguments)
+        if ctx.reduction == "none":
+            grad_loss = grad_loss.reshape(-1)
+        d_hidden, d_weight = (g.to(hidden.dtype) for g in head.gradients(lse, ctx.reduction, grad_loss, counted))
+        wanted = ctx.needs_input_grad
+        return d_hidden.view(ctx.shape) if wanted[0] else None, d_weight if wanted[1] else None, None, None, None, None
 
-                    decoder.scale_gradients(grad_loss.to(torch.float32), *made)
-                    d_hidden, d_weight = made
-                else:
-                    d_hidden, d_weight = _device_gradients(ctx, grad_loss, hidden, weight, targets, lse, want_hidden, want_weight)
-        else:
-            head = _HostHead(hidden, weight, targets, ctx.ignore_index, ctx.first_word, ctx.vocabulary)
-            d_hidden, d_weight = (g.to(hidden.dtype) for g in head.gradients(lse, ctx.reduction, grad_loss.reshape(-1) if
-                                                                             ctx.reduction == "none" else grad_loss, counted))
-        if want_hidden and _world(ctx.group) > 1:
-            dist.all_reduce(d_hidden, group=ctx.group)
-        return d_hidden.view(ctx.shape) if want_hidden else None, d_weight if want_weight else None, None, None, None, None, None
+
+class _SumGradient(torch.autograd.Function):
+    """Hidden states that every rank of a group has: each rank's words give a part of their gradient."""
+
+    @staticmethod
+    def forward(ctx, hidden, group):
+        ctx.group = group
+        return hidden.view_as(hidden)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        grad = grad.contiguous()
+        dist.all_reduce(grad, group=ctx.group)
+        return grad, None
 
 
 def linear_cross_entropy(
@@ -211,7 +181,15 @@ def linear_cross_entropy(
     if targets.numel() == 0:
         loss = (hidden.sum() + weight[:0].sum()).to(_wide(hidden.dtype))
         return loss.expand(targets.shape) if reduction == "none" else loss
-    return _LinearCrossEntropy.apply(hidden, weight, targets, reduction, ignore_index, group, workspace_bytes)
+    world = _world(group)
+    if world > 1:
+        hidden = _SumGradient.apply(hidden, group)
+    if not hidden.is_cuda:
+        return _LinearCrossEntropy.apply(hidden, weight, targets, reduction, ignore_index, group)
+    decoder, words = _native(), weight.shape[0]
+    return decoder.native.linear_cross_entropy(
+        hidden, weight, targets, decoder.REDUCTIONS[reduction], ignore_index, 0 if group is None else dist.get_rank(group) * words, words * world,
+        workspace_bytes, decoder.status(hidden.device), functools.partial(_join, group) if world > 1 else None)
 
 
 __all__ = ["linear_cross_entropy"]

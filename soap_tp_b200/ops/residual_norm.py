@@ -6,35 +6,47 @@ over memory, forward and backward; :func:`rms_norm` is the norm alone.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 LONGEST_ROW = 32768
+_ON_CUDA = (torch.bfloat16, torch.float16, torch.float32)
+_ON_CPU = (*_ON_CUDA, torch.float64)
 
 
-def _validate(x: Tensor, branch: Optional[Tensor], vectors: dict, scale: float, eps: float) -> None:
-    if x.ndim < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must be (..., dim), got {tuple(x.shape)}.")
-    allowed = (torch.bfloat16, torch.float16, torch.float32) + (() if x.is_cuda else (torch.float64,))
-    if x.dtype not in allowed:
-        raise TypeError(f"on {x.device.type} x must be one of {allowed}, got {x.dtype}.")
-    if x.is_cuda and x.shape[-1] > LONGEST_ROW:
-        raise ValueError(f"rows of more than {LONGEST_ROW} values are not supported on CUDA, got {x.shape[-1]}.")
-    if branch is not None and (branch.shape != x.shape or branch.dtype != x.dtype or branch.device != x.device):
-        raise ValueError(f"branch must match x: {tuple(x.shape)} {x.dtype} {x.device}, got {tuple(branch.shape)} {branch.dtype} {branch.device}.")
-    given = {name: v for name, v in vectors.items() if v is not None}
-    for name, v in given.items():
-        if v.shape != x.shape[-1:] or v.device != x.device:
-            raise ValueError(f"{name} must have shape {tuple(x.shape[-1:])} on {x.device}, got {tuple(v.shape)} on {v.device}.")
-        if v.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"{name} must be {x.dtype} or float32, got {v.dtype}.")
-    if len({v.dtype for v in given.values()}) > 1:
-        raise TypeError(f"{', '.join(given)} must have one dtype, got {[v.dtype for v in given.values()]}.")
-    if branch is None and any(given.get(name) is not None for name in ("branch_weight", "gate")):
-        raise ValueError("branch_weight and gate need a branch.")
+@functools.cache
+def _native():
+    from ..engine import decoder
+
+    return decoder.native
+
+
+def _validate(x: Tensor, branch: Optional[Tensor], weight: Optional[Tensor], branch_weight: Optional[Tensor], gate: Optional[Tensor],
+              scale: float, eps: float) -> None:
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"x must be (..., dim), got {tuple(shape)}.")
+    allowed = _ON_CUDA if x.is_cuda else _ON_CPU
+    if dtype not in allowed:
+        raise TypeError(f"on {device.type} x must be one of {allowed}, got {dtype}.")
+    if shape[-1] > LONGEST_ROW and x.is_cuda:
+        raise ValueError(f"rows of more than {LONGEST_ROW} values are not supported on CUDA, got {shape[-1]}.")
+    if branch is not None and (branch.shape != shape or branch.dtype != dtype or branch.device != device):
+        raise ValueError(f"branch must match x: {tuple(shape)} {dtype} {device}, got {tuple(branch.shape)} {branch.dtype} {branch.device}.")
+    common = None
+    for name, v in (("weight", weight), ("branch_weight", branch_weight), ("gate", gate)):
+        if v is None:
+            continue
+        if v.shape != shape[-1:] or v.device != device:
+            raise ValueError(f"{name} must have shape {tuple(shape[-1:])} on {device}, got {tuple(v.shape)} on {v.device}.")
+        if v.dtype != dtype and v.dtype != torch.float32:
+            raise TypeError(f"{name} must be {dtype} or float32, got {v.dtype}.")
+        if common is not None and v.dtype != common:
+            raise TypeError(f"weight, branch_weight and gate must have one dtype, got {common} and {v.dtype}.")
+        common = v.dtype
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}.")
     if not scale - scale == 0.0:
@@ -59,38 +71,6 @@ def _host_forward(x, branch, weight, branch_weight, gate, scale, eps):
     return x if branch is None else h.to(x.dtype), None if weight is None else norm(h, weight).to(x.dtype)
 
 
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, branch, weight, branch_weight, gate, scale, eps):
-        from ..engine import decoder
-
-        with torch.cuda.device(x.device):
-            h, y, rms, branch_rms = decoder.residual_norm_forward(x, branch, weight, branch_weight, gate, scale, eps)
-        ctx.save_for_backward(h, branch if branch_weight is not None or gate is not None else None, weight, branch_weight, gate, rms,
-                              branch_rms)
-        ctx.scale, ctx.eps = scale, eps
-        ctx.with_branch = branch is not None
-        ctx.set_materialize_grads(False)
-        return (h if branch is not None else None), y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_h, grad_y):
-        h, branch, weight, branch_weight, gate, rms, branch_rms = ctx.saved_tensors
-        if grad_h is None and grad_y is None:
-            return (None,) * 7
-        from ..engine import decoder
-
-        with torch.cuda.device(h.device):
-            want = list(ctx.needs_input_grad[:5])
-            # (a branch that is only added is not read again: h stands for its place)
-            grads = decoder.residual_norm_backward(h, branch if branch is not None else (h if ctx.with_branch else None), weight, branch_weight,
-                                                   gate, ctx.scale, ctx.eps, rms, branch_rms, grad_h, grad_y, want)
-        if grad_y is None:
-            grads = (*grads[:2], None, *grads[3:])
-        return (*grads, None, None)
-
-
 def residual_norm(
     x: Tensor,
     branch: Tensor,
@@ -108,24 +88,23 @@ def residual_norm(
     The vectors have ``x``'s dtype or are fp32.  Means, sums and the vectors' gradients are held in fp32; ``h`` and ``y`` are each
     rounded once.  Differentiable once.
     """
-    _validate(x, branch, dict(weight=weight, branch_weight=branch_weight, gate=gate), scale, eps)
     if branch is None:
         raise ValueError("residual_norm needs a branch; rms_norm is the norm alone.")
+    _validate(x, branch, weight, branch_weight, gate, scale, eps)
     if not x.is_cuda or x.numel() == 0:
         return _host_forward(x, branch, weight, branch_weight, gate, scale, eps)
-    dim = x.shape[-1]
-    vectors = [None if v is None else v.contiguous() for v in (weight, branch_weight, gate)]
-    h, y = _ResidualNorm.apply(x.reshape(-1, dim), branch.reshape(-1, dim), *vectors, float(scale), float(eps))
-    return h.view(x.shape), None if y is None else y.view(x.shape)
+    out = _native().residual_norm(x, branch, weight, branch_weight, gate, scale, eps)
+    return out[0], out[1] if weight is not None else None
 
 
 def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-5) -> Tensor:
     """``norm(x) * weight`` as :func:`residual_norm` computes its ``y``."""
-    _validate(x, None, dict(weight=weight), 1.0, eps)
+    if weight is None:
+        raise ValueError("rms_norm needs a weight.")
+    _validate(x, None, weight, None, None, 1.0, eps)
     if not x.is_cuda or x.numel() == 0:
         return _host_forward(x, None, weight, None, None, 1.0, eps)[1]
-    _, y = _ResidualNorm.apply(x.reshape(-1, x.shape[-1]), None, weight.contiguous(), None, None, 1.0, float(eps))
-    return y.view(x.shape)
+    return _native().residual_norm(x, None, weight, None, None, 1.0, eps)[0]
 
 
 __all__ = ["residual_norm", "rms_norm"]

@@ -28,7 +28,9 @@ def _no_timeouts():
 @pytest.mark.parametrize("m,n,k", [(1, 8, 1), (128, 256, 64), (256, 256, 128), (130, 72, 200), (513, 300, 65), (300, 1000, 2000), (2600, 2300, 1096),
                                    (100, 700, 30000)])
 def test_gemm16(m, n, k, k_major, dtype, split):
-    from soap_tp_b200.engine import kernels
+    from soap_tp_b200.engine import decoder, kernels
+
+    native = decoder.native
 
     def padded(rows, cols, seed):
         return _rand(rows, kernels.round_up(cols, 8), seed=seed, dtype=dtype)[:, :cols]
@@ -36,16 +38,14 @@ def test_gemm16(m, n, k, k_major, dtype, split):
     a = padded(m, k, 1) if k_major else padded(k, m, 1)
     b = padded(k, n, 2)
     c = torch.full((m + 1, n + 3), 7.0, dtype=dtype, device="cuda")
-    parts = torch.full((kernels._C.SPLIT_SCRATCH,), float("nan"), device="cuda")
-    counters = torch.zeros(kernels._C.SPLIT_COUNTERS, dtype=torch.int32, device="cuda")
-    kernels._C.gemm16_store(dtype == BF16, k_major, [a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), m, n, k, c.data_ptr(), c.stride(0),
-                                                     parts.data_ptr() if split else 0, counters.data_ptr() if split else 0,
-                                                     kernels.status_word(a.device).data_ptr(), kernels._stream()])
+    parts = torch.full((native.SPLIT_SCRATCH,), float("nan"), device="cuda") if split else None
+    counters = torch.zeros(native.SPLIT_COUNTERS, dtype=torch.int32, device="cuda") if split else None
+    native.gemm16(a, b, c, not k_major, decoder.status(a.device), parts, counters)
     x = a.double() if k_major else a.double().t()
     exact = x @ b.double()
     bound = half_step(dtype) * exact.abs() + (k // 16 + 2) * 2.0 ** -23 * (x.abs() @ b.double().abs()) + smallest(dtype)
     within(c[:m, :n], (exact, bound))
-    assert bool((c[m] == 7).all()) and bool((c[:, n:] == 7).all()) and not counters.any()
+    assert bool((c[m] == 7).all()) and bool((c[:, n:] == 7).all()) and (counters is None or not counters.any())
 
 
 # ---- cross entropy ------------------------------------------------------------------------------------------------------
@@ -402,6 +402,21 @@ def test_swiglu8(rows, dim, dtype):
     exact = out_grad.double().t() @ kept_y
     e = (u + c) * 1.01 * kept_y.abs()
     within(d_weight, (exact, u * exact.abs() + out_grad.double().abs().t() @ (e + rows * 2.0 ** -23 * kept_y.abs()) + smallest(dtype)))
+
+
+def test_operators_are_differentiable_once():
+    from soap_tp_b200 import ops
+
+    x, b, gate, up = (_rand(4, 64, seed=i, dtype=BF16).requires_grad_() for i in range(4))
+    hidden, weight, targets = _head(30, 64, 300, BF16)
+    h, y = ops.residual_norm(x, b, torch.ones(64, device="cuda", dtype=BF16))
+    outputs = [(h.float() * y.float()).sum(), ops.swiglu8(gate, up).float().sum(), ops.linear_cross_entropy(hidden, weight, targets),
+               ops.swiglu_linear8(gate, up, x).float().sum()]
+    for output, leaf in zip(outputs, (x, gate, hidden, up)):
+        grad = torch.autograd.grad(output, leaf, create_graph=True)[0]
+        assert grad.requires_grad
+        with pytest.raises(RuntimeError, match="once"):
+            grad.float().sum().backward()
 
 
 # ---- streams, graphs, several at once -----------------------------------------------------------------------------------
