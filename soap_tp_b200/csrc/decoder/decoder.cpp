@@ -82,7 +82,7 @@ struct Vectors {
   Tensor weight, branch_weight, gate;
 };
 
-NormProblem norm_problem(const Tensor& rows, const Tensor& branch, const Vectors& v, double scale, double eps, const Tensor& rms) {
+NormProblem norm_problem(const Tensor& rows, const Tensor& branch, const Vectors& v, double scale, double eps, const Tensor& rms, int64_t status) {
   NormProblem p{};
   p.type = type_of(rows.scalar_type());
   p.vector_type = p.type;
@@ -97,6 +97,7 @@ NormProblem norm_problem(const Tensor& rows, const Tensor& branch, const Vectors
   p.weight = pointer(v.weight); p.branch_weight = pointer(v.branch_weight); p.gate = pointer(v.gate);
   p.rms = rms.data_ptr<float>();
   p.branch_rms = p.rms + p.rows;
+  p.status = reinterpret_cast<int*>(static_cast<uintptr_t>(status));
   return p;
 }
 
@@ -104,14 +105,14 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   // h, if there is a branch, and y, if there is a weight
   using Maybe = std::optional<Tensor>;
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& branch_, const Maybe& weight_, const Maybe& branch_weight_,
-                               const Maybe& gate_, double scale, double eps, std::vector<int64_t> want) {
+                               const Maybe& gate_, double scale, double eps, int64_t status, std::vector<int64_t> want) {
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor branch = given(branch_), weight = given(weight_), branch_weight = given(branch_weight_), gate = given(gate_);
     const Vectors v{weight, branch_weight, gate};
     const Tensor x_rows = rows_of(x), branch_rows = branch.defined() ? rows_of(branch) : Tensor();
     Tensor h = branch.defined() ? like_rows(x) : Tensor(), y = weight.defined() ? like_rows(x) : Tensor();
     const Tensor rms = at::empty({2, x_rows.size(0)}, x.options().dtype(at::kFloat));
-    const NormProblem p = norm_problem(x_rows, branch_rows, v, scale, eps, rms);
+    const NormProblem p = norm_problem(x_rows, branch_rows, v, scale, eps, rms, status);
     residual_norm_forward(p, pointer(h), pointer(y), p.dim, current_stream());
     count(1);
     // (a branch that is only added is not read again)
@@ -120,6 +121,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["want"] = std::move(want);
     ctx->saved_data["branch"] = branch.defined();
+    ctx->saved_data["status"] = status;
     ctx->set_materialize_grads(false);
     variable_list out;
     for (const Tensor* t : {&h, &y})
@@ -128,7 +130,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(8);
+    variable_list out(9);
     const auto saved = ctx->get_saved_variables();
     const bool graph = at::GradMode::is_enabled(), with_branch = ctx->saved_data["branch"].toBool();
     const Tensor grad_h = with_branch ? grads[0] : Tensor(), grad_y = saved[2].defined() ? grads[with_branch ? 1 : 0] : Tensor();
@@ -139,7 +141,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const auto want = ctx->saved_data["want"].toIntVector();
     const Tensor h = rows_of(saved[0]), branch = saved[1].defined() ? rows_of(saved[1]) : Tensor();
     const Tensor gh = grad_h.defined() ? rows_of(grad_h) : Tensor(), gy = grad_y.defined() ? rows_of(grad_y) : Tensor();
-    NormProblem p = norm_problem(h, branch, v, ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), saved[5]);
+    NormProblem p = norm_problem(h, branch, v, ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), saved[5],
+                                 ctx->saved_data["status"].toInt());
     // each gradient in memory of its own: where x and the branch are views of leaves, torch accumulates into what it is handed
     for (int i = 0; i < 2; ++i)
       if (want[i]) out[i] = like_rows(saved[0]);
@@ -149,10 +152,10 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     g.grad_h = address(gh); g.grad_y = address(gy);
     g.d_x = pointer(out[0]); g.d_branch = pointer(out[1]); g.ld = p.dim;
     g.d_weight = pointer(out[2]); g.d_branch_weight = pointer(out[3]); g.d_gate = pointer(out[4]);
-    g.blocks = residual_norm_blocks(p.rows, p.dim);
+    g.blocks = residual_norm_blocks(p, g);
     Tensor partials;
     if (g.d_weight || g.d_branch_weight || g.d_gate) {
-      partials = at::empty({g.blocks, 3, p.dim}, h.options().dtype(at::kFloat));
+      partials = at::empty({g.blocks, 2, p.dim}, h.options().dtype(at::kFloat));
       g.partials = partials.data_ptr<float>();
       count(1);
     }
@@ -447,12 +450,12 @@ bool wanted(const Tensor& x) { return x.defined() && at::GradMode::is_enabled() 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "Operators of a decoder's training step, with gradients, on CUDA tensors";
   m.def("residual_norm", [](const Tensor& x, const std::optional<Tensor>& branch, const std::optional<Tensor>& weight,
-                            const std::optional<Tensor>& branch_weight, const std::optional<Tensor>& gate, double scale, double eps) {
+                            const std::optional<Tensor>& branch_weight, const std::optional<Tensor>& gate, double scale, double eps, int64_t status) {
     using Maybe = std::optional<Tensor>;
     auto vector = [](const Maybe& v) { return v ? Maybe(v->contiguous()) : Maybe(); };
     const Maybe w = vector(weight), wb = vector(branch_weight), g = vector(gate);
     std::vector<int64_t> want{wanted(x), wanted(given(branch)), wanted(given(w)), wanted(given(wb)), wanted(given(g))};
-    return ResidualNorm::apply(x, branch, w, wb, g, scale, eps, std::move(want));
+    return ResidualNorm::apply(x, branch, w, wb, g, scale, eps, status, std::move(want));
   });
   m.def("pack8", &pack);
   m.def("unpack8", [](const Tensor& values, const Tensor& scales, std::vector<int64_t> shape, at::ScalarType type) {

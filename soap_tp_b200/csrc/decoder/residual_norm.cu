@@ -4,11 +4,16 @@
 //   t = dy w             dh = dh' + r (t - h r^2 mean(t h))          dw  = sum over rows of dy h r
 //   db' = s g dh         dg = sum of s dh b'                         dx  = dh
 //   t_b = db' w_b        db = r_b (t_b - b r_b^2 mean(t_b b))        dw_b = sum of db' b r_b
+// dg and dw_b are one sum, of s dh b r_b, times w_b and g.
 // All sums in fp32, h and y rounded once, y from the unrounded h.
 //
-// Memory bounds it: a row is read once into registers (a warp for short rows, a block for long ones), the means are block sums, and
-// everything leaves in one pass.  The backward pass runs a fixed number of blocks over all rows; each thread keeps its columns' sums for the
-// vectors' gradients in registers, and a second kernel adds the blocks' sums in a fixed order.
+// Memory bounds it.  A fixed number of blocks goes over all rows; in a block one to sixteen warps share a row (16 values a thread), and
+// groups of warps take rows of their own.  Each group keeps a ring of rows in shared memory, which untiled bulk copies fill ahead of their use: the
+// means are sums over a group that everything else of a row waits for, and what must be under way meanwhile (some 40 KB an SM) does
+// not fit in registers next to the sums of the vectors' gradients.  Those stay in registers until a block's last row; a second kernel adds the
+// blocks' sums in a fixed order.  The vectors stay in registers as well, as fp32, and arithmetic goes two values at a time: with 40 instructions a value,
+// converted and multiplied anew for every row, issue bounded it.  Rows that do not lie on 16-byte boundaries are copied from the boundary before them and read value by
+// value; rows too long for two of them in shared memory are read straight into registers.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -16,51 +21,96 @@
 #include <string>
 
 #include "launch_util.h"
+#include "ptx.cuh"
 #include "residual_norm.h"
 #include "value16.cuh"
 
 namespace soapb200 {
 namespace {
 
-// A thread's E values of a row that start at `column`, as fp32.  E = 8: a run that lies on 16-byte boundaries; E = 1: any row.
-template <typename T, int E>
-struct Run {
-  static __device__ __forceinline__ void read(const T* p, float (&v)[E]) {
+// A thread's 2 P values of a row, as pairs of fp32.  E = 8: runs of eight neighbouring values on 16-byte boundaries, blockDim.x runs apart;
+// E = 1: single values, blockDim.x apart.  Values beyond the row are zero and are not written.
+template <int E, int P>
+struct Lane {
+  uint64_t v[P];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = 0;
+  }
+  __device__ __forceinline__ float get(int i) const { return pair_element(v[i / 2], i & 1); }
+
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, int dim) {
     if constexpr (E == 8) {
-      Eight<T> e;
-      e.load(p);
-      e.get(v);
+#pragma unroll
+      for (int i = 0; i < P / 4; ++i) {
+        const int column = 8 * (threadIdx.x + i * blockDim.x);
+        if (column < dim) {
+          Eight<T> e;
+          e.load(row + column);
+          float f[8];
+          e.get(f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * i + j] = pack_floats(f[2 * j], f[2 * j + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * i + j] = 0;
+        }
+      }
     } else {
-      v[0] = to_float(*p);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int first = threadIdx.x + 2 * i * blockDim.x, second = first + blockDim.x;
+        v[i] = pack_floats(first < dim ? to_float(row[first]) : 0.f, second < dim ? to_float(row[second]) : 0.f);
+      }
     }
   }
-  static __device__ __forceinline__ void write(T* p, const float (&v)[E]) {
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int dim) const {
     if constexpr (E == 8) {
-      Eight<T> e;
-      e.set(v);
-      e.store(p);
+#pragma unroll
+      for (int i = 0; i < P / 4; ++i) {
+        const int column = 8 * (threadIdx.x + i * blockDim.x);
+        if (column < dim) {
+          Eight<T> e;
+          const float f[8] = {get(8 * i), get(8 * i + 1), get(8 * i + 2), get(8 * i + 3), get(8 * i + 4), get(8 * i + 5), get(8 * i + 6), get(8 * i + 7)};
+          e.set(f);
+          e.store(row + column);
+        }
+      }
     } else {
-      *p = from_float<T>(v[0]);
+#pragma unroll
+      for (int i = 0; i < 2 * P; ++i) {
+        const int column = threadIdx.x + i * blockDim.x;
+        if (column < dim) row[column] = from_float<T>(get(i));
+      }
+    }
+  }
+  // A vector of type T or fp32; ones where there is none.
+  template <typename T>
+  __device__ __forceinline__ void load_vector(const void* vector, bool fp32, int dim) {
+    if (!vector) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = pack_floats(1.f, 1.f);
+    } else if (fp32) {
+      load(static_cast<const float*>(vector), dim);
+    } else {
+      load(static_cast<const T*>(vector), dim);
     }
   }
 };
 
-template <int E>
-__device__ __forceinline__ void read_vector(const void* p, bool fp32, const __nv_bfloat16*, int column, float (&v)[E]) {
-  if (fp32) Run<float, E>::read(static_cast<const float*>(p) + column, v);
-  else Run<__nv_bfloat16, E>::read(static_cast<const __nv_bfloat16*>(p) + column, v);
-}
-template <int E>
-__device__ __forceinline__ void read_vector(const void* p, bool fp32, const __half*, int column, float (&v)[E]) {
-  if (fp32) Run<float, E>::read(static_cast<const float*>(p) + column, v);
-  else Run<__half, E>::read(static_cast<const __half*>(p) + column, v);
-}
-template <int E>
-__device__ __forceinline__ void read_vector(const void* p, bool, const float*, int column, float (&v)[E]) {
-  Run<float, E>::read(static_cast<const float*>(p) + column, v);
+__device__ __forceinline__ float sum_of(uint64_t pair) { return pair_element(pair, 0) + pair_element(pair, 1); }
+__device__ __forceinline__ uint64_t twice(float v) { return pack_floats(v, v); }
+
+// The threads of a row wait for one another: a warp, or blockDim.x threads at a barrier of their own.
+__device__ __forceinline__ void row_sync() {
+  if (blockDim.x == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.y), "r"(blockDim.x) : "memory");
 }
 
-// Sum over the threads of a row: a warp (blockDim.x = 32), or the block.  `shared`: 33 floats; `turn` alternates so that one barrier a sum is enough.
+// Sum over the threads of a row.  `shared`: 64 floats of the row's own; `turn` alternates so that one barrier a sum is enough.
 __device__ __forceinline__ float row_sum(float v, float* shared, int& turn) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -68,7 +118,7 @@ __device__ __forceinline__ float row_sum(float v, float* shared, int& turn) {
   float* slot = shared + 32 * turn;
   turn ^= 1;
   if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
-  __syncthreads();
+  row_sync();
   const int warps = blockDim.x >> 5;
   v = (threadIdx.x & 31) < warps ? slot[threadIdx.x & 31] : 0.f;
 #pragma unroll
@@ -76,261 +126,261 @@ __device__ __forceinline__ float row_sum(float v, float* shared, int& turn) {
   return v;
 }
 
-template <typename T, int E, int N, int THREADS, bool AFTER>
-__global__ void __launch_bounds__(THREADS) residual_norm_forward_kernel(NormProblem p, T* __restrict__ h_out, T* __restrict__ y_out, int64_t ld, int runs) {
-  __shared__ float shared[64];
+constexpr int kMostGroups = 8, kMostStages = 8, kMostInputs = 4;
+
+// How a row is dealt to threads, and what a group of them keeps ahead.
+struct Deal {
+  bool ring;
+  int run, values, threads, groups, bound;                // neighbouring values, values a thread, threads a row, rows at once
+  int stages, row_bytes;                                  // of the ring
+  int smem, blocks;
+};
+
+// The rows of up to four matrices, one row of each a stage.  INPUTS that are absent have a null base.
+template <typename T, int INPUTS>
+struct Ring {
+  Rows inputs[INPUTS];
+  uint8_t* data;
+  uint64_t* full;
+  int stages, row_bytes, dim;
+  int stage = 0;
+  uint32_t parity = 0;
+
+  __device__ __forceinline__ uintptr_t address(int i, int64_t row) const {
+    return reinterpret_cast<uintptr_t>(inputs[i].data) + row * inputs[i].ld * static_cast<int64_t>(sizeof(T));
+  }
+  // One thread: row's copies into stage `s`, from the 16-byte boundary before it to the one behind.
+  __device__ __forceinline__ void fetch(int s, int64_t row) {
+    uint32_t bytes[INPUTS], sum = 0;
+#pragma unroll
+    for (int i = 0; i < INPUTS; ++i) {
+      bytes[i] = 0;
+      if (inputs[i].data) {
+        const uintptr_t from = address(i, row);
+        bytes[i] = static_cast<uint32_t>(((from + dim * sizeof(T) + 15) & ~uintptr_t(15)) - (from & ~uintptr_t(15)));
+        sum += bytes[i];
+      }
+    }
+    mbar_expect_tx(&full[s], sum);
+#pragma unroll
+    for (int i = 0; i < INPUTS; ++i)
+      if (bytes[i]) bulk_load(data + (s * INPUTS + i) * row_bytes, reinterpret_cast<const void*>(address(i, row) & ~uintptr_t(15)), bytes[i], &full[s]);
+  }
+  // Input `i` of the current row.
+  __device__ __forceinline__ const T* at(int i, int64_t row) const {
+    return reinterpret_cast<const T*>(data + (stage * INPUTS + i) * row_bytes + (address(i, row) & 15));
+  }
+  template <bool RING>
+  __device__ __forceinline__ const T* row_at(int i, int64_t row) const {
+    return RING ? at(i, row) : reinterpret_cast<const T*>(address(i, row));
+  }
+  // (a copy of this GPU's own memory always arrives; where it should not have in time, that is recorded, and the results are wrong)
+  __device__ __forceinline__ void wait(int* status) {
+    for (uint32_t it = 0; it < (1u << 24); ++it)
+      if (mbar_try_wait(&full[stage], parity)) return;
+    if (status) atomicCAS(status, 0, kStatusRowWaitTimeout);
+  }
+  // The group is done with the current row; the row `stages` further on takes its place.
+  __device__ __forceinline__ void next(int64_t row, int64_t step, int64_t rows) {
+    row_sync();
+    if (threadIdx.x == 0 && row + stages * step < rows) fetch(stage, row + stages * step);
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+  __device__ __forceinline__ void start(int64_t row, int64_t step, int64_t rows) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < stages && row + s * step < rows; ++s) fetch(s, row + s * step);
+    }
+  }
+};
+
+template <typename T, int INPUTS, bool RING>
+__device__ __forceinline__ Ring<T, INPUTS> make_ring(const Deal& d, int dim, uint8_t* dynamic, uint64_t (&bars)[kMostGroups][kMostStages]) {
+  Ring<T, INPUTS> ring;
+  ring.stages = d.stages; ring.row_bytes = d.row_bytes; ring.dim = dim;
+  ring.data = dynamic + static_cast<int64_t>(threadIdx.y) * d.stages * INPUTS * d.row_bytes;
+  ring.full = bars[threadIdx.y];
+  if constexpr (RING) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < d.stages; ++s) mbar_init(&ring.full[s], 1);
+      mbar_fence_init();
+    }
+    __syncthreads();
+  }
+  return ring;
+}
+
+// Products of a row's vectors: `weight` that y is multiplied by, and scale * gate * branch_weight, which the branch is.
+template <typename T, int E, int P>
+__device__ __forceinline__ void load_vectors(const NormProblem& p, Lane<E, P>& weight, Lane<E, P>& branch) {
+  const bool fp32 = p.vector_type == kFp32;
+  weight.template load_vector<T>(p.weight, fp32, p.dim);
+  branch.template load_vector<T>(p.branch_weight, fp32, p.dim);
+  Lane<E, P> gate;
+  gate.template load_vector<T>(p.gate, fp32, p.dim);
+#pragma unroll
+  for (int i = 0; i < P; ++i) branch.v[i] = mul_pair(mul_pair(branch.v[i], gate.v[i]), twice(p.scale));
+}
+
+template <typename T, int E, int P, int THREADS, bool RING, bool AFTER>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) residual_norm_forward_kernel(NormProblem p, T* __restrict__ h_out, T* __restrict__ y_out, int64_t ld, Deal d) {
+  __shared__ float sums[kMostGroups][64];
+  __shared__ uint64_t bars[kMostGroups][kMostStages];
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  float* shared = sums[threadIdx.y];
   int turn = 0;
+  Ring<T, 2> ring = make_ring<T, 2, RING>(d, p.dim, dynamic, bars);
+  ring.inputs[0] = p.x; ring.inputs[1] = p.branch;
   wait_for_predecessor();
   let_successor_start();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;             // (a whole warp, or no one: blockDim.y > 1 only with rows of a warp)
-  const bool fp32 = p.vector_type == kFp32;
-  const T* x = static_cast<const T*>(p.x.data) + row * p.x.ld;
-  const T* b = static_cast<const T*>(p.branch.data) + row * p.branch.ld;
-  const T* tag = nullptr;
-  float h[N][E];
   const bool with_branch = p.branch.data != nullptr;
-  if (with_branch) {
+  const float inverse_dim = 1.f / static_cast<float>(p.dim);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if constexpr (RING) ring.start(row, step, p.rows);
+  Lane<E, P> weight, branch_factor;
+  load_vectors<T>(p, weight, branch_factor);
+  for (; row < p.rows; row += step) {
+    if constexpr (RING) ring.wait(p.status);
+    Lane<E, P> h;
+    h.load(ring.template row_at<RING>(0, row), p.dim);
+    if (with_branch) {
+      Lane<E, P> b;
+      b.load(ring.template row_at<RING>(1, row), p.dim);
+      float r_b = 1.f;
+      if (AFTER) {
+        uint64_t squares = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int run = threadIdx.x + i * blockDim.x;
-      if (run < runs) {
-        Run<T, E>::read(b + run * E, h[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[i][e] = 0.f;
+        for (int i = 0; i < P; ++i) fma_pair(squares, b.v[i], b.v[i]);
+        r_b = 1.f / sqrtf(row_sum(sum_of(squares), shared, turn) * inverse_dim + p.eps);
+        if (threadIdx.x == 0) p.branch_rms[row] = r_b;
       }
+#pragma unroll
+      for (int i = 0; i < P; ++i) fma_pair(h.v[i], AFTER ? mul_pair(b.v[i], twice(r_b)) : b.v[i], branch_factor.v[i]);
     }
-    float r_b = 1.f;
-    if (AFTER) {
-      float squares = 0.f;
+    if (h_out) h.store(h_out + row * ld, p.dim);
+    if (y_out) {
+      uint64_t squares = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int i = 0; i < P; ++i) fma_pair(squares, h.v[i], h.v[i]);
+      const float r = 1.f / sqrtf(row_sum(sum_of(squares), shared, turn) * inverse_dim + p.eps);
+      if (threadIdx.x == 0) p.rms[row] = r;
 #pragma unroll
-        for (int e = 0; e < E; ++e) squares = fmaf(h[i][e], h[i][e], squares);
-      r_b = 1.f / sqrtf(row_sum(squares, shared, turn) / static_cast<float>(p.dim) + p.eps);
-      if (threadIdx.x == 0) p.branch_rms[row] = r_b;
+      for (int i = 0; i < P; ++i) h.v[i] = mul_pair(mul_pair(h.v[i], twice(r)), weight.v[i]);
+      h.store(y_out + row * ld, p.dim);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int run = threadIdx.x + i * blockDim.x;
-      if (run < runs) {
-        float v[E];
-        if (AFTER) {
-          read_vector<E>(p.branch_weight, fp32, tag, run * E, v);
-#pragma unroll
-          for (int e = 0; e < E; ++e) h[i][e] *= r_b * v[e];
-        }
-        if (p.gate) {
-          read_vector<E>(p.gate, fp32, tag, run * E, v);
-#pragma unroll
-          for (int e = 0; e < E; ++e) h[i][e] *= v[e];
-        }
-        Run<T, E>::read(x + run * E, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[i][e] = fmaf(p.scale, h[i][e], v[e]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int run = threadIdx.x + i * blockDim.x;
-      if (run < runs) {
-        Run<T, E>::read(x + run * E, h[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[i][e] = 0.f;
-      }
-    }
-  }
-  if (h_out) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int run = threadIdx.x + i * blockDim.x;
-      if (run < runs) Run<T, E>::write(h_out + row * ld + run * E, h[i]);
-    }
-  }
-  if (!y_out) return;
-  float squares = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (static_cast<int>(threadIdx.x + i * blockDim.x) < runs) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) squares = fmaf(h[i][e], h[i][e], squares);
-    }
-  }
-  const float r = 1.f / sqrtf(row_sum(squares, shared, turn) / static_cast<float>(p.dim) + p.eps);
-  if (threadIdx.x == 0) p.rms[row] = r;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int run = threadIdx.x + i * blockDim.x;
-    if (run < runs) {
-      float w[E];
-      read_vector<E>(p.weight, fp32, tag, run * E, w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) w[e] *= h[i][e] * r;
-      Run<T, E>::write(y_out + row * ld + run * E, w);
-    }
+    if constexpr (RING) ring.next(row, step, p.rows);
   }
 }
 
-// Blocks of blockDim.y rows at a time, over all rows.  N runs of E values a thread.  SCALED: the branch has a norm or a gate.
-template <typename T, int E, int N, int THREADS, bool SCALED>
+// SCALED: the branch has a norm or a gate.
+template <typename T, int E, int P, int THREADS, bool RING, bool SCALED>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
-residual_norm_backward_kernel(NormProblem p, NormGradients g, int runs) {
-  __shared__ float shared[64];
-  extern __shared__ float joined[];      // dim floats where several rows share a block
+residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
+  __shared__ float sums[kMostGroups][64];
+  __shared__ uint64_t bars[kMostGroups][kMostStages];
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  float* shared = sums[threadIdx.y];
   int turn = 0;
+  Ring<T, 4> ring = make_ring<T, 4, RING>(d, p.dim, dynamic, bars);
+  ring.inputs[0] = g.grad_y; ring.inputs[1] = g.grad_y.data ? p.x : Rows{nullptr, 0};
+  ring.inputs[2] = g.grad_h; ring.inputs[3] = SCALED ? p.branch : Rows{nullptr, 0};
   wait_for_predecessor();
   let_successor_start();
-  const bool fp32 = p.vector_type == kFp32;
-  const T* tag = nullptr;
   const float inverse_dim = 1.f / static_cast<float>(p.dim);
-  const bool after = SCALED && p.branch_weight, gated = SCALED && p.gate;
-  float d_w[N][E], d_wb[SCALED ? N : 1][E], d_g[SCALED ? N : 1][E];
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      d_w[i][e] = 0.f;
-      if (SCALED) d_wb[i][e] = d_g[i][e] = 0.f;
+  const bool after = SCALED && p.branch_weight;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if constexpr (RING) ring.start(row, step, p.rows);
+  Lane<E, P> weight, branch_factor, d_weight, d_branch;      // the last: the sum that both of the branch's vectors' gradients are made of
+  load_vectors<T>(p, weight, branch_factor);
+  d_weight.clear();
+  d_branch.clear();
+  // (a row's reciprocal root mean squares travel while the row before it is worked on)
+  float r_next = 0.f, r_b_next = 1.f;
+  auto look_up = [&](int64_t of) {
+    if (of < p.rows) {
+      if (g.grad_y.data) r_next = p.rms[of];
+      if (after) r_b_next = p.branch_rms[of];
     }
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < p.rows; row += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    float dh[N][E];
-    const T* gh = static_cast<const T*>(g.grad_h.data) + row * g.grad_h.ld;
-    const T* gy = static_cast<const T*>(g.grad_y.data) + row * g.grad_y.ld;
-    const T* h = static_cast<const T*>(p.x.data) + row * p.x.ld;
-    const T* b = static_cast<const T*>(p.branch.data) + row * p.branch.ld;
+  };
+  look_up(row);
+  for (; row < p.rows; row += step) {
+    const float r = r_next, r_b = r_b_next;
+    look_up(row + step);
+    if constexpr (RING) ring.wait(p.status);
+    Lane<E, P> dh;
     if (g.grad_y.data) {
-      const float r = p.rms[row];
-      float hv[N][E], dot = 0.f;
+      Lane<E, P> h;
+      dh.load(ring.template row_at<RING>(0, row), p.dim);
+      h.load(ring.template row_at<RING>(1, row), p.dim);
+      uint64_t dot = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int run = threadIdx.x + i * blockDim.x;
-        if (run < runs) {
-          float w[E];
-          Run<T, E>::read(gy + run * E, dh[i]);
-          Run<T, E>::read(h + run * E, hv[i]);
-          read_vector<E>(p.weight, fp32, tag, run * E, w);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            d_w[i][e] = fmaf(dh[i][e], hv[i][e] * r, d_w[i][e]);
-            dh[i][e] *= w[e];
-            dot = fmaf(dh[i][e], hv[i][e], dot);
-          }
-        }
+      for (int i = 0; i < P; ++i) {
+        const uint64_t product = mul_pair(dh.v[i], h.v[i]);
+        fma_pair(d_weight.v[i], product, twice(r));
+        fma_pair(dot, product, weight.v[i]);
+        dh.v[i] = mul_pair(dh.v[i], weight.v[i]);
       }
-      const float c = row_sum(dot, shared, turn) * inverse_dim * r * r;
+      const float c = row_sum(sum_of(dot), shared, turn) * inverse_dim * r * r;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int i = 0; i < P; ++i) dh.v[i] = mul_pair(fma_pair_of(h.v[i], twice(-c), dh.v[i]), twice(r));
+    } else {
+      dh.clear();
+    }
+    if (g.grad_h.data) {
+      Lane<E, P> gh;
+      gh.load(ring.template row_at<RING>(2, row), p.dim);
 #pragma unroll
-        for (int e = 0; e < E; ++e) dh[i][e] = r * (dh[i][e] - hv[i][e] * c);
+      for (int i = 0; i < P; ++i) add_pair(dh.v[i], gh.v[i]);
+    }
+    if (g.d_x) dh.store(static_cast<T*>(g.d_x) + row * g.ld, p.dim);
+    if constexpr (SCALED) {
+      Lane<E, P> b;
+      b.load(ring.template row_at<RING>(3, row), p.dim);
+      const float by = p.scale * r_b;
+      uint64_t dot = 0;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        fma_pair(d_branch.v[i], mul_pair(dh.v[i], b.v[i]), twice(by));
+        dh.v[i] = mul_pair(dh.v[i], branch_factor.v[i]);
+        fma_pair(dot, dh.v[i], b.v[i]);
+      }
+      if (after) {
+        const float c = row_sum(sum_of(dot), shared, turn) * inverse_dim * r_b * r_b;
+#pragma unroll
+        for (int i = 0; i < P; ++i) dh.v[i] = mul_pair(fma_pair_of(b.v[i], twice(-c), dh.v[i]), twice(r_b));
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int e = 0; e < E; ++e) dh[i][e] = 0.f;
+      for (int i = 0; i < P; ++i) dh.v[i] = mul_pair(dh.v[i], twice(p.scale));
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int run = threadIdx.x + i * blockDim.x;
-      if (run < runs) {
-        if (g.grad_h.data) {
-          float v[E];
-          Run<T, E>::read(gh + run * E, v);
-#pragma unroll
-          for (int e = 0; e < E; ++e) dh[i][e] += v[e];
-        }
-        if (g.d_x) Run<T, E>::write(static_cast<T*>(g.d_x) + row * g.ld + run * E, dh[i]);
-      }
-    }
-    if constexpr (!SCALED) {
-      if (g.d_branch) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int run = threadIdx.x + i * blockDim.x;
-          if (run < runs) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) dh[i][e] *= p.scale;
-            Run<T, E>::write(static_cast<T*>(g.d_branch) + row * g.ld + run * E, dh[i]);
-          }
-        }
-      }
-    } else {
-      const float r_b = after ? p.branch_rms[row] : 1.f;
-      float bv[N][E], dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int run = threadIdx.x + i * blockDim.x;
-        if (run < runs) {
-          float wb[E], gate[E];
-          Run<T, E>::read(b + run * E, bv[i]);
-#pragma unroll
-          for (int e = 0; e < E; ++e) wb[e] = gate[e] = 1.f;
-          if (after) read_vector<E>(p.branch_weight, fp32, tag, run * E, wb);
-          if (gated) read_vector<E>(p.gate, fp32, tag, run * E, gate);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float normed = bv[i][e] * r_b;
-            dh[i][e] *= p.scale;
-            d_g[i][e] = fmaf(dh[i][e], normed * wb[e], d_g[i][e]);
-            dh[i][e] *= gate[e];
-            d_wb[i][e] = fmaf(dh[i][e], normed, d_wb[i][e]);
-            dh[i][e] *= wb[e];
-            dot = fmaf(dh[i][e], bv[i][e], dot);
-          }
-        }
-      }
-      const float c = after ? row_sum(dot, shared, turn) * inverse_dim * r_b * r_b : 0.f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int run = threadIdx.x + i * blockDim.x;
-        if (run < runs) {
-          if (after) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) dh[i][e] = r_b * (dh[i][e] - bv[i][e] * c);
-          }
-          if (g.d_branch) Run<T, E>::write(static_cast<T*>(g.d_branch) + row * g.ld + run * E, dh[i]);
-        }
-      }
-    }
+    if (g.d_branch) dh.store(static_cast<T*>(g.d_branch) + row * g.ld, p.dim);
+    if constexpr (RING) ring.next(row, step, p.rows);
   }
-  // this block's sums: rows that share the block are added one after another
-  auto leave = [&](float (&sums)[N][E], int which) {
-    float* out = g.partials + (static_cast<int64_t>(blockIdx.x) * 3 + which) * p.dim;
-    if (blockDim.y == 1) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int run = threadIdx.x + i * blockDim.x;
-        if (run < runs) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) out[run * E + e] = sums[i][e];
-        }
-      }
-      return;
-    }
+  // this block's sums: rows that share the block are added one after another, where the ring was
+  float* joined = reinterpret_cast<float*>(dynamic);
+  auto leave = [&](const Lane<E, P>& values, int which) {
+    float* out = g.partials + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.dim;
     for (int y = 0; y < static_cast<int>(blockDim.y); ++y) {
-      __syncthreads();
+      if (blockDim.y > 1) __syncthreads();
       if (static_cast<int>(threadIdx.y) == y) {
+        Lane<E, P> sum = values;
+        if (y) {
+          Lane<E, P> before;
+          before.load(joined, p.dim);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int run = threadIdx.x + i * blockDim.x;
-          if (run < runs) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float before = y ? joined[run * E + e] : 0.f;
-              if (y + 1 < static_cast<int>(blockDim.y)) joined[run * E + e] = before + sums[i][e];
-              else out[run * E + e] = before + sums[i][e];
-            }
-          }
+          for (int i = 0; i < P; ++i) add_pair(sum.v[i], before.v[i]);
         }
+        sum.store(y + 1 < static_cast<int>(blockDim.y) ? joined : out, p.dim);
       }
     }
   };
-  if (g.d_weight) leave(d_w, 0);
+  if (g.d_weight) leave(d_weight, 0);
   if constexpr (SCALED) {
-    if (g.d_branch_weight) leave(d_wb, 1);
-    if (g.d_gate) leave(d_g, 2);
+    if (g.d_branch_weight || g.d_gate) leave(d_branch, 1);
   }
 }
 
@@ -341,47 +391,76 @@ __global__ void __launch_bounds__(32 * kSumSlices) norm_vectors_kernel(NormProbl
   wait_for_predecessor();
   let_successor_start();
   const int which = blockIdx.y;
-  void* out = which == 0 ? g.d_weight : which == 1 ? g.d_branch_weight : g.d_gate;
-  if (!out) return;
+  if (which == 0 ? !g.d_weight : !g.d_branch_weight && !g.d_gate) return;
   const int column = blockIdx.x * 32 + threadIdx.x;
   float sum = 0.f;
   if (column < p.dim) {
 #pragma unroll 8
-    for (int i = threadIdx.y; i < g.blocks; i += kSumSlices) sum += g.partials[(static_cast<int64_t>(i) * 3 + which) * p.dim + column];
+    for (int i = threadIdx.y; i < g.blocks; i += kSumSlices) sum += g.partials[(static_cast<int64_t>(i) * 2 + which) * p.dim + column];
   }
   shared[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.y == 0 && column < p.dim) {
 #pragma unroll
     for (int s = 1; s < kSumSlices; ++s) sum += shared[s][threadIdx.x];
-    if (p.vector_type == kFp32) static_cast<float*>(out)[column] = sum;
-    else if (p.vector_type == kFp16) static_cast<__half*>(out)[column] = __float2half_rn(sum);
-    else static_cast<__nv_bfloat16*>(out)[column] = __float2bfloat16_rn(sum);
+    auto vector = [&](const void* v) {
+      if (!v) return 1.f;
+      return p.vector_type == kFp32 ? static_cast<const float*>(v)[column]
+                                    : p.vector_type == kFp16 ? __half2float(static_cast<const __half*>(v)[column])
+                                                             : __bfloat162float(static_cast<const __nv_bfloat16*>(v)[column]);
+    };
+    auto write = [&](void* out, float value) {
+      if (!out) return;
+      if (p.vector_type == kFp32) static_cast<float*>(out)[column] = value;
+      else if (p.vector_type == kFp16) static_cast<__half*>(out)[column] = __float2half_rn(value);
+      else static_cast<__nv_bfloat16*>(out)[column] = __float2bfloat16_rn(value);
+    };
+    if (which == 0) {
+      write(g.d_weight, sum);
+    } else {
+      write(g.d_branch_weight, sum * vector(p.gate));
+      write(g.d_gate, sum * vector(p.branch_weight));
+    }
   }
 }
 
-// How a row is dealt to threads: runs of eight values where everything lies on 16-byte boundaries, single values otherwise; a warp
-// for up to 512 or 256 values, otherwise as many warps as 16 or 8 values a thread ask for.  `bound`: what the kernel is compiled for.
-struct Deal {
-  int run, per_thread, threads, rows, runs, bound;
-};
-constexpr int kShortRow = 256;      // values of a row that one warp takes, whatever the run
-Deal deal_of(bool wide, int dim) {
+int sms_of_device() {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    throw std::runtime_error("residual_norm: no device");
+  return sms;
+}
+
+// A warp for every 512 values, rounded up to a power of two, with 16 values a thread.  Blocks of eight warps share an SM's shared memory by
+// twos or threes (a backward pass's registers allow two).
+constexpr int kRingBytes = 216 * 1024;      // of an SM's 227 KB
+Deal deal_of(bool wide, int64_t rows, int dim, int size, int inputs, int resident) {
   Deal d{};
+  const int warps_of = (dim + 511) / 512;
+  int warps = 1;
+  while (warps < warps_of) warps *= 2;
   d.run = wide ? 8 : 1;
-  d.runs = (dim + d.run - 1) / d.run;
-  d.per_thread = wide ? 2 : 8;
-  if (dim <= kShortRow) {
-    d.threads = 32;
-    d.rows = 8;
-    d.bound = 256;
-    return d;
+  d.values = 16;
+  d.threads = 32 * warps;
+  d.groups = warps < 8 ? 8 / warps : 1;
+  d.bound = warps <= 8 ? 256 : 512;
+  d.row_bytes = (dim * size + (wide ? 0 : 15) + 15) / 16 * 16;
+  const int64_t stage = static_cast<int64_t>(d.groups) * inputs * d.row_bytes;
+  for (int ctas = warps <= 8 ? resident : 1; ctas >= 1 && !d.ring; --ctas) {
+    d.stages = static_cast<int>(std::min<int64_t>(kMostStages, (kRingBytes / ctas - 4096) / stage));      // (what else a block has is under 4 KB)
+    if (d.stages < 2 || warps > 16) continue;
+    d.ring = true;
+    d.smem = static_cast<int>(d.stages * stage);
+    d.blocks = static_cast<int>(std::min<int64_t>((rows + d.groups - 1) / d.groups, int64_t{ctas} * sms_of_device()));
   }
-  d.rows = 1;
-  if (d.runs > 1024 * d.per_thread) d.per_thread = wide ? 4 : 32;
-  if (d.runs > 1024 * d.per_thread) throw std::invalid_argument("residual_norm: rows of more than 32768 values are not supported");
-  d.threads = ((d.runs + d.per_thread - 1) / d.per_thread + 31) / 32 * 32;
-  d.bound = d.threads <= 256 ? 256 : d.threads <= 512 ? 512 : 1024;
+  if (d.ring) return d;
+  d.stages = d.row_bytes = 0;
+  d.groups = 1;
+  if (!wide || dim > 1024 * 16) d.values = 32;
+  if (dim > 1024 * d.values) throw std::invalid_argument("residual_norm: rows of more than 32768 values are not supported");
+  d.threads = ((dim + d.values - 1) / d.values + 31) / 32 * 32;
+  d.bound = 1024;
+  d.blocks = static_cast<int>(std::min<int64_t>(rows, 2 * sms_of_device()));
   return d;
 }
 
@@ -412,72 +491,82 @@ void for_type(int type, F f) {
   else throw std::invalid_argument("residual_norm: unknown type");
 }
 
-template <int E_, int N_, int THREADS_>
+template <int E_, int P_, int THREADS_, bool RING_>
 struct Form {
-  static constexpr int E = E_, N = N_, THREADS = THREADS_;
+  static constexpr int E = E_, P = P_, THREADS = THREADS_;
+  static constexpr bool RING = RING_;
 };
 template <typename F>
 void for_deal(const Deal& d, F f) {
-  if (d.run == 8) {
-    if (d.per_thread == 4) f(Form<8, 4, 1024>{});
-    else if (d.bound == 256) f(Form<8, 2, 256>{});
-    else if (d.bound == 512) f(Form<8, 2, 512>{});
-    else f(Form<8, 2, 1024>{});
+  if (d.ring) {
+    if (d.run == 8 && d.bound == 256) f(Form<8, 8, 256, true>{});
+    else if (d.run == 8) f(Form<8, 8, 512, true>{});
+    else if (d.bound == 256) f(Form<1, 8, 256, true>{});
+    else f(Form<1, 8, 512, true>{});
+  } else if (d.run == 8) {
+    if (d.values == 32) f(Form<8, 16, 1024, false>{});
+    else f(Form<8, 8, 1024, false>{});
   } else {
-    if (d.per_thread == 32) f(Form<1, 32, 1024>{});
-    else if (d.bound == 256) f(Form<1, 8, 256>{});
-    else f(Form<1, 8, 1024>{});
+    f(Form<1, 16, 1024, false>{});
   }
+}
+
+Deal forward_deal(const NormProblem& p, const void* h, const void* y, int64_t ld) {
+  const int size = size_of(p.type);
+  return deal_of(wide_problem(p) && on_16(h, ld, size) && on_16(y, ld, size), p.rows, p.dim, size, 2, 3);
+}
+Deal backward_deal(const NormProblem& p, const NormGradients& g) {
+  const int size = size_of(p.type);
+  const bool wide = wide_problem(p) && on_16(g.grad_h.data, g.grad_h.ld, size) && on_16(g.grad_y.data, g.grad_y.ld, size) &&
+                    on_16(g.d_x, g.ld, size) && on_16(g.d_branch, g.ld, size);
+  return deal_of(wide, p.rows, p.dim, size, 4, 2);
+}
+
+template <typename Kernel, typename... Arguments>
+void start(const char* what, Kernel kernel, const Deal& d, PerDeviceOnce& once, cudaStream_t stream, Arguments&&... arguments) {
+  allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes, once, what);
+  check(launch_dependent(kernel, dim3(d.blocks), dim3(d.threads, d.groups), d.smem, stream, std::forward<Arguments>(arguments)...), what);
 }
 
 }  // namespace
 
-int residual_norm_blocks(int64_t rows, int dim) {
-  int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    throw std::runtime_error("residual_norm: no device");
-  const int at_once = dim <= kShortRow ? 8 : 1;
-  return static_cast<int>(std::min<int64_t>((rows + at_once - 1) / at_once, 2 * sms));
-}
+int residual_norm_blocks(const NormProblem& p, const NormGradients& g) { return backward_deal(p, g).blocks; }
 
 void residual_norm_forward(const NormProblem& p, void* h, void* y, int64_t ld, cudaStream_t stream) {
   check_problem(p);
-  const int size = size_of(p.type);
-  const Deal d = deal_of(wide_problem(p) && on_16(h, ld, size) && on_16(y, ld, size), p.dim);
-  const int64_t blocks = (p.rows + d.rows - 1) / d.rows;
-  if (blocks > 0x7fffffff) throw std::invalid_argument("residual_norm: too many rows");
+  const Deal d = forward_deal(p, h, y, ld);
   for_type(p.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     for_deal(d, [&](auto form) {
       using F = decltype(form);
-      auto kernel = p.branch_weight ? residual_norm_forward_kernel<T, F::E, F::N, F::THREADS, true>
-                                    : residual_norm_forward_kernel<T, F::E, F::N, F::THREADS, false>;
-      check(launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), dim3(d.threads, d.rows), 0, stream, p, static_cast<T*>(h),
-                             static_cast<T*>(y), ld, d.runs),
-            "residual_norm_forward");
+      static PerDeviceOnce plain, after;
+      if (p.branch_weight)
+        start("residual_norm_forward", residual_norm_forward_kernel<T, F::E, F::P, F::THREADS, F::RING, true>, d, after, stream, p,
+              static_cast<T*>(h), static_cast<T*>(y), ld, d);
+      else
+        start("residual_norm_forward", residual_norm_forward_kernel<T, F::E, F::P, F::THREADS, F::RING, false>, d, plain, stream, p,
+              static_cast<T*>(h), static_cast<T*>(y), ld, d);
     });
   });
 }
 
 void residual_norm_backward(const NormProblem& p, const NormGradients& g, cudaStream_t stream) {
   check_problem(p);
-  const int size = size_of(p.type);
-  const Deal d = deal_of(wide_problem(p) && on_16(g.grad_h.data, g.grad_h.ld, size) && on_16(g.grad_y.data, g.grad_y.ld, size) &&
-                             on_16(g.d_x, g.ld, size) && on_16(g.d_branch, g.ld, size),
-                         p.dim);
-  if (g.blocks < 1) throw std::invalid_argument("residual_norm: no blocks");
+  const Deal d = backward_deal(p, g);
+  if (g.blocks != d.blocks) throw std::invalid_argument("residual_norm: as many blocks as residual_norm_blocks says");
   for_type(p.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     for_deal(d, [&](auto form) {
       using F = decltype(form);
-      auto kernel = p.branch_weight || p.gate ? residual_norm_backward_kernel<T, F::E, F::N, F::THREADS, true>
-                                              : residual_norm_backward_kernel<T, F::E, F::N, F::THREADS, false>;
-      check(launch_dependent(kernel, dim3(g.blocks), dim3(d.threads, d.rows), d.rows > 1 ? p.dim * sizeof(float) : 0, stream, p, g, d.runs),
-            "residual_norm_backward");
+      static PerDeviceOnce plain, scaled;
+      if (p.branch_weight || p.gate)
+        start("residual_norm_backward", residual_norm_backward_kernel<T, F::E, F::P, F::THREADS, F::RING, true>, d, scaled, stream, p, g, d);
+      else
+        start("residual_norm_backward", residual_norm_backward_kernel<T, F::E, F::P, F::THREADS, F::RING, false>, d, plain, stream, p, g, d);
     });
   });
   if (g.d_weight || g.d_branch_weight || g.d_gate)
-    check(launch_dependent(norm_vectors_kernel, dim3((p.dim + 31) / 32, 3), dim3(32, kSumSlices), 0, stream, p, g), "norm_vectors");
+    check(launch_dependent(norm_vectors_kernel, dim3((p.dim + 31) / 32, 2), dim3(32, kSumSlices), 0, stream, p, g), "norm_vectors");
 }
 
 }  // namespace soapb200

@@ -19,13 +19,14 @@ struct NormProblem {
   Rows branch;                    // null: h = x
   const void *weight, *branch_weight, *gate;      // any may be null
   float *rms, *branch_rms;        // [rows]: 1 / sqrt(mean of squares + eps), of h and of the branch
+  int* status;
 };
 
 // h (null: not written) and y (null where there is no weight), rows `ld` elements apart.
 void residual_norm_forward(const NormProblem& p, void* h, void* y, int64_t ld, cudaStream_t stream);
 
-// Gradients.  `grad_h`, `grad_y`, d_x and d_branch may be null.  `partials`: blocks x 3 x dim floats
-// (weight, branch_weight, gate), of which the ones asked for are summed into d_weight, d_branch_weight, d_gate (vector_type).
+// Gradients.  `grad_h`, `grad_y`, d_x and d_branch may be null.  `partials`: blocks x 2 x dim floats,
+// of which d_weight, d_branch_weight and d_gate (vector_type; any may be null) are made.
 struct NormGradients {
   Rows grad_h, grad_y;
   void *d_x, *d_branch;
@@ -35,7 +36,7 @@ struct NormGradients {
   void *d_weight, *d_branch_weight, *d_gate;
 };
 void residual_norm_backward(const NormProblem& p, const NormGradients& g, cudaStream_t stream);
-// How many blocks a backward pass of this shape uses.
-int residual_norm_blocks(int64_t rows, int dim);
+// How many blocks a backward pass uses (`g` but for partials and blocks).
+int residual_norm_blocks(const NormProblem& p, const NormGradients& g);
 
 }  // namespace soapb200

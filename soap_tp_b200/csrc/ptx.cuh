@@ -77,6 +77,12 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tensor_m
       ::"r"(smem_u32(smem_dst)), "l"(tensor_map), "r"(smem_u32(bar)), "r"(x), "r"(y)
       : "memory");
 }
+// Untiled copy into this CTA's shared memory: both addresses and the size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* source, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(smem_dst)), "l"(source), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_descriptor(const void* tensor_map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(tensor_map) : "memory");
 }
@@ -165,6 +171,16 @@ __device__ __forceinline__ float pair_element(uint64_t pair, int which) {
 }
 __device__ __forceinline__ void fma_pair(uint64_t& sum, uint64_t a, uint64_t b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t product;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(product) : "l"(a), "l"(b));
+  return product;
+}
+__device__ __forceinline__ uint64_t fma_pair_of(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t sum;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(sum) : "l"(a), "l"(b), "l"(c));
+  return sum;
 }
 __device__ __forceinline__ void add_pair(uint64_t& sum, uint64_t a) {
   asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(a));

@@ -15,6 +15,7 @@ enum StatusCode : int {
   kStatusPanelExchangeTimeout = 6,    // QR panel: a poll of the exchange between its thread blocks ran out
   kStatusPeerFlagTimeout = 7,         // a wait for a peer's "data ready" flag ran out
   kStatusGridBarrierTimeout = 8,      // tridiagonalisation: a barrier over the CTAs of the launch ran out
+  kStatusRowWaitTimeout = 9,          // a norm's rows never arrived in shared memory
 };
 
 }  // namespace soapb200

@@ -35,6 +35,7 @@ STATUS_MESSAGES = {
     6: "QR panel exchange between thread blocks timed out",
     7: "wait for a peer's data-ready flag timed out",
     8: "tridiagonalisation grid barrier timed out",
+    9: "a norm's rows never arrived in shared memory",
 }
 
 LAUNCH_COUNTS: Dict[str, int] = {}

@@ -21,7 +21,7 @@ _ON_CPU = (*_ON_CUDA, torch.float64)
 def _native():
     from ..engine import decoder
 
-    return decoder.native
+    return decoder
 
 
 def _validate(x: Tensor, branch: Optional[Tensor], weight: Optional[Tensor], branch_weight: Optional[Tensor], gate: Optional[Tensor],
@@ -93,7 +93,8 @@ def residual_norm(
     _validate(x, branch, weight, branch_weight, gate, scale, eps)
     if not x.is_cuda or x.numel() == 0:
         return _host_forward(x, branch, weight, branch_weight, gate, scale, eps)
-    out = _native().residual_norm(x, branch, weight, branch_weight, gate, scale, eps)
+    decoder = _native()
+    out = decoder.native.residual_norm(x, branch, weight, branch_weight, gate, scale, eps, decoder.status(x.device))
     return out[0], out[1] if weight is not None else None
 
 
@@ -104,7 +105,8 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-5) -> Tensor:
     _validate(x, None, weight, None, None, 1.0, eps)
     if not x.is_cuda or x.numel() == 0:
         return _host_forward(x, None, weight, None, None, 1.0, eps)[1]
-    return _native().residual_norm(x, None, weight, None, None, 1.0, eps)[0]
+    decoder = _native()
+    return decoder.native.residual_norm(x, None, weight, None, None, 1.0, eps, decoder.status(x.device))[0]
 
 
 __all__ = ["residual_norm", "rms_norm"]
