@@ -8,8 +8,11 @@
 // y = silu(g) u keeps g and u this way, and its backward pass works from them: dg = dy u' s (1 + g' (1 - s)), du = dy g' s with
 // s = sigmoid(g').
 //
-// Memory bounds all four: eight threads take a group, eight values each (16-byte loads and stores of 16-bit types, 8-byte ones of
-// the kept values), and the group's maximum goes round with three shuffles.
+// Memory bounds all four, once instructions do not: eight threads take a group, eight values each (16-byte loads and stores of 16-bit types,
+// 8-byte ones of the kept values), and the group's maximum goes round with three shuffles.  Magnitudes of 16-bit values are compared two at a
+// time as they lie; a value becomes its whole number by one multiply-add that leaves it in the low byte of 1.5 * 2^23 + q, and comes back
+// as the low byte of 2^23 + q + 128.  (Conversion instructions, at a quarter of the rate, and a division for each address made 19
+// instructions a value and bounded packing at 32768 x 4096: 112 us where its bytes take 63.)
 #include <cuda_runtime.h>
 
 #include <stdexcept>
@@ -27,75 +30,125 @@ constexpr int kPerThread = 8;
 constexpr int kGroupThreads = kScaleGroup / kPerThread;
 constexpr float kSmallestScale = 1.17549435e-38f;      // 2^-126
 
-// Where this thread's eight values are.
-struct Place {
-  int64_t row;
-  int group, column, valid;      // valid <= 0: beyond the row
+// Division of numbers below 2^31 by a number that is known before the launch: (n m) >> (32 + s) with m = ceil(2^(32 + s) / d), s =
+// ceil(log2 d) - 1 (Granlund and Montgomery, 1994; d = 1 apart).
+struct Divisor {
+  uint32_t d, multiplier, shift;
+  explicit Divisor(uint32_t divisor) : d(divisor), multiplier(0), shift(0) {
+    if (d == 1) return;
+    while ((uint64_t{1} << (shift + 1)) < d) ++shift;
+    multiplier = static_cast<uint32_t>(((uint64_t{1} << (32 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1 ? n : __umulhi(n, multiplier) >> shift; }
 };
 
 struct Shape {
-  int64_t rows;
-  int dim, groups;               // groups of a row
-  __device__ __forceinline__ bool place(int64_t group, int lane8, Place& p) const {
-    if (group >= rows * groups) return false;
-    if (rows * groups <= 0x7fffffff) {
-      p.row = static_cast<uint32_t>(group) / static_cast<uint32_t>(groups);
-      p.group = static_cast<int>(static_cast<uint32_t>(group) - static_cast<uint32_t>(p.row) * static_cast<uint32_t>(groups));
-    } else {
-      p.row = group / groups;
-      p.group = static_cast<int>(group - p.row * groups);
-    }
-    p.column = p.group * kScaleGroup + lane8 * kPerThread;
-    p.valid = min(kPerThread, dim - p.column);
-    return true;
+  uint32_t count;                // groups in all
+  int dim;
+  Divisor groups;                // of a row
+};
+
+// Where this thread's eight values are.
+struct Place {
+  uint32_t group;                // of all
+  int64_t row;
+  int column, valid;             // valid <= 0: beyond the row
+  __device__ __forceinline__ explicit Place(const Shape& s) {
+    group = blockIdx.x * static_cast<uint32_t>(kThreads / kGroupThreads) + threadIdx.x / kGroupThreads;
+    row = s.groups.of(group);
+    column = static_cast<int>(group - static_cast<uint32_t>(row) * s.groups.d) * kScaleGroup + (threadIdx.x % kGroupThreads) * kPerThread;
+    valid = group < s.count ? min(kPerThread, s.dim - column) : 0;
   }
 };
 
-__device__ __forceinline__ int64_t first_group() {
-  return (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kGroupThreads;
+// WIDE: all rows lie on 16-byte boundaries and are multiples of eight values long.
+template <bool WIDE, typename T>
+__device__ __forceinline__ Eight<T> load8(const T* p, int valid) {
+  Eight<T> e;
+  if (WIDE) {
+    if (valid > 0) e.load(p);
+    else e.clear();
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_float(p[i]) : 0.f;
+    e.set(v);                    // (exact: the values have this type)
+  }
+  return e;
+}
+template <bool WIDE, typename T>
+__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
+  if (WIDE) {
+    Eight<T> e;
+    e.set(v);
+    e.store(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) p[i] = from_float<T>(v[i]);
+  }
 }
 
-// The scale of a group whose eight threads hold its values; all 32 lanes call.
-__device__ __forceinline__ float group_scale(const float (&v)[8]) {
-  uint32_t most = 0;                       // of the magnitudes' bits: infinities and NaN come out above all numbers
+// The scale of a group whose eight threads hold its values; all 32 lanes call.  Magnitudes are compared as whole numbers: infinities and NaN
+// come out above all others.
+template <typename T>
+__device__ __forceinline__ float group_scale(const Eight<T>& e) {
+  uint32_t most;
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t w[8] = {e.words[0].x, e.words[0].y, e.words[0].z, e.words[0].w, e.words[1].x, e.words[1].y, e.words[1].z, e.words[1].w};
+    most = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) most = max(most, w[i] & 0x7fffffffu);
 #pragma unroll
-  for (int o = 1; o < kGroupThreads; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int o = 1; o < kGroupThreads; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  } else {
+    constexpr uint32_t kMagnitude = 0x7fff7fffu;
+    most = __vmaxu2(__vmaxu2(e.words[0].x & kMagnitude, e.words[0].y & kMagnitude), __vmaxu2(e.words[0].z & kMagnitude, e.words[0].w & kMagnitude));
+#pragma unroll
+    for (int o = 1; o < kGroupThreads; o <<= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = max(most & 0xffffu, most >> 16);
+    if constexpr (std::is_same<T, __half>::value) most = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(most))));
+    else most <<= 16;
+  }
   return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(most) / 127.f, kSmallestScale);
 }
 
-// 16-bit values are multiplied by the reciprocal, whose rounding can move what lies within 2^-16 of a step from a tie to the other side;
+// 16-bit values are multiplied by the reciprocal, whose rounding can move what lies within 2^-15 of a step from a tie to the other side;
 // fp32 values, which come back exactly but for their step, are divided.
 template <typename T>
-__device__ __forceinline__ uint2 quantise(const float (&v)[8], float scale) {
-  const float inverse = 1.f / scale;
-  uint32_t w[2] = {0, 0};
+__device__ __forceinline__ uint2 quantise(const Eight<T>& e, float scale) {
+  constexpr float kShift = 12582912.f;       // 1.5 * 2^23: its neighbours are whole numbers, in two's complement in the low byte
+  float v[8];
+  e.get(v);
+  uint32_t bits[8];
+  const float inverse = __fdividef(1.f, scale);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float quotient = std::is_same<T, float>::value ? v[i] / scale : v[i] * inverse;
-    w[i / 4] |= (static_cast<uint32_t>(__float2int_rn(quotient)) & 0xffu) << (8 * (i & 3));
-  }
+  for (int i = 0; i < 8; ++i)
+    bits[i] = __float_as_uint(std::is_same<T, float>::value ? v[i] / scale + kShift : fmaf(v[i], inverse, kShift));
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __byte_perm(__byte_perm(bits[4 * i], bits[4 * i + 1], 0x0040), __byte_perm(bits[4 * i + 2], bits[4 * i + 3], 0x0040), 0x5410);
   return make_uint2(w[0], w[1]);
 }
 
 __device__ __forceinline__ void dequantise(uint2 q, float scale, float (&v)[8]) {
-  const uint32_t w[2] = {q.x, q.y};
+  constexpr uint32_t kBits = 0x4b000000u;    // 2^23
+  const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i & 3)))) * scale;
+  for (int i = 0; i < 8; ++i) v[i] = (__uint_as_float(__byte_perm(w[i / 4], kBits, 0x7650 | (i & 3))) - 8388736.f) * scale;
 }
 
+// All 32 lanes call.
 template <typename T>
-__device__ __forceinline__ void keep(const Kept8& kept, const Shape& shape, const Place& p, bool here, int lane8, const float (&v)[8]) {
-  const float scale = group_scale(v);
-  if (!here) return;
-  if (p.valid > 0) *reinterpret_cast<uint2*>(kept.values + p.row * kept.pitch + p.column) = quantise<T>(v, scale);
-  if (lane8 == 0) kept.scales[p.row * shape.groups + p.group] = scale;
+__device__ __forceinline__ void keep(const Kept8& kept, const Shape& shape, const Place& p, const Eight<T>& e) {
+  const float scale = group_scale(e);
+  if (p.valid > 0) *reinterpret_cast<uint2*>(kept.values + p.row * kept.pitch + p.column) = quantise(e, scale);
+  if (threadIdx.x % kGroupThreads == 0 && p.group < shape.count) kept.scales[p.group] = scale;
 }
 
-__device__ __forceinline__ void kept_values(const Kept8& kept, const Shape& shape, const Place& p, float (&v)[8]) {
-  dequantise(*reinterpret_cast<const uint2*>(kept.values + p.row * kept.pitch + p.column),
-             kept.scales[p.row * shape.groups + p.group], v);
+__device__ __forceinline__ void kept_values(const Kept8& kept, const Place& p, float (&v)[8]) {
+  dequantise(*reinterpret_cast<const uint2*>(kept.values + p.row * kept.pitch + p.column), kept.scales[p.group], v);
 }
 
 template <typename T>
@@ -107,82 +160,80 @@ __device__ __forceinline__ float sigmoid(float x) {
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t ld, Shape shape, Kept8 kept, bool wide) {
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t ld, Shape shape, Kept8 kept) {
   wait_for_predecessor();
   let_successor_start();
-  const int lane8 = threadIdx.x % kGroupThreads;
-  Place p{};
-  const bool here = shape.place(first_group(), lane8, p);
-  float v[8];
-  read_eight(x + p.row * ld + p.column, here ? p.valid : 0, wide, v);
-  keep<T>(kept, shape, p, here, lane8, v);
+  const Place p(shape);
+  keep(kept, shape, p, load8<WIDE>(x + p.row * ld + p.column, p.valid));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) unpack8_kernel(Kept8 kept, Shape shape, T* __restrict__ out, int64_t ld, bool wide) {
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kThreads) unpack8_kernel(Kept8 kept, Shape shape, T* __restrict__ out, int64_t ld) {
   wait_for_predecessor();
   let_successor_start();
-  Place p{};
-  if (!shape.place(first_group(), threadIdx.x % kGroupThreads, p) || p.valid <= 0) return;
+  const Place p(shape);
+  if (p.valid <= 0) return;
   float v[8];
-  kept_values(kept, shape, p, v);
-  write_eight(out + p.row * ld + p.column, p.valid, wide, v);
+  kept_values(kept, p, v);
+  store8<WIDE>(out + p.row * ld + p.column, p.valid, v);
 }
 
-template <typename T, bool KEEP>
+template <typename T, bool WIDE, bool KEEP>
 __global__ void __launch_bounds__(kThreads)
 swiglu8_forward_kernel(const T* __restrict__ gate, int64_t ld_gate, const T* __restrict__ up, int64_t ld_up, Shape shape,
-                       T* __restrict__ y, int64_t ld, Kept8 gate8, Kept8 up8, bool wide) {
+                       T* __restrict__ y, int64_t ld, Kept8 gate8, Kept8 up8) {
   wait_for_predecessor();
   let_successor_start();
-  const int lane8 = threadIdx.x % kGroupThreads;
-  Place p{};
-  const bool here = shape.place(first_group(), lane8, p);
-  const int valid = here ? p.valid : 0;
-  float g[8], u[8];
-  read_eight(gate + p.row * ld_gate + p.column, valid, wide, g);
-  read_eight(up + p.row * ld_up + p.column, valid, wide, u);
+  const Place p(shape);
+  const Eight<T> g8 = load8<WIDE>(gate + p.row * ld_gate + p.column, p.valid);
+  const Eight<T> u8 = load8<WIDE>(up + p.row * ld_up + p.column, p.valid);
   if (KEEP) {
-    keep<T>(gate8, shape, p, here, lane8, g);
-    keep<T>(up8, shape, p, here, lane8, u);
+    keep(gate8, shape, p, g8);
+    keep(up8, shape, p, u8);
   }
-  if (valid <= 0) return;
+  if (p.valid <= 0) return;
+  float g[8], u[8];
+  g8.get(g);
+  u8.get(u);
 #pragma unroll
   for (int i = 0; i < 8; ++i) u[i] *= g[i] * sigmoid<T>(g[i]);
-  write_eight(y + p.row * ld + p.column, valid, wide, u);
+  store8<WIDE>(y + p.row * ld + p.column, p.valid, u);
 }
 
-template <typename T, bool WITH_Y>
+template <typename T, bool WIDE, bool WITH_Y>
 __global__ void __launch_bounds__(kThreads)
 swiglu8_backward_kernel(const T* __restrict__ grad, int64_t ld_grad, Kept8 gate8, Kept8 up8, Shape shape, T* __restrict__ d_gate,
-                        T* __restrict__ d_up, T* __restrict__ y, int64_t ld, bool wide) {
+                        T* __restrict__ d_up, T* __restrict__ y, int64_t ld) {
   wait_for_predecessor();
   let_successor_start();
-  Place p{};
-  if (!shape.place(first_group(), threadIdx.x % kGroupThreads, p) || p.valid <= 0) return;
+  const Place p(shape);
+  if (p.valid <= 0) return;
   float d[8], g[8], u[8], out_g[8], out_u[8];
-  read_eight(grad + p.row * ld_grad + p.column, p.valid, wide, d);
-  kept_values(gate8, shape, p, g);
-  kept_values(up8, shape, p, u);
+  const Eight<T> d8 = load8<WIDE>(grad + p.row * ld_grad + p.column, p.valid);
+  kept_values(gate8, p, g);
+  kept_values(up8, p, u);
+  d8.get(d);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float s = sigmoid<T>(g[i]), silu = g[i] * s;
     out_u[i] = d[i] * silu;
-    out_g[i] = d[i] * u[i] * (s + silu * (1.f - s));
+    out_g[i] = d[i] * u[i] * fmaf(silu, 1.f - s, s);
     if (WITH_Y) u[i] *= silu;
   }
   const int64_t at = p.row * ld + p.column;
-  write_eight(d_gate + at, p.valid, wide, out_g);
-  write_eight(d_up + at, p.valid, wide, out_u);
-  if (WITH_Y) write_eight(y + at, p.valid, wide, u);
+  store8<WIDE>(d_gate + at, p.valid, out_g);
+  store8<WIDE>(d_up + at, p.valid, out_u);
+  if (WITH_Y) store8<WIDE>(y + at, p.valid, u);
 }
 
 bool on_16(const void* data, int64_t ld, int size) { return (reinterpret_cast<uintptr_t>(data) & 15) == 0 && (ld * size) % 16 == 0; }
 
 Shape shape_of(int64_t rows, int dim) {
   if (rows < 0 || dim < 1) throw std::invalid_argument("activation8: bad shape");
-  return Shape{rows, dim, (dim + kScaleGroup - 1) / kScaleGroup};
+  const int64_t groups = (static_cast<int64_t>(dim) + kScaleGroup - 1) / kScaleGroup;
+  if (rows * groups > INT32_MAX) throw std::invalid_argument("activation8: more than 2^31 - 1 groups of 64 values");
+  return Shape{static_cast<uint32_t>(rows * groups), dim, Divisor(static_cast<uint32_t>(groups))};
 }
 
 void check_kept(const Kept8& kept, int dim) {
@@ -190,25 +241,27 @@ void check_kept(const Kept8& kept, int dim) {
     throw std::invalid_argument("activation8: kept rows lie on 8-byte boundaries");
 }
 
-dim3 grid_of(const Shape& s) {
-  const int64_t blocks = (s.rows * s.groups * kGroupThreads + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffff) throw std::invalid_argument("activation8: too many values");
-  return dim3(static_cast<unsigned>(blocks));
-}
-
 template <typename... P, typename... A>
 void start(const char* what, void (*kernel)(P...), const Shape& shape, cudaStream_t stream, A&&... arguments) {
-  const cudaError_t err = launch_dependent(kernel, grid_of(shape), dim3(kThreads), 0, stream, std::forward<A>(arguments)...);
+  const dim3 grid((shape.count + kThreads / kGroupThreads - 1) / (kThreads / kGroupThreads));
+  const cudaError_t err = launch_dependent(kernel, grid, dim3(kThreads), 0, stream, std::forward<A>(arguments)...);
   if (err != cudaSuccess) throw std::runtime_error(std::string(what) + " launch: " + cudaGetErrorString(err));
 }
 
+// f(type, whether rows are wide)
 template <typename F>
-void for_type(int type, F f) {
-  if (type == kBf16) f(static_cast<__nv_bfloat16*>(nullptr));
-  else if (type == kFp16) f(static_cast<__half*>(nullptr));
-  else if (type == kFp32) f(static_cast<float*>(nullptr));
+void for_type(int type, bool wide, F f) {
+  auto with = [&](auto* t) {
+    if (wide) f(t, std::true_type{});
+    else f(t, std::false_type{});
+  };
+  if (type == kBf16) with(static_cast<__nv_bfloat16*>(nullptr));
+  else if (type == kFp16) with(static_cast<__half*>(nullptr));
+  else if (type == kFp32) with(static_cast<float*>(nullptr));
   else throw std::invalid_argument("activation8: unknown type");
 }
+
+int size_of(int type) { return type == kFp32 ? 4 : 2; }
 
 }  // namespace
 
@@ -216,9 +269,9 @@ void pack8(int type, const Rows& x, int64_t rows, int dim, const Kept8& kept, cu
   const Shape shape = shape_of(rows, dim);
   check_kept(kept, dim);
   if (rows == 0) return;
-  for_type(type, [&](auto* t) {
+  for_type(type, dim % 8 == 0 && on_16(x.data, x.ld, size_of(type)), [&](auto* t, auto wide) {
     using T = std::remove_pointer_t<decltype(t)>;
-    start("pack8", pack8_kernel<T>, shape, stream, static_cast<const T*>(x.data), x.ld, shape, kept, on_16(x.data, x.ld, sizeof(T)));
+    start("pack8", pack8_kernel<T, decltype(wide)::value>, shape, stream, static_cast<const T*>(x.data), x.ld, shape, kept);
   });
 }
 
@@ -226,9 +279,9 @@ void unpack8(int type, const Kept8& kept, int64_t rows, int dim, void* out, int6
   const Shape shape = shape_of(rows, dim);
   check_kept(kept, dim);
   if (rows == 0) return;
-  for_type(type, [&](auto* t) {
+  for_type(type, dim % 8 == 0 && on_16(out, ld, size_of(type)), [&](auto* t, auto wide) {
     using T = std::remove_pointer_t<decltype(t)>;
-    start("unpack8", unpack8_kernel<T>, shape, stream, kept, shape, static_cast<T*>(out), ld, on_16(out, ld, sizeof(T)));
+    start("unpack8", unpack8_kernel<T, decltype(wide)::value>, shape, stream, kept, shape, static_cast<T*>(out), ld);
   });
 }
 
@@ -240,12 +293,13 @@ void swiglu8_forward(int type, const Rows& gate, const Rows& up, int64_t rows, i
     check_kept(*up8, dim);
   }
   if (rows == 0) return;
-  for_type(type, [&](auto* t) {
+  const int size = size_of(type);
+  for_type(type, dim % 8 == 0 && on_16(gate.data, gate.ld, size) && on_16(up.data, up.ld, size) && on_16(y, ld, size), [&](auto* t, auto wide) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool wide = on_16(gate.data, gate.ld, sizeof(T)) && on_16(up.data, up.ld, sizeof(T)) && on_16(y, ld, sizeof(T));
-    start("swiglu8_forward", gate8 ? swiglu8_forward_kernel<T, true> : swiglu8_forward_kernel<T, false>, shape, stream,
+    constexpr bool kWide = decltype(wide)::value;
+    start("swiglu8_forward", gate8 ? swiglu8_forward_kernel<T, kWide, true> : swiglu8_forward_kernel<T, kWide, false>, shape, stream,
           static_cast<const T*>(gate.data), gate.ld, static_cast<const T*>(up.data), up.ld, shape, static_cast<T*>(y), ld,
-          gate8 ? *gate8 : Kept8{}, gate8 ? *up8 : Kept8{}, wide);
+          gate8 ? *gate8 : Kept8{}, gate8 ? *up8 : Kept8{});
   });
 }
 
@@ -255,13 +309,14 @@ void swiglu8_backward(int type, const Rows& grad, const Kept8& gate8, const Kept
   check_kept(gate8, dim);
   check_kept(up8, dim);
   if (rows == 0) return;
-  for_type(type, [&](auto* t) {
+  const int size = size_of(type);
+  for_type(type, dim % 8 == 0 && on_16(grad.data, grad.ld, size) && on_16(d_gate, ld, size) && on_16(d_up, ld, size) && (!y || on_16(y, ld, size)),
+           [&](auto* t, auto wide) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool wide = on_16(grad.data, grad.ld, sizeof(T)) && on_16(d_gate, ld, sizeof(T)) && on_16(d_up, ld, sizeof(T)) &&
-                      (!y || on_16(y, ld, sizeof(T)));
-    start("swiglu8_backward", y ? swiglu8_backward_kernel<T, true> : swiglu8_backward_kernel<T, false>, shape, stream,
+    constexpr bool kWide = decltype(wide)::value;
+    start("swiglu8_backward", y ? swiglu8_backward_kernel<T, kWide, true> : swiglu8_backward_kernel<T, kWide, false>, shape, stream,
           static_cast<const T*>(grad.data), grad.ld, gate8, up8, shape, static_cast<T*>(d_gate), static_cast<T*>(d_up),
-          static_cast<T*>(y), ld, wide);
+          static_cast<T*>(y), ld);
   });
 }
 
