@@ -115,8 +115,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const NormProblem p = norm_problem(x_rows, branch_rows, v, scale, eps, rms, status);
     residual_norm_forward(p, pointer(h), pointer(y), p.dim, current_stream());
     count(1);
-    // (a branch that is only added is not read again)
-    ctx->save_for_backward({branch.defined() ? h : x, branch_weight.defined() || gate.defined() ? branch : Tensor(), weight, branch_weight, gate, rms});
+    ctx->save_for_backward({x, branch, weight, branch_weight, gate, rms});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["want"] = std::move(want);
@@ -139,9 +138,9 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const c10::cuda::CUDAGuard guard(saved[0].device());
     const at::NoGradGuard no_grad;
     const auto want = ctx->saved_data["want"].toIntVector();
-    const Tensor h = rows_of(saved[0]), branch = saved[1].defined() ? rows_of(saved[1]) : Tensor();
+    const Tensor x = rows_of(saved[0]), branch = saved[1].defined() ? rows_of(saved[1]) : Tensor();
     const Tensor gh = grad_h.defined() ? rows_of(grad_h) : Tensor(), gy = grad_y.defined() ? rows_of(grad_y) : Tensor();
-    NormProblem p = norm_problem(h, branch, v, ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), saved[5],
+    NormProblem p = norm_problem(x, branch, v, ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), saved[5],
                                  ctx->saved_data["status"].toInt());
     // each gradient in memory of its own: where x and the branch are views of leaves, torch accumulates into what it is handed
     for (int i = 0; i < 2; ++i)
@@ -155,7 +154,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     g.blocks = residual_norm_blocks(p, g);
     Tensor partials;
     if (g.d_weight || g.d_branch_weight || g.d_gate) {
-      partials = at::empty({g.blocks, 2, p.dim}, h.options().dtype(at::kFloat));
+      partials = at::empty({g.blocks, 2, p.dim}, x.options().dtype(at::kFloat));
       g.partials = partials.data_ptr<float>();
       count(1);
     }

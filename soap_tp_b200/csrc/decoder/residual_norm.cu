@@ -1,6 +1,6 @@
 // h = x + s g * b',  b' = b or r_b b w_b;  y = r h w   with r = 1 / sqrt(mean(h^2) + eps), r_b the same of b.
 //
-// Backward, from the gradients of h and y, at the h that was stored and the r that was computed:
+// Backward, from the gradients of h and y; h comes from x and b once more (as it was stored it has 2^-9 less, and dw with it):
 //   t = dy w             dh = dh' + r (t - h r^2 mean(t h))          dw  = sum over rows of dy h r
 //   db' = s g dh         dg = sum of s dh b'                         dx  = dh
 //   t_b = db' w_b        db = r_b (t_b - b r_b^2 mean(t_b b))        dw_b = sum of db' b r_b
@@ -285,8 +285,9 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
   float* shared = sums[threadIdx.y];
   int turn = 0;
   Ring<T, 4> ring = make_ring<T, 4, RING>(d, p.dim, dynamic, bars);
+  const bool with_branch = p.branch.data != nullptr;
   ring.inputs[0] = g.grad_y; ring.inputs[1] = g.grad_y.data ? p.x : Rows{nullptr, 0};
-  ring.inputs[2] = g.grad_h; ring.inputs[3] = SCALED ? p.branch : Rows{nullptr, 0};
+  ring.inputs[2] = g.grad_h; ring.inputs[3] = SCALED || g.grad_y.data ? p.branch : Rows{nullptr, 0};
   wait_for_predecessor();
   let_successor_start();
   const float inverse_dim = 1.f / static_cast<float>(p.dim);
@@ -314,8 +315,13 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
     Lane<E, P> dh;
     if (g.grad_y.data) {
       Lane<E, P> h;
-      dh.load(ring.template row_at<RING>(0, row), p.dim);
       h.load(ring.template row_at<RING>(1, row), p.dim);
+      if (with_branch) {
+        dh.load(ring.template row_at<RING>(3, row), p.dim);
+#pragma unroll
+        for (int i = 0; i < P; ++i) fma_pair(h.v[i], SCALED ? mul_pair(dh.v[i], twice(r_b)) : dh.v[i], branch_factor.v[i]);
+      }
+      dh.load(ring.template row_at<RING>(0, row), p.dim);
       uint64_t dot = 0;
 #pragma unroll
       for (int i = 0; i < P; ++i) {

@@ -15,7 +15,7 @@ struct NormProblem {
   int64_t rows;
   int dim;
   float scale, eps;
-  Rows x;                         // the backward pass: h
+  Rows x;
   Rows branch;                    // null: h = x
   const void *weight, *branch_weight, *gate;      // any may be null
   float *rms, *branch_rms;        // [rows]: 1 / sqrt(mean of squares + eps), of h and of the branch

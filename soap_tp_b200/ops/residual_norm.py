@@ -86,7 +86,7 @@ def residual_norm(
 
     Without ``branch_weight`` the branch has no norm, without ``gate`` no gate; without ``weight`` there is no second norm and ``y`` is None.
     The vectors have ``x``'s dtype or are fp32.  Means, sums and the vectors' gradients are held in fp32; ``h`` and ``y`` are each
-    rounded once.  Differentiable once.
+    rounded once.  The backward pass keeps x, the branch and two numbers a row.  Differentiable once.
     """
     if branch is None:
         raise ValueError("residual_norm needs a branch; rms_norm is the norm alone.")

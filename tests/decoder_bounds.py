@@ -84,7 +84,7 @@ def norm_exact(x, branch, weight, branch_weight, gate, scale, eps, grad_h, grad_
     """Results and gradients of ``residual_norm`` with bounds, by name.
 
     fp32 sums over ``dim`` values in runs, lanes and warps: relative errors of ``c`` half steps with c = 64 + dim / 64 (a thread adds 32 values at
-    most one after another up to 32768, the rest is trees).  The backward pass uses h as it was stored: u of it more.
+    most one after another up to 32768, the rest is trees).
     """
     u, c = half_step(x.dtype), (64 + x.shape[-1] / 64) * F32
     v = {k: t.detach().double() for k, t in dict(x=x, b=branch, w=weight, wb=branch_weight, g=gate).items() if t is not None}
@@ -107,14 +107,14 @@ def norm_exact(x, branch, weight, branch_weight, gate, scale, eps, grad_h, grad_
         gy = grad_y.double() if grad_y is not None else torch.zeros_like(h)
         t = gy * w
         mean, mean_abs = (t * h).mean(-1, keepdim=True), (t.abs() * mh).mean(-1, keepdim=True)
-        stored = u * h.abs() + c * mh
+        again = c * mh                                  # h, computed once more
         dh = gh + r * (t - h * r * r * mean)
-        e_dh = c * gh.abs() + r * (c + e_r) * t.abs() + r ** 3 * ((u + 4 * c + 3 * e_r) * mh * mean_abs + stored * mean_abs
-                                                                  + h.abs() * (t.abs() * stored).mean(-1, keepdim=True))
+        e_dh = c * gh.abs() + r * (c + e_r) * t.abs() + r ** 3 * ((4 * c + 3 * e_r) * mh * mean_abs + again * mean_abs
+                                                                  + h.abs() * (t.abs() * again).mean(-1, keepdim=True))
         dw = (gy * h * r).sum(0)
         e_sum = (64 + x.shape[0] / 8) * F32             # rows one after another in a block, blocks in eight slices
         out["weight"] = (dw, (u if weight.dtype == x.dtype else F32) * dw.abs()
-                         + (gy.abs() * r * (stored + (c + e_r + e_sum) * mh)).sum(0) + smallest(weight.dtype))
+                         + (gy.abs() * r * (again + (c + e_r + e_sum) * mh)).sum(0) + smallest(weight.dtype))
     out["x"] = (dh, u * dh.abs() + e_dh + smallest(x.dtype))
     dn = scale * g * dh
     e_dn = abs(scale) * g.abs() * (e_dh + 2 * F32 * dh.abs())
