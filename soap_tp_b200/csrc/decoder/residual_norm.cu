@@ -120,6 +120,10 @@ __device__ __forceinline__ float row_sum(float v, float* shared, int& turn) {
   if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
   row_sync();
   const int warps = blockDim.x >> 5;
+  if (warps == 8) {      // (rows of 2049 to 4096 values: two wide loads are sooner done than another round of shuffles)
+    const float4 a = *reinterpret_cast<const float4*>(slot), b = *reinterpret_cast<const float4*>(slot + 4);
+    return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+  }
   v = (threadIdx.x & 31) < warps ? slot[threadIdx.x & 31] : 0.f;
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -137,7 +141,7 @@ struct Deal {
 };
 
 // The rows of up to four matrices, one row of each a stage.  INPUTS that are absent have a null base.
-template <typename T, int INPUTS>
+template <typename T, int INPUTS, int E>
 struct Ring {
   Rows inputs[INPUTS];
   uint8_t* data;
@@ -168,7 +172,7 @@ struct Ring {
   }
   // Input `i` of the current row.
   __device__ __forceinline__ const T* at(int i, int64_t row) const {
-    return reinterpret_cast<const T*>(data + (stage * INPUTS + i) * row_bytes + (address(i, row) & 15));
+    return reinterpret_cast<const T*>(data + (stage * INPUTS + i) * row_bytes + (E == 8 ? 0 : address(i, row) & 15));
   }
   template <bool RING>
   __device__ __forceinline__ const T* row_at(int i, int64_t row) const {
@@ -196,9 +200,9 @@ struct Ring {
   }
 };
 
-template <typename T, int INPUTS, bool RING>
-__device__ __forceinline__ Ring<T, INPUTS> make_ring(const Deal& d, int dim, uint8_t* dynamic, uint64_t (&bars)[kMostGroups][kMostStages]) {
-  Ring<T, INPUTS> ring;
+template <typename T, int INPUTS, int E, bool RING>
+__device__ __forceinline__ Ring<T, INPUTS, E> make_ring(const Deal& d, int dim, uint8_t* dynamic, uint64_t (&bars)[kMostGroups][kMostStages]) {
+  Ring<T, INPUTS, E> ring;
   ring.stages = d.stages; ring.row_bytes = d.row_bytes; ring.dim = dim;
   ring.data = dynamic + static_cast<int64_t>(threadIdx.y) * d.stages * INPUTS * d.row_bytes;
   ring.full = bars[threadIdx.y];
@@ -225,13 +229,13 @@ __device__ __forceinline__ void load_vectors(const NormProblem& p, Lane<E, P>& w
 }
 
 template <typename T, int E, int P, int THREADS, bool RING, bool AFTER>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) residual_norm_forward_kernel(NormProblem p, T* __restrict__ h_out, T* __restrict__ y_out, int64_t ld, Deal d) {
-  __shared__ float sums[kMostGroups][64];
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) residual_norm_forward_kernel(NormProblem p, T* __restrict__ h_out, T* __restrict__ y_out, int64_t ld, Deal d) {
+  __shared__ __align__(16) float sums[kMostGroups][64];
   __shared__ uint64_t bars[kMostGroups][kMostStages];
   extern __shared__ __align__(128) uint8_t dynamic[];
   float* shared = sums[threadIdx.y];
   int turn = 0;
-  Ring<T, 2> ring = make_ring<T, 2, RING>(d, p.dim, dynamic, bars);
+  Ring<T, 2, E> ring = make_ring<T, 2, E, RING>(d, p.dim, dynamic, bars);
   ring.inputs[0] = p.x; ring.inputs[1] = p.branch;
   wait_for_predecessor();
   let_successor_start();
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) residual_norm
         uint64_t squares = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) fma_pair(squares, b.v[i], b.v[i]);
-        r_b = 1.f / sqrtf(row_sum(sum_of(squares), shared, turn) * inverse_dim + p.eps);
+        r_b = rsqrtf(row_sum(sum_of(squares), shared, turn) * inverse_dim + p.eps);
         if (threadIdx.x == 0) p.branch_rms[row] = r_b;
       }
 #pragma unroll
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) residual_norm
       uint64_t squares = 0;
 #pragma unroll
       for (int i = 0; i < P; ++i) fma_pair(squares, h.v[i], h.v[i]);
-      const float r = 1.f / sqrtf(row_sum(sum_of(squares), shared, turn) * inverse_dim + p.eps);
+      const float r = rsqrtf(row_sum(sum_of(squares), shared, turn) * inverse_dim + p.eps);
       if (threadIdx.x == 0) p.rms[row] = r;
 #pragma unroll
       for (int i = 0; i < P; ++i) h.v[i] = mul_pair(mul_pair(h.v[i], twice(r)), weight.v[i]);
@@ -279,12 +283,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) residual_norm
 template <typename T, int E, int P, int THREADS, bool RING, bool SCALED>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
-  __shared__ float sums[kMostGroups][64];
+  __shared__ __align__(16) float sums[kMostGroups][64];
   __shared__ uint64_t bars[kMostGroups][kMostStages];
   extern __shared__ __align__(128) uint8_t dynamic[];
   float* shared = sums[threadIdx.y];
   int turn = 0;
-  Ring<T, 4> ring = make_ring<T, 4, RING>(d, p.dim, dynamic, bars);
+  Ring<T, 4, E> ring = make_ring<T, 4, E, RING>(d, p.dim, dynamic, bars);
   const bool with_branch = p.branch.data != nullptr;
   ring.inputs[0] = g.grad_y; ring.inputs[1] = g.grad_y.data ? p.x : Rows{nullptr, 0};
   ring.inputs[2] = g.grad_h; ring.inputs[3] = SCALED || g.grad_y.data ? p.branch : Rows{nullptr, 0};
@@ -519,7 +523,7 @@ void for_deal(const Deal& d, F f) {
 
 Deal forward_deal(const NormProblem& p, const void* h, const void* y, int64_t ld) {
   const int size = size_of(p.type);
-  return deal_of(wide_problem(p) && on_16(h, ld, size) && on_16(y, ld, size), p.rows, p.dim, size, 2, 3);
+  return deal_of(wide_problem(p) && on_16(h, ld, size) && on_16(y, ld, size), p.rows, p.dim, size, 2, 2);
 }
 Deal backward_deal(const NormProblem& p, const NormGradients& g) {
   const int size = size_of(p.type);
