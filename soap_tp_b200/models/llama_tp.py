@@ -14,6 +14,11 @@ with SOAP-TP on every 2-D weight" needs one, so this module provides it:
 
 Every 2-D weight carries ``tp_shard_dim`` and ``tp_global_shape`` so the optimizer can hand it to
 ``soap_step`` unchanged.  Works on CPU (gloo) for tests and on CUDA (NCCL) for training.
+
+What is not a plain product can run on the package's own operators instead of eager torch, each switched on by an attribute of
+``LlamaTP`` (all off, and the results then those of eager torch): ``fused_loss`` (the head's cross entropy without logits),
+``fused_norms`` (residual sums, norms, gates in one pass), ``mlp_bits = 8`` and ``checkpoint_bits = 8`` (the MLPs' inputs of the down
+projection, and the blocks' inputs where activations are checkpointed, kept in 8 bits).
 """
 from __future__ import annotations
 
@@ -28,6 +33,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from ..ops.activation8 import checkpoint8, swiglu_linear8
+from ..ops.linear_cross_entropy import linear_cross_entropy
+from ..ops.residual_norm import residual_norm, rms_norm
+
 
 @dataclass
 class LlamaConfig:
@@ -40,6 +49,10 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     rms_eps: float = 1e-5
     max_seq_len: int = 4096
+    # between a block's output and the residual sum: a norm, a learnt gate for each feature, a scale for all
+    norm_after: bool = False
+    gated_residual: bool = False
+    residual_scale: float = 1.0
 
     @staticmethod
     def llama3_8b(**overrides) -> "LlamaConfig":
@@ -228,6 +241,8 @@ class Attention(nn.Module):
 
 
 class MLP(nn.Module):
+    bits = 16        # 8: gate and up are kept in 8 bits for the backward pass, and the down projection's input is not kept
+
     def __init__(self, cfg: LlamaConfig, *, dtype, device, std: float, out_std: float) -> None:
         super().__init__()
         self.gate_proj = ColumnParallelLinear(cfg.hidden_size, cfg.intermediate_size, dtype=dtype, device=device, std=std)
@@ -235,7 +250,31 @@ class MLP(nn.Module):
         self.down_proj = RowParallelLinear(cfg.intermediate_size, cfg.hidden_size, dtype=dtype, device=device, std=out_std)
 
     def forward(self, x: Tensor) -> Tensor:
+        if self.bits == 8:
+            return _ReduceFromTensorParallel.apply(swiglu_linear8(self.gate_proj(x), self.up_proj(x), self.down_proj.weight))
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+
+
+class Residual(nn.Module):
+    """What lies between a block's output and the residual sum, where anything does."""
+
+    def __init__(self, cfg: LlamaConfig, *, dtype, device) -> None:
+        super().__init__()
+        self.scale = cfg.residual_scale
+        self.norm = RMSNorm(cfg.hidden_size, cfg.rms_eps, dtype=dtype, device=device) if cfg.norm_after else None
+        self.gate = nn.Parameter(torch.ones(cfg.hidden_size, dtype=dtype, device=device)) if cfg.gated_residual else None
+
+    def forward(self, x: Tensor, branch: Tensor) -> Tensor:
+        if self.norm is not None:
+            branch = self.norm(branch)
+        if self.gate is not None:
+            branch = branch * self.gate
+        return x + branch if self.scale == 1.0 else x + self.scale * branch
+
+    def fused(self, x: Tensor, branch: Tensor, weight: Optional[Tensor], eps: float) -> tuple[Tensor, Optional[Tensor]]:
+        """The sum, and its norm times ``weight`` if there is one."""
+        return residual_norm(x, branch, weight, branch_weight=None if self.norm is None else self.norm.weight, gate=self.gate,
+                             scale=self.scale, eps=eps)
 
 
 class Block(nn.Module):
@@ -243,12 +282,23 @@ class Block(nn.Module):
         super().__init__()
         self.input_norm = RMSNorm(cfg.hidden_size, cfg.rms_eps, dtype=dtype, device=device)
         self.attention = Attention(cfg, dtype=dtype, device=device, std=std, out_std=out_std)
+        self.attention_residual = Residual(cfg, dtype=dtype, device=device)
         self.post_norm = RMSNorm(cfg.hidden_size, cfg.rms_eps, dtype=dtype, device=device)
         self.mlp = MLP(cfg, dtype=dtype, device=device, std=std, out_std=out_std)
+        self.mlp_residual = Residual(cfg, dtype=dtype, device=device)
+        self.eps = cfg.rms_eps
 
     def forward(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
-        x = x + self.attention(self.input_norm(x), cos, sin)
-        return x + self.mlp(self.post_norm(x))
+        x = self.attention_residual(x, self.attention(self.input_norm(x), cos, sin))
+        return self.mlp_residual(x, self.mlp(self.post_norm(x)))
+
+    def fused(self, x: Tensor, normed: Tensor, next_weight: Optional[Tensor], cos: Tensor, sin: Tensor) -> tuple[Tensor, Optional[Tensor]]:
+        """The block on its normed input; the sum that leaves it, and that sum's norm times ``next_weight``."""
+        x, normed = self.attention_residual.fused(x, self.attention(normed, cos, sin), self.post_norm.weight, self.eps)
+        return self.mlp_residual.fused(x, self.mlp(normed), next_weight, self.eps)
+
+    def fused_from_sum(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
+        return self.fused(x, rms_norm(x, self.input_norm.weight, self.eps), None, cos, sin)[0]
 
 
 class LlamaTP(nn.Module):
@@ -268,18 +318,60 @@ class LlamaTP(nn.Module):
         # recompute every block in the backward pass instead of keeping its activations (32 layers at sequence
         # length 4096 and batch 8 would otherwise hold over 100 GB of activations per rank)
         self.checkpoint_activations = False
+        self.checkpoint_bits = 16      # 8: what is kept of a checkpointed block is its input in 8 bits
+        self.fused_loss = False        # the head's cross entropy without logits
+        self.fused_norms = False       # residual sums and norms in one pass
+
+    @property
+    def mlp_bits(self) -> int:
+        return self.blocks[0].mlp.bits if len(self.blocks) else 16
+
+    @mlp_bits.setter
+    def mlp_bits(self, bits: int) -> None:
+        if bits not in (8, 16):
+            raise ValueError(f"mlp_bits must be 8 or 16, got {bits}.")
+        for block in self.blocks:
+            block.mlp.bits = bits
+
+    def _checkpointed(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
+        for block in self.blocks:
+            function = block.fused_from_sum if self.fused_norms else block
+            if self.checkpoint_bits == 8:
+                x = checkpoint8(function, x, cos, sin, parameters=block.parameters())
+            else:
+                x = torch.utils.checkpoint.checkpoint(function, x, cos, sin, use_reentrant=False)
+        return x
+
+    def _normed(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
+        """All blocks and the final norm."""
+        if self.checkpoint_bits not in (8, 16):
+            raise ValueError(f"checkpoint_bits must be 8 or 16, got {self.checkpoint_bits}.")
+        checkpointed = self.checkpoint_activations and torch.is_grad_enabled()
+        if checkpointed:
+            x = self._checkpointed(x, cos, sin)
+        if not self.fused_norms:
+            if not checkpointed:
+                for block in self.blocks:
+                    x = block(x, cos, sin)
+            return self.final_norm(x)
+        final = self.final_norm.weight
+        if checkpointed or not len(self.blocks):
+            return rms_norm(x, final, self.cfg.rms_eps)
+        # every residual sum meets the norm that follows it, the next block's or the final one
+        weights = [block.input_norm.weight for block in self.blocks] + [final]
+        normed = rms_norm(x, weights[0], self.cfg.rms_eps)
+        for block, weight in zip(self.blocks, weights[1:]):
+            x, normed = block.fused(x, normed, weight, cos, sin)
+        return normed
 
     def forward(self, tokens: Tensor, targets: Optional[Tensor] = None) -> Tensor:
         """Mean next-token loss if ``targets`` is given, else this rank's slice of the logits."""
         _, seq = tokens.shape
         cos, sin = rope_tables(self.cfg.hidden_size // self.cfg.num_heads, seq, self.cfg.rope_theta, tokens.device)
-        x = self.embed(tokens)
-        for block in self.blocks:
-            if self.checkpoint_activations and torch.is_grad_enabled():
-                x = torch.utils.checkpoint.checkpoint(block, x, cos, sin, use_reentrant=False)
-            else:
-                x = block(x, cos, sin)
-        logits = self.lm_head(self.final_norm(x))
+        normed = self._normed(self.embed(tokens), cos, sin)
+        if targets is not None and self.fused_loss:
+            return linear_cross_entropy(normed, self.lm_head.weight, targets, group=dist.group.WORLD if _world() > 1 else None)
+        logits = self.lm_head(normed)
         if targets is None:
             return logits
         return _VocabParallelCrossEntropy.apply(logits, targets, self.vocab_start).mean()

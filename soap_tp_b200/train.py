@@ -42,7 +42,16 @@ def parse_args(argv=None) -> argparse.Namespace:
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--checkpoint-activations", action="store_true",
                         help="recompute each decoder block in the backward pass (needed for all 32 layers of the 8B preset)")
-    return parser.parse_args(argv)
+    parser.add_argument("--checkpoint-bits", type=int, choices=(8, 16), default=16,
+                        help="with --checkpoint-activations: 8 keeps the blocks' inputs in 8 bits")
+    parser.add_argument("--mlp-bits", type=int, choices=(8, 16), default=16,
+                        help="8 keeps the MLPs' activations in 8 bits for the backward pass")
+    parser.add_argument("--fused-norms", action="store_true", help="residual sums and norms in one pass over memory")
+    parser.add_argument("--fused-loss", action="store_true", help="the head's cross entropy without logits")
+    args = parser.parse_args(argv)
+    if args.checkpoint_bits == 8 and not args.checkpoint_activations:
+        parser.error("--checkpoint-bits 8 needs --checkpoint-activations")
+    return args
 
 
 def train(args: argparse.Namespace) -> dict:
@@ -65,6 +74,8 @@ def train(args: argparse.Namespace) -> dict:
     dtype = torch.bfloat16 if args.device == "cuda" else torch.float32
     model = LlamaTP(cfg, dtype=dtype, device=device, seed=args.seed)
     model.checkpoint_activations = bool(args.checkpoint_activations)
+    model.checkpoint_bits, model.mlp_bits = args.checkpoint_bits, args.mlp_bits
+    model.fused_norms, model.fused_loss = args.fused_norms, args.fused_loss
     matrices, others = model.soap_parameters()
     optimizer = SoapTP(
         [{"params": matrices}, {"params": others, "weight_decay": 0.0}],
