@@ -310,13 +310,6 @@ scale_gradients_kernel(const float* __restrict__ factor, __nv_bfloat16* __restri
   }
 }
 
-int sms_of_device() {
-  int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    throw std::runtime_error("cross entropy: no device");
-  return sms;
-}
-
 Hidden16 hidden_of(const HeadProblem& p, int first) {
   const int64_t at = static_cast<int64_t>(first);
   return Hidden16{Matrix16{static_cast<const uint16_t*>(p.packed.data) + at * p.packed.ld, p.packed.ld, true},
@@ -340,7 +333,7 @@ void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaS
   check(launch_dependent(head_count_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.targets, p.tokens, p.ignore_index, p.first_word,
                          p.words, p.vocabulary, p.count, p.where, p.column, p.split_counters),
         "head_count");
-  const int blocks = std::min((p.tokens + 7) / 8, 8 * sms_of_device());
+  const int blocks = std::min((p.tokens + 7) / 8, 8 * multiprocessors());
   check(launch_dependent(head_gather_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<const uint16_t*>(p.hidden.data), p.hidden.ld,
                          p.tokens, p.depth, p.targets, p.ignore_index, p.count, p.where,
                          static_cast<uint16_t*>(const_cast<void*>(p.packed.data)), p.packed.ld, static_cast<uint16_t*>(d_hidden), ld_hidden),
@@ -436,7 +429,7 @@ void scale_gradients(const float* factor, void* a, int64_t count_a, void* b, int
     throw std::invalid_argument("scale_gradients: matrices lie on 16-byte boundaries");
   const int64_t runs = (count_a + 7) / 8 + (count_b + 7) / 8;
   if (runs == 0) return;
-  const int blocks = static_cast<int>(std::min<int64_t>((runs + kScaleThreads - 1) / kScaleThreads, 8 * sms_of_device()));
+  const int blocks = static_cast<int>(std::min<int64_t>((runs + kScaleThreads - 1) / kScaleThreads, 8 * multiprocessors()));
   check(launch_dependent(scale_gradients_kernel, dim3(blocks), dim3(kScaleThreads), 0, stream, factor, static_cast<__nv_bfloat16*>(a), count_a,
                          static_cast<__nv_bfloat16*>(b), count_b),
         "scale_gradients");

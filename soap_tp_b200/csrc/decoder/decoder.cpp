@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstring>
 #include <functional>
 #include <optional>
 #include <vector>
@@ -75,6 +76,17 @@ Rows address(const Tensor& rows) { return rows.defined() ? Rows{rows.data_ptr(),
 void* pointer(const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; }
 Tensor like_rows(const Tensor& x) { return at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous); }
 
+int64_t bits_of(double value) {
+  int64_t bits;
+  std::memcpy(&bits, &value, sizeof bits);
+  return bits;
+}
+double double_of(int64_t bits) {
+  double value;
+  std::memcpy(&value, &bits, sizeof value);
+  return value;
+}
+
 Tensor given(const std::optional<Tensor>& x) { return x ? *x : Tensor(); }
 
 // ---- norms --------------------------------------------------------------------------------------------------------------
@@ -116,11 +128,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     residual_norm_forward(p, pointer(h), pointer(y), p.dim, current_stream());
     count(1);
     ctx->save_for_backward({x, branch, weight, branch_weight, gate, rms});
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["want"] = std::move(want);
-    ctx->saved_data["branch"] = branch.defined();
-    ctx->saved_data["status"] = status;
+    want.insert(want.end(), {branch.defined(), status, bits_of(scale), bits_of(eps)});      // (one look-up in the backward pass)
+    ctx->saved_data["numbers"] = std::move(want);
     ctx->set_materialize_grads(false);
     variable_list out;
     for (const Tensor* t : {&h, &y})
@@ -131,17 +140,17 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(9);
     const auto saved = ctx->get_saved_variables();
-    const bool graph = at::GradMode::is_enabled(), with_branch = ctx->saved_data["branch"].toBool();
+    const auto numbers = ctx->saved_data["numbers"].toIntVector();
+    const int64_t* want = numbers.data();
+    const bool graph = at::GradMode::is_enabled(), with_branch = numbers[5];
     const Tensor grad_h = with_branch ? grads[0] : Tensor(), grad_y = saved[2].defined() ? grads[with_branch ? 1 : 0] : Tensor();
     if (!grad_h.defined() && !grad_y.defined()) return out;
     const Vectors v{saved[2], saved[3], saved[4]};
     const c10::cuda::CUDAGuard guard(saved[0].device());
     const at::NoGradGuard no_grad;
-    const auto want = ctx->saved_data["want"].toIntVector();
     const Tensor x = rows_of(saved[0]), branch = saved[1].defined() ? rows_of(saved[1]) : Tensor();
     const Tensor gh = grad_h.defined() ? rows_of(grad_h) : Tensor(), gy = grad_y.defined() ? rows_of(grad_y) : Tensor();
-    NormProblem p = norm_problem(x, branch, v, ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), saved[5],
-                                 ctx->saved_data["status"].toInt());
+    NormProblem p = norm_problem(x, branch, v, double_of(numbers[7]), double_of(numbers[8]), saved[5], numbers[6]);
     // each gradient in memory of its own: where x and the branch are views of leaves, torch accumulates into what it is handed
     for (int i = 0; i < 2; ++i)
       if (want[i]) out[i] = like_rows(saved[0]);

@@ -9,6 +9,10 @@
 // Operands whose M or N runs along memory's rows go in as they lie (kUmmaMnMajorA, kUmmaMnMajorB): the gradients' products
 // read the logits' gradient in both directions, and no matrix is transposed.
 //
+// What bounds it: a pair's tile takes 64 KB of L2's bandwidth every 512 cycles of products, 64 bytes a cycle and SM, which is all that an SM gets; and
+// the power cap in long runs.  8192 x 4096 x 128256 alone 1.31 PFLOP/s (torch.matmul 1.55), for seconds 1.17 to 1.23 (1.38).  Fetching tiles into L2
+// ahead of their loads only adds to that (4096 x 4096 x 16032: 416 -> 493 us).
+//
 // The tensor core truncates as it adds: some 2^-24 of the running sum per 16 of K.  Logits are drained from TMEM into sums in registers (round
 // to nearest) every 2048 of K, gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
 // Draining every 256 of K costs 150 of 690 thousand cycles at 4096 x 16032 x 4096: handing the accumulator over takes the tensor core about
@@ -284,6 +288,31 @@ __device__ __forceinline__ int drain_blocks(int left) {
   return (left + drains - 1) / drains;
 }
 
+// A producer's way through its units, k-block by k-block.
+struct Cursor {
+  const Units& units;
+  const Tiles& tiles;
+  int cta, unit, step, kb, end, m0, n0;
+  __device__ __forceinline__ Cursor(const Units& units_, const Tiles& tiles_, int cta_, int first, int step_)
+      : units(units_), tiles(tiles_), cta(cta_), unit(first - step_), step(step_), kb(0), end(0) { settle(); }
+  __device__ __forceinline__ bool done() const { return unit >= units.count(); }
+  __device__ __forceinline__ void settle() {
+    while (kb >= end) {
+      unit += step;
+      if (done()) return;
+      int tile, part;
+      units.place(unit, tile, kb, end, part);
+      tiles.place(tile, m0, n0);
+      m0 += cta * kRows;
+      n0 += cta * kRows;
+    }
+  }
+  __device__ __forceinline__ void advance() {
+    ++kb;
+    settle();
+  }
+};
+
 template <int EPI, bool A_K, bool B_K, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Epi<EPI != kStore16>::kThreads, 1)
 gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_all,
@@ -349,38 +378,29 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
       // ---------------- TMA producer (each CTA its own rows; the bytes are credited to the leader) ----------------
       int s = 0;
       uint32_t parity = 1;
-      bool first_round = true, ok = true;
-      for (int u = cluster; u < units.count() && ok; u += clusters) {
-        int m0, n0, tile, begin, end, part;
-        units.place(u, tile, begin, end, part);
-        tiles.place(tile, m0, n0);
-        m0 += cta * kRows;
-        n0 += cta * kRows;
-        for (int kb = begin; kb < end; ++kb) {
-          if (!first_round && !mbar_wait_bounded(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) {
-            ok = false;
-            break;
-          }
-          uint8_t* stage = smem + s * kStageBytes;
-          if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
-          const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
-          if constexpr (A_K) {
-            tma_load_2d_pair(stage, source_a, bar, kb * kBK, m0);
-          } else {
-            tma_load_2d_pair(stage, source_a, bar, m0, kb * kBK);
-            tma_load_2d_pair(stage + kOperandBytes / 2, source_a, bar, m0 + 64, kb * kBK);
-          }
-          if constexpr (B_K) {
-            tma_load_2d_pair(stage + kOperandBytes, source_b, bar, kb * kBK, n0);
-          } else {
-            tma_load_2d_pair(stage + kOperandBytes, source_b, bar, n0, kb * kBK);
-            tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, source_b, bar, n0 + 64, kb * kBK);
-          }
-          if (++s == kStages) {
-            s = 0;
-            parity ^= 1;
-            first_round = false;
-          }
+      bool first_round = true;
+      Cursor at(units, tiles, cta, cluster, clusters);
+      for (; !at.done(); at.advance()) {
+        if (!first_round && !mbar_wait_parked(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) break;
+        uint8_t* stage = smem + s * kStageBytes;
+        if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
+        const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
+        if constexpr (A_K) {
+          tma_load_2d_pair(stage, source_a, bar, at.kb * kBK, at.m0);
+        } else {
+          tma_load_2d_pair(stage, source_a, bar, at.m0, at.kb * kBK);
+          tma_load_2d_pair(stage + kOperandBytes / 2, source_a, bar, at.m0 + 64, at.kb * kBK);
+        }
+        if constexpr (B_K) {
+          tma_load_2d_pair(stage + kOperandBytes, source_b, bar, at.kb * kBK, at.n0);
+        } else {
+          tma_load_2d_pair(stage + kOperandBytes, source_b, bar, at.n0, at.kb * kBK);
+          tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, source_b, bar, at.n0 + 64, at.kb * kBK);
+        }
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+          first_round = false;
         }
       }
       if (*abort_flag) {
@@ -404,7 +424,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         units.place(u, tile, begin, end, part);
         for (int kb = begin; kb < end && ok; ++it) {
           const int buf = it & 1;
-          if (it >= 2 && !drained && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
+          if (it >= 2 && !drained && !mbar_wait_parked(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
             ok = false;
             break;
           }
@@ -412,7 +432,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
           const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
           const int blocks = drain_blocks<kLogits>(end - kb);
           for (int i = 0; i < blocks; ++i, ++kb) {
-            if (!loaded && !mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
+            if (!loaded && !mbar_wait_parked(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
               ok = false;
               break;
             }
@@ -450,7 +470,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(col0);
     int it = 0;
     auto filled = [&]() {
-      if (!mbar_wait_bounded(&acc_full[it & 1], (it >> 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) return false;
+      if (!mbar_wait_parked(&acc_full[it & 1], (it >> 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) return false;
       tc_fence_after_sync();
       return true;
     };
@@ -503,15 +523,18 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
           product_epilogue<T>(prob, M, m_warp, n0 + col0, mine, lane, accumulated);
           if (!empty) release();
         } else {
-          // This part's sums, 256 x 256 of them a part; the warp that is the last to leave its region of the tile adds the parts up in order.
-          const int row = cta * kRows + quarter * 32;
+          // This part's sums, 256 x 256 of them a part, as the registers hold them: a line of 32 lanes for each column of a warp's region.  The
+          // warp that is the last to leave its region of the tile adds the parts up in order.
+          constexpr int64_t kRegion = 32 * E::kColumns;
+          const int64_t region = static_cast<int64_t>(cta * E::kWarps + ew) * kRegion + lane;
           const int first = (tile - units.whole) * units.split;
+          float* mine_of = prob.split_parts + part * int64_t{kTile * kTile} + region;
 #pragma unroll
           for (int at = 0; at < E::kColumns; at += 32) {
             uint32_t raw[32];
             accumulated(at, raw);
-            store_lines<128>(mine, raw, reinterpret_cast<uint8_t*>(prob.split_parts + part * int64_t{kTile * kTile} + col0 + at), kTile * 4, nullptr,
-                             row, 32, 128, 4, true, lane);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) mine_of[(at + j) * 32] = __uint_as_float(raw[j]);
           }
           release();
           __threadfence();
@@ -526,16 +549,10 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             product_epilogue<T>(prob, M, m_warp, n0 + col0, mine, lane, [&](int at, uint32_t (&raw)[32]) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) raw[j] = 0;
-              for (int i = 0; i < units.split; ++i) {
-                const float* from_part = prob.split_parts + (first + i) * int64_t{kTile * kTile} + (row + lane) * kTile + col0 + at;
+              const float* from_part = prob.split_parts + first * int64_t{kTile * kTile} + region + at * 32;
+              for (int i = 0; i < units.split; ++i, from_part += kTile * kTile) {
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                  const float4 v = __ldcg(reinterpret_cast<const float4*>(from_part + j));
-                  raw[j] = __float_as_uint(__uint_as_float(raw[j]) + v.x);
-                  raw[j + 1] = __float_as_uint(__uint_as_float(raw[j + 1]) + v.y);
-                  raw[j + 2] = __float_as_uint(__uint_as_float(raw[j + 2]) + v.z);
-                  raw[j + 3] = __float_as_uint(__uint_as_float(raw[j + 3]) + v.w);
-                }
+                for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) + __ldcg(from_part + j * 32));
               }
             });
           }
@@ -559,13 +576,6 @@ CUtensorMap map_of(bool bf16, const Matrix16& x, int64_t rows, int64_t K) {
                    : encode_k_major(type, x.data, rows, K, 2 * x.ld, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-int pairs_of_device() {
-  int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    throw std::runtime_error("gemm16: no device");
-  return sms / 2;
-}
-
 template <int EPI, bool A_K, bool B_K, typename T>
 void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* status, cudaStream_t stream, const Hidden16* hidden) {
   static PerDeviceOnce configured;
@@ -577,7 +587,7 @@ void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* s
   if (tiles > (1 << 30)) throw std::invalid_argument("gemm16: too many tiles");
   // (where tokens are left out there may be fewer tiles in the end than here, and more parts of one)
   const int64_t parts = p.split_parts ? std::max(1, std::min(Units::kMostSplit, (p.K + kBK - 1) / kBK / Units::kLeastBlocks)) : 1;
-  const int clusters = static_cast<int>(std::min<int64_t>(tiles * parts, pairs_of_device()));
+  const int clusters = static_cast<int>(std::min<int64_t>(tiles * parts, multiprocessors() / 2));
   cudaError_t err = launch_dependent(gemm16_kernel<EPI, A_K, B_K, T>, dim3(2 * clusters), dim3(Epi<EPI != kStore16>::kThreads), kSmemBytes, stream, map_a,
                                      map_b, map_all, hidden ? hidden->tokens : -1, p, status);
   if (err != cudaSuccess) throw std::runtime_error(std::string("gemm16 launch: ") + cudaGetErrorString(err));

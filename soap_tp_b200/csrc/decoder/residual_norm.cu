@@ -434,13 +434,6 @@ __global__ void __launch_bounds__(32 * kSumSlices) norm_vectors_kernel(NormProbl
   }
 }
 
-int sms_of_device() {
-  int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    throw std::runtime_error("residual_norm: no device");
-  return sms;
-}
-
 // A warp for every 512 values, rounded up to a power of two, with 16 values a thread.  Blocks of eight warps share an SM's shared memory by
 // twos or threes (a backward pass's registers allow two).
 constexpr int kRingBytes = 216 * 1024;      // of an SM's 227 KB
@@ -461,7 +454,7 @@ Deal deal_of(bool wide, int64_t rows, int dim, int size, int inputs, int residen
     if (d.stages < 2 || warps > 16) continue;
     d.ring = true;
     d.smem = static_cast<int>(d.stages * stage);
-    d.blocks = static_cast<int>(std::min<int64_t>((rows + d.groups - 1) / d.groups, int64_t{ctas} * sms_of_device()));
+    d.blocks = static_cast<int>(std::min<int64_t>((rows + d.groups - 1) / d.groups, int64_t{ctas} * multiprocessors()));
   }
   if (d.ring) return d;
   d.stages = d.row_bytes = 0;
@@ -470,7 +463,7 @@ Deal deal_of(bool wide, int64_t rows, int dim, int size, int inputs, int residen
   if (dim > 1024 * d.values) throw std::invalid_argument("residual_norm: rows of more than 32768 values are not supported");
   d.threads = ((dim + d.values - 1) / d.values + 31) / 32 * 32;
   d.bound = 1024;
-  d.blocks = static_cast<int>(std::min<int64_t>(rows, 2 * sms_of_device()));
+  d.blocks = static_cast<int>(std::min<int64_t>(rows, 2 * multiprocessors()));
   return d;
 }
 

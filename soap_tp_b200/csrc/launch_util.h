@@ -26,6 +26,19 @@ inline void allow_dynamic_smem(const void* kernel, size_t bytes, PerDeviceOnce& 
   if (tracked) once.done[device] = true;
 }
 
+// Multiprocessors of the current device.
+inline int multiprocessors() {
+  static int known[PerDeviceOnce::kMaxDevices] = {};
+  int device = 0, count = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  const bool tracked = device >= 0 && device < PerDeviceOnce::kMaxDevices;
+  if (err == cudaSuccess && tracked && known[device]) return known[device];
+  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+  if (err != cudaSuccess) throw std::runtime_error(std::string("multiprocessors: ") + cudaGetErrorString(err));
+  if (tracked) known[device] = count;
+  return count;
+}
+
 // An event for ordering streams, given back when the scope ends (work that waits for it keeps what it needs).
 class ScopedEvent {
  public:

@@ -70,6 +70,26 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return false;
 }
 
+// The same for waits that are long by nature (an epilogue's for a whole tile): the thread may be suspended for some microseconds at a time,
+// so that it does not spend the power that others compute with.  The budget is some ten seconds.
+__device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  for (uint32_t it = 0; it < (1u << 21); ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(5000u)
+        : "memory");
+    if (done) return true;
+    if ((it & 63u) == 63u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  if (status) atomicCAS(status, 0, code);
+  return false;
+}
+
 // ---- TMA (tiled, 2-D, no multicast) ---------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tensor_map, uint64_t* bar, int x, int y) {
   asm volatile(
