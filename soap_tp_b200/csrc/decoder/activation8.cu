@@ -61,31 +61,37 @@ struct Place {
   }
 };
 
-// WIDE: all rows lie on 16-byte boundaries and are multiples of eight values long.
+// WIDE: all rows lie on 16-byte boundaries and are multiples of eight values long.  Otherwise 16-bit rows are shifted as they are moved, and fp32
+// values go one by one.
 template <bool WIDE, typename T>
 __device__ __forceinline__ Eight<T> load8(const T* p, int valid) {
   Eight<T> e;
-  if (WIDE) {
+  if constexpr (WIDE) {
     if (valid > 0) e.load(p);
     else e.clear();
+  } else if constexpr (sizeof(T) == 2) {
+    e = load8_shifted(p, valid);
   } else {
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_float(p[i]) : 0.f;
-    e.set(v);                    // (exact: the values have this type)
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? p[i] : 0.f;
+    e.set(v);
   }
   return e;
 }
+// All 32 lanes call.
 template <bool WIDE, typename T>
-__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
-  if (WIDE) {
-    Eight<T> e;
-    e.set(v);
-    e.store(p);
+__device__ __forceinline__ void store8(T* p, const Place& place, const float (&v)[8]) {
+  Eight<T> e;
+  e.set(v);
+  if constexpr (WIDE) {
+    if (place.valid > 0) e.store(p);
+  } else if constexpr (sizeof(T) == 2) {
+    store8_shifted(p, e, place.valid, place.column != 0);      // (lanes go along rows)
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < valid) p[i] = from_float<T>(v[i]);
+      if (i < place.valid) p[i] = v[i];
   }
 }
 
@@ -148,6 +154,11 @@ __device__ __forceinline__ void keep(const Kept8& kept, const Shape& shape, cons
 }
 
 __device__ __forceinline__ void kept_values(const Kept8& kept, const Place& p, float (&v)[8]) {
+  if (p.valid <= 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    return;
+  }
   dequantise(*reinterpret_cast<const uint2*>(kept.values + p.row * kept.pitch + p.column), kept.scales[p.group], v);
 }
 
@@ -173,10 +184,9 @@ __global__ void __launch_bounds__(kThreads) unpack8_kernel(Kept8 kept, Shape sha
   wait_for_predecessor();
   let_successor_start();
   const Place p(shape);
-  if (p.valid <= 0) return;
   float v[8];
   kept_values(kept, p, v);
-  store8<WIDE>(out + p.row * ld + p.column, p.valid, v);
+  store8<WIDE>(out + p.row * ld + p.column, p, v);
 }
 
 template <typename T, bool WIDE, bool KEEP>
@@ -192,13 +202,12 @@ swiglu8_forward_kernel(const T* __restrict__ gate, int64_t ld_gate, const T* __r
     keep(gate8, shape, p, g8);
     keep(up8, shape, p, u8);
   }
-  if (p.valid <= 0) return;
   float g[8], u[8];
   g8.get(g);
   u8.get(u);
 #pragma unroll
   for (int i = 0; i < 8; ++i) u[i] *= g[i] * sigmoid<T>(g[i]);
-  store8<WIDE>(y + p.row * ld + p.column, p.valid, u);
+  store8<WIDE>(y + p.row * ld + p.column, p, u);
 }
 
 template <typename T, bool WIDE, bool WITH_Y>
@@ -208,7 +217,6 @@ swiglu8_backward_kernel(const T* __restrict__ grad, int64_t ld_grad, Kept8 gate8
   wait_for_predecessor();
   let_successor_start();
   const Place p(shape);
-  if (p.valid <= 0) return;
   float d[8], g[8], u[8], out_g[8], out_u[8];
   const Eight<T> d8 = load8<WIDE>(grad + p.row * ld_grad + p.column, p.valid);
   kept_values(gate8, p, g);
@@ -222,9 +230,9 @@ swiglu8_backward_kernel(const T* __restrict__ grad, int64_t ld_grad, Kept8 gate8
     if (WITH_Y) u[i] *= silu;
   }
   const int64_t at = p.row * ld + p.column;
-  store8<WIDE>(d_gate + at, p.valid, out_g);
-  store8<WIDE>(d_up + at, p.valid, out_u);
-  if (WITH_Y) store8<WIDE>(y + at, p.valid, u);
+  store8<WIDE>(d_gate + at, p, out_g);
+  store8<WIDE>(d_up + at, p, out_u);
+  if (WITH_Y) store8<WIDE>(y + at, p, u);
 }
 
 bool on_16(const void* data, int64_t ld, int size) { return (reinterpret_cast<uintptr_t>(data) & 15) == 0 && (ld * size) % 16 == 0; }

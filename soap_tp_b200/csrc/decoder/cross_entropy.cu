@@ -302,11 +302,18 @@ scale_gradients_kernel(const float* __restrict__ factor, __nv_bfloat16* __restri
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kScaleThreads + threadIdx.x; i < runs; i += static_cast<int64_t>(gridDim.x) * kScaleThreads) {
     __nv_bfloat16* at = i < runs_a ? a + 8 * i : b + 8 * (i - runs_a);
     const int valid = static_cast<int>(min(static_cast<int64_t>(8), i < runs_a ? count_a - 8 * i : count_b - 8 * (i - runs_a)));
-    float v[8];
-    read_eight(at, valid, true, v);
+    if (valid == 8) {
+      Eight<__nv_bfloat16> e;
+      float v[8];
+      e.load(at);
+      e.get(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= f;
-    write_eight(at, valid, true, v);
+      for (int j = 0; j < 8; ++j) v[j] *= f;
+      e.set(v);
+      e.store(at);
+    } else {
+      for (int j = 0; j < valid; ++j) at[j] = __float2bfloat16_rn(__bfloat162float(at[j]) * f);
+    }
   }
 }
 

@@ -12,8 +12,8 @@
 // means are sums over a group that everything else of a row waits for, and what must be under way meanwhile (some 40 KB an SM) does
 // not fit in registers next to the sums of the vectors' gradients.  Those stay in registers until a block's last row; a second kernel adds the
 // blocks' sums in a fixed order.  The vectors stay in registers as well, as fp32, and arithmetic goes two values at a time: with 40 instructions a value,
-// converted and multiplied anew for every row, issue bounded it.  Rows that do not lie on 16-byte boundaries are copied from the boundary before them and read value by
-// value; rows too long for two of them in shared memory are read straight into registers.
+// converted and multiplied anew for every row, issue bounded it.  Rows that do not lie on 16-byte boundaries are copied from the boundary before them and read shifted (fp32:
+// value by value); rows too long for two of them in shared memory are read straight into registers.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -28,9 +28,10 @@
 namespace soapb200 {
 namespace {
 
-// A thread's 2 P values of a row, as pairs of fp32.  E = 8: runs of eight neighbouring values on 16-byte boundaries, blockDim.x runs apart;
-// E = 1: single values, blockDim.x apart.  Values beyond the row are zero and are not written.
-template <int E, int P>
+// A thread's 2 P values of a row, as pairs of fp32.  kWhole: runs of eight neighbouring values on 16-byte boundaries, blockDim.x runs apart;
+// kShifted: the same anywhere (16-bit types); kSingle: single values, blockDim.x apart.  Values beyond the row are zero and are not written.
+enum Access : int { kWhole, kShifted, kSingle };
+template <int A, int P>
 struct Lane {
   uint64_t v[P];
 
@@ -39,51 +40,60 @@ struct Lane {
     for (int i = 0; i < P; ++i) v[i] = 0;
   }
   __device__ __forceinline__ float get(int i) const { return pair_element(v[i / 2], i & 1); }
+  static __device__ __forceinline__ int column_of(int run) { return 8 * (threadIdx.x + run * blockDim.x); }
 
   template <typename T>
   __device__ __forceinline__ void load(const T* row, int dim) {
-    if constexpr (E == 8) {
-#pragma unroll
-      for (int i = 0; i < P / 4; ++i) {
-        const int column = 8 * (threadIdx.x + i * blockDim.x);
-        if (column < dim) {
-          Eight<T> e;
-          e.load(row + column);
-          float f[8];
-          e.get(f);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[4 * i + j] = pack_floats(f[2 * j], f[2 * j + 1]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[4 * i + j] = 0;
-        }
-      }
-    } else {
+    if constexpr (A == kSingle) {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const int first = threadIdx.x + 2 * i * blockDim.x, second = first + blockDim.x;
         v[i] = pack_floats(first < dim ? to_float(row[first]) : 0.f, second < dim ? to_float(row[second]) : 0.f);
       }
-    }
-  }
-  template <typename T>
-  __device__ __forceinline__ void store(T* row, int dim) const {
-    if constexpr (E == 8) {
+    } else {
 #pragma unroll
       for (int i = 0; i < P / 4; ++i) {
-        const int column = 8 * (threadIdx.x + i * blockDim.x);
-        if (column < dim) {
+        const int column = column_of(i);
+        float f[8];
+        if constexpr (A == kShifted && sizeof(T) == 4) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = column + j < dim ? to_float(row[column + j]) : 0.f;
+        } else {
           Eight<T> e;
-          const float f[8] = {get(8 * i), get(8 * i + 1), get(8 * i + 2), get(8 * i + 3), get(8 * i + 4), get(8 * i + 5), get(8 * i + 6), get(8 * i + 7)};
-          e.set(f);
-          e.store(row + column);
+          if constexpr (A == kShifted) e = load8_shifted(row + column, min(8, dim - column));
+          else if (column < dim) e.load(row + column);
+          else e.clear();
+          e.get(f);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * i + j] = pack_floats(f[2 * j], f[2 * j + 1]);
       }
-    } else {
+    }
+  }
+  // (with kShifted all lanes of a warp call)
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int dim) const {
+    if constexpr (A == kSingle) {
 #pragma unroll
       for (int i = 0; i < 2 * P; ++i) {
         const int column = threadIdx.x + i * blockDim.x;
         if (column < dim) row[column] = from_float<T>(get(i));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < P / 4; ++i) {
+        const int column = column_of(i);
+        const float f[8] = {get(8 * i), get(8 * i + 1), get(8 * i + 2), get(8 * i + 3), get(8 * i + 4), get(8 * i + 5), get(8 * i + 6), get(8 * i + 7)};
+        if constexpr (A == kShifted && sizeof(T) == 4) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (column + j < dim) row[column + j] = from_float<T>(f[j]);
+        } else {
+          Eight<T> e;
+          e.set(f);
+          if constexpr (A == kShifted) store8_shifted(row + column, e, min(8, dim - column), true);
+          else if (column < dim) e.store(row + column);
+        }
       }
     }
   }
@@ -135,13 +145,13 @@ constexpr int kMostGroups = 8, kMostStages = 8, kMostInputs = 4;
 // How a row is dealt to threads, and what a group of them keeps ahead.
 struct Deal {
   bool ring;
-  int run, values, threads, groups, bound;                // neighbouring values, values a thread, threads a row, rows at once
+  int access, values, threads, groups, bound;             // values a thread, threads a row, rows at once, threads the kernel is compiled for
   int stages, row_bytes;                                  // of the ring
   int smem, blocks;
 };
 
 // The rows of up to four matrices, one row of each a stage.  INPUTS that are absent have a null base.
-template <typename T, int INPUTS, int E>
+template <typename T, int INPUTS, int A>
 struct Ring {
   Rows inputs[INPUTS];
   uint8_t* data;
@@ -172,7 +182,7 @@ struct Ring {
   }
   // Input `i` of the current row.
   __device__ __forceinline__ const T* at(int i, int64_t row) const {
-    return reinterpret_cast<const T*>(data + (stage * INPUTS + i) * row_bytes + (E == 8 ? 0 : address(i, row) & 15));
+    return reinterpret_cast<const T*>(data + (stage * INPUTS + i) * row_bytes + (A == kWhole ? 0 : address(i, row) & 15));
   }
   template <bool RING>
   __device__ __forceinline__ const T* row_at(int i, int64_t row) const {
@@ -200,9 +210,9 @@ struct Ring {
   }
 };
 
-template <typename T, int INPUTS, int E, bool RING>
-__device__ __forceinline__ Ring<T, INPUTS, E> make_ring(const Deal& d, int dim, uint8_t* dynamic, uint64_t (&bars)[kMostGroups][kMostStages]) {
-  Ring<T, INPUTS, E> ring;
+template <typename T, int INPUTS, int A, bool RING>
+__device__ __forceinline__ Ring<T, INPUTS, A> make_ring(const Deal& d, int dim, uint8_t* dynamic, uint64_t (&bars)[kMostGroups][kMostStages]) {
+  Ring<T, INPUTS, A> ring;
   ring.stages = d.stages; ring.row_bytes = d.row_bytes; ring.dim = dim;
   ring.data = dynamic + static_cast<int64_t>(threadIdx.y) * d.stages * INPUTS * d.row_bytes;
   ring.full = bars[threadIdx.y];
@@ -217,25 +227,25 @@ __device__ __forceinline__ Ring<T, INPUTS, E> make_ring(const Deal& d, int dim, 
 }
 
 // Products of a row's vectors: `weight` that y is multiplied by, and scale * gate * branch_weight, which the branch is.
-template <typename T, int E, int P>
-__device__ __forceinline__ void load_vectors(const NormProblem& p, Lane<E, P>& weight, Lane<E, P>& branch) {
+template <typename T, int A, int P>
+__device__ __forceinline__ void load_vectors(const NormProblem& p, Lane<A, P>& weight, Lane<A, P>& branch) {
   const bool fp32 = p.vector_type == kFp32;
   weight.template load_vector<T>(p.weight, fp32, p.dim);
   branch.template load_vector<T>(p.branch_weight, fp32, p.dim);
-  Lane<E, P> gate;
+  Lane<A, P> gate;
   gate.template load_vector<T>(p.gate, fp32, p.dim);
 #pragma unroll
   for (int i = 0; i < P; ++i) branch.v[i] = mul_pair(mul_pair(branch.v[i], gate.v[i]), twice(p.scale));
 }
 
-template <typename T, int E, int P, int THREADS, bool RING, bool AFTER>
+template <typename T, int A, int P, int THREADS, bool RING, bool AFTER>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) residual_norm_forward_kernel(NormProblem p, T* __restrict__ h_out, T* __restrict__ y_out, int64_t ld, Deal d) {
   __shared__ __align__(16) float sums[kMostGroups][64];
   __shared__ uint64_t bars[kMostGroups][kMostStages];
   extern __shared__ __align__(128) uint8_t dynamic[];
   float* shared = sums[threadIdx.y];
   int turn = 0;
-  Ring<T, 2, E> ring = make_ring<T, 2, E, RING>(d, p.dim, dynamic, bars);
+  Ring<T, 2, A> ring = make_ring<T, 2, A, RING>(d, p.dim, dynamic, bars);
   ring.inputs[0] = p.x; ring.inputs[1] = p.branch;
   wait_for_predecessor();
   let_successor_start();
@@ -244,14 +254,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) residual_norm
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
   int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if constexpr (RING) ring.start(row, step, p.rows);
-  Lane<E, P> weight, branch_factor;
+  Lane<A, P> weight, branch_factor;
   load_vectors<T>(p, weight, branch_factor);
   for (; row < p.rows; row += step) {
     if constexpr (RING) ring.wait(p.status);
-    Lane<E, P> h;
+    Lane<A, P> h;
     h.load(ring.template row_at<RING>(0, row), p.dim);
     if (with_branch) {
-      Lane<E, P> b;
+      Lane<A, P> b;
       b.load(ring.template row_at<RING>(1, row), p.dim);
       float r_b = 1.f;
       if (AFTER) {
@@ -280,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) residual_norm
 }
 
 // SCALED: the branch has a norm or a gate.
-template <typename T, int E, int P, int THREADS, bool RING, bool SCALED>
+template <typename T, int A, int P, int THREADS, bool RING, bool SCALED>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
   __shared__ __align__(16) float sums[kMostGroups][64];
@@ -288,7 +298,7 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
   extern __shared__ __align__(128) uint8_t dynamic[];
   float* shared = sums[threadIdx.y];
   int turn = 0;
-  Ring<T, 4, E> ring = make_ring<T, 4, E, RING>(d, p.dim, dynamic, bars);
+  Ring<T, 4, A> ring = make_ring<T, 4, A, RING>(d, p.dim, dynamic, bars);
   const bool with_branch = p.branch.data != nullptr;
   ring.inputs[0] = g.grad_y; ring.inputs[1] = g.grad_y.data ? p.x : Rows{nullptr, 0};
   ring.inputs[2] = g.grad_h; ring.inputs[3] = SCALED || g.grad_y.data ? p.branch : Rows{nullptr, 0};
@@ -299,7 +309,7 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
   int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if constexpr (RING) ring.start(row, step, p.rows);
-  Lane<E, P> weight, branch_factor, d_weight, d_branch;      // the last: the sum that both of the branch's vectors' gradients are made of
+  Lane<A, P> weight, branch_factor, d_weight, d_branch;      // the last: the sum that both of the branch's vectors' gradients are made of
   load_vectors<T>(p, weight, branch_factor);
   d_weight.clear();
   d_branch.clear();
@@ -316,9 +326,9 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
     const float r = r_next, r_b = r_b_next;
     look_up(row + step);
     if constexpr (RING) ring.wait(p.status);
-    Lane<E, P> dh;
+    Lane<A, P> dh;
     if (g.grad_y.data) {
-      Lane<E, P> h;
+      Lane<A, P> h;
       h.load(ring.template row_at<RING>(1, row), p.dim);
       if (with_branch) {
         dh.load(ring.template row_at<RING>(3, row), p.dim);
@@ -341,14 +351,14 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
       dh.clear();
     }
     if (g.grad_h.data) {
-      Lane<E, P> gh;
+      Lane<A, P> gh;
       gh.load(ring.template row_at<RING>(2, row), p.dim);
 #pragma unroll
       for (int i = 0; i < P; ++i) add_pair(dh.v[i], gh.v[i]);
     }
     if (g.d_x) dh.store(static_cast<T*>(g.d_x) + row * g.ld, p.dim);
     if constexpr (SCALED) {
-      Lane<E, P> b;
+      Lane<A, P> b;
       b.load(ring.template row_at<RING>(3, row), p.dim);
       const float by = p.scale * r_b;
       uint64_t dot = 0;
@@ -372,15 +382,15 @@ residual_norm_backward_kernel(NormProblem p, NormGradients g, Deal d) {
   }
   // this block's sums: rows that share the block are added one after another, where the ring was
   float* joined = reinterpret_cast<float*>(dynamic);
-  auto leave = [&](const Lane<E, P>& values, int which) {
+  auto leave = [&](const Lane<A, P>& values, int which) {
     float* out = g.partials + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.dim;
     for (int y = 0; y < static_cast<int>(blockDim.y); ++y) {
       if (blockDim.y > 1) __syncthreads();
       if (static_cast<int>(threadIdx.y) == y) {
-        Lane<E, P> sum = values;
+        Lane<A, P> sum = values;
         if (y) {
-          Lane<E, P> before;
-          before.load(joined, p.dim);
+          Lane<A, P> before;
+          before.load(static_cast<const float*>(joined), p.dim);
 #pragma unroll
           for (int i = 0; i < P; ++i) add_pair(sum.v[i], before.v[i]);
         }
@@ -442,7 +452,7 @@ Deal deal_of(bool wide, int64_t rows, int dim, int size, int inputs, int residen
   const int warps_of = (dim + 511) / 512;
   int warps = 1;
   while (warps < warps_of) warps *= 2;
-  d.run = wide ? 8 : 1;
+  d.access = wide ? kWhole : size == 2 ? kShifted : kSingle;
   d.values = 16;
   d.threads = 32 * warps;
   d.groups = warps < 8 ? 8 / warps : 1;
@@ -459,6 +469,7 @@ Deal deal_of(bool wide, int64_t rows, int dim, int size, int inputs, int residen
   if (d.ring) return d;
   d.stages = d.row_bytes = 0;
   d.groups = 1;
+  if (!wide) d.access = kSingle;
   if (!wide || dim > 1024 * 16) d.values = 32;
   if (dim > 1024 * d.values) throw std::invalid_argument("residual_norm: rows of more than 32768 values are not supported");
   d.threads = ((dim + d.values - 1) / d.values + 31) / 32 * 32;
@@ -494,23 +505,24 @@ void for_type(int type, F f) {
   else throw std::invalid_argument("residual_norm: unknown type");
 }
 
-template <int E_, int P_, int THREADS_, bool RING_>
+template <int A_, int P_, int THREADS_, bool RING_>
 struct Form {
-  static constexpr int E = E_, P = P_, THREADS = THREADS_;
+  static constexpr int A = A_, P = P_, THREADS = THREADS_;
   static constexpr bool RING = RING_;
 };
-template <typename F>
+template <typename T, typename F>
 void for_deal(const Deal& d, F f) {
+  constexpr int kOdd = sizeof(T) == 2 ? kShifted : kSingle;
   if (d.ring) {
-    if (d.run == 8 && d.bound == 256) f(Form<8, 8, 256, true>{});
-    else if (d.run == 8) f(Form<8, 8, 512, true>{});
-    else if (d.bound == 256) f(Form<1, 8, 256, true>{});
-    else f(Form<1, 8, 512, true>{});
-  } else if (d.run == 8) {
-    if (d.values == 32) f(Form<8, 16, 1024, false>{});
-    else f(Form<8, 8, 1024, false>{});
+    if (d.access == kWhole && d.bound == 256) f(Form<kWhole, 8, 256, true>{});
+    else if (d.access == kWhole) f(Form<kWhole, 8, 512, true>{});
+    else if (d.bound == 256) f(Form<kOdd, 8, 256, true>{});
+    else f(Form<kOdd, 8, 512, true>{});
+  } else if (d.access == kWhole) {
+    if (d.values == 32) f(Form<kWhole, 16, 1024, false>{});
+    else f(Form<kWhole, 8, 1024, false>{});
   } else {
-    f(Form<1, 16, 1024, false>{});
+    f(Form<kSingle, 16, 1024, false>{});
   }
 }
 
@@ -540,14 +552,14 @@ void residual_norm_forward(const NormProblem& p, void* h, void* y, int64_t ld, c
   const Deal d = forward_deal(p, h, y, ld);
   for_type(p.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    for_deal(d, [&](auto form) {
+    for_deal<T>(d, [&](auto form) {
       using F = decltype(form);
       static PerDeviceOnce plain, after;
       if (p.branch_weight)
-        start("residual_norm_forward", residual_norm_forward_kernel<T, F::E, F::P, F::THREADS, F::RING, true>, d, after, stream, p,
+        start("residual_norm_forward", residual_norm_forward_kernel<T, F::A, F::P, F::THREADS, F::RING, true>, d, after, stream, p,
               static_cast<T*>(h), static_cast<T*>(y), ld, d);
       else
-        start("residual_norm_forward", residual_norm_forward_kernel<T, F::E, F::P, F::THREADS, F::RING, false>, d, plain, stream, p,
+        start("residual_norm_forward", residual_norm_forward_kernel<T, F::A, F::P, F::THREADS, F::RING, false>, d, plain, stream, p,
               static_cast<T*>(h), static_cast<T*>(y), ld, d);
     });
   });
@@ -559,13 +571,13 @@ void residual_norm_backward(const NormProblem& p, const NormGradients& g, cudaSt
   if (g.blocks != d.blocks) throw std::invalid_argument("residual_norm: as many blocks as residual_norm_blocks says");
   for_type(p.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    for_deal(d, [&](auto form) {
+    for_deal<T>(d, [&](auto form) {
       using F = decltype(form);
       static PerDeviceOnce plain, scaled;
       if (p.branch_weight || p.gate)
-        start("residual_norm_backward", residual_norm_backward_kernel<T, F::E, F::P, F::THREADS, F::RING, true>, d, scaled, stream, p, g, d);
+        start("residual_norm_backward", residual_norm_backward_kernel<T, F::A, F::P, F::THREADS, F::RING, true>, d, scaled, stream, p, g, d);
       else
-        start("residual_norm_backward", residual_norm_backward_kernel<T, F::E, F::P, F::THREADS, F::RING, false>, d, plain, stream, p, g, d);
+        start("residual_norm_backward", residual_norm_backward_kernel<T, F::A, F::P, F::THREADS, F::RING, false>, d, plain, stream, p, g, d);
     });
   });
   if (g.d_weight || g.d_branch_weight || g.d_gate)

@@ -250,7 +250,8 @@ def _check_norm(rows, dim, dtype, after, gated, normed=True, vector_dtype=None, 
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 7), (20, 32), (300, 256), (7, 257), (33, 1000), (400, 1032), (9, 3001), (1000, 4096), (5, 5000), (4, 8200)])
+@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 7), (20, 32), (300, 256), (7, 257), (33, 1000), (400, 1032), (9, 3001), (1000, 4096), (5, 5000), (4, 8200),
+                                      (20, 4099), (7, 8191), (600, 33)])
 @pytest.mark.parametrize("after,gated", [(False, False), (True, True)])
 def test_residual_norm(rows, dim, dtype, after, gated):
     _check_norm(rows, dim, dtype, after, gated)
@@ -314,7 +315,7 @@ def test_residual_norm_gradients_do_not_share_memory_between_leaves():
 
 
 # ---- activations in 8 bits ----------------------------------------------------------------------------------------------
-SHAPES8 = [(1, 1), (2, 7), (3, 64), (5, 65), (128, 32), (33, 200), (300, 1000), (77, 1792), (4, 14336)]
+SHAPES8 = [(1, 1), (2, 7), (3, 64), (5, 65), (600, 9), (70, 127), (41, 3001), (128, 32), (33, 200), (300, 1000), (77, 1792), (4, 14336)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
@@ -361,6 +362,19 @@ def test_pack8_beyond_32_bits():
     assert torch.equal(packed.values[-1:], last.values) and torch.equal(packed.scales[-1:], last.scales)
     del x
     assert torch.equal(unpack8(packed)[-1:], unpack8(last))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [5, 8, 61, 64, 200, 1001])
+def test_rows_at_every_offset_from_a_boundary(dim, dtype):
+    from soap_tp_b200.ops import pack8, swiglu8, unpack8
+
+    for offset in range(8):
+        for pitch in (dim, dim + 3):
+            flat = _rand(40 * pitch + 16, seed=offset, dtype=dtype)
+            x = flat[offset:].as_strided((33, dim), (pitch, 1))
+            assert torch.equal(unpack8(pack8(x)), unpack8(pack8(x.clone())))
+            assert torch.equal(swiglu8(x, x), swiglu8(x.clone(), x.clone()))
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
