@@ -52,46 +52,60 @@ __device__ __forceinline__ V block_reduce(V v, Op op, V* shared) {
   return v;
 }
 
-// One block: a thread takes a run of neighbouring tokens, counts, learns how many come before, and writes.
+// One block, 8192 tokens at a time: a thread takes eight neighbouring ones, counts, learns how many come before, and writes.  With `factor`
+// what the gradient of a reduced loss multiplies rows by is left as well (head_factors).
+constexpr int kCountTokens = 8;
 __global__ void __launch_bounds__(kSingleThreads)
 head_count_kernel(const int64_t* __restrict__ targets, int tokens, int64_t ignored, int64_t first_word, int words, int64_t vocabulary,
-                  int* __restrict__ count, int* __restrict__ where, int* __restrict__ column, int* __restrict__ split_counters) {
+                  int* __restrict__ count, int* __restrict__ where, int* __restrict__ column, int* __restrict__ split_counters, bool mean,
+                  float* __restrict__ factor, float* __restrict__ alpha) {
   __shared__ int warps[32];
   wait_for_predecessor();
   let_successor_start();
   for (int i = threadIdx.x; i < kSplitCounters; i += kSingleThreads) split_counters[i] = 0;
-  const int each = (tokens + kSingleThreads - 1) / kSingleThreads;
-  const int begin = min(tokens, static_cast<int>(threadIdx.x) * each), end = min(tokens, begin + each);
-  int mine = 0;
-  for (int i = begin; i < end; ++i) mine += targets[i] != ignored;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = mine;
+  int counted = 0;
+  for (int64_t base = 0; base < tokens; base += kSingleThreads * kCountTokens) {
+    const int64_t begin = base + threadIdx.x * kCountTokens;
+    int64_t target[kCountTokens];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int other = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += other;
-  }
-  if (lane == 31) warps[warp] = before;
-  __syncthreads();
-  if (warp == 0) {
+    for (int i = 0; i < kCountTokens; ++i) target[i] = begin + i < tokens ? targets[begin + i] : ignored;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kCountTokens; ++i) mine += target[i] != ignored;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += other;
+    }
+    if (lane == 31) warps[warp] = before;
+    __syncthreads();
     int sum = warps[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int other = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += other;
     }
-    warps[lane] = sum;
+    const int ahead = __shfl_sync(0xffffffffu, sum, max(warp - 1, 0));      // in the warps before this one
+    int at = counted + before - mine + (warp ? ahead : 0);
+#pragma unroll
+    for (int i = 0; i < kCountTokens; ++i) {
+      if (target[i] == ignored) continue;
+      const int64_t here = target[i] - first_word;
+      const int c = target[i] < 0 || target[i] >= vocabulary ? kUnknown : here < 0 || here >= words ? kElsewhere : static_cast<int>(here);
+      where[at] = static_cast<int>(begin + i);
+      column[at] = c;
+      if (factor) factor[at] = c == kUnknown ? nanf("") : 1.f;
+      ++at;
+    }
+    counted += __shfl_sync(0xffffffffu, sum, 31);
+    __syncthreads();      // before `warps` is written again
   }
-  __syncthreads();
-  int at = before - mine + (warp ? warps[warp - 1] : 0);
-  for (int i = begin; i < end; ++i) {
-    const int64_t target = targets[i];
-    if (target == ignored) continue;
-    const int64_t here = target - first_word;
-    where[at] = i;
-    column[at++] = target < 0 || target >= vocabulary ? kUnknown : here < 0 || here >= words ? kElsewhere : static_cast<int>(here);
+  if (threadIdx.x == 0) {
+    *count = counted;
+    if (factor) *alpha = !mean ? 1.f : counted ? 1.f / static_cast<float>(counted) : 0.f;
   }
-  if (threadIdx.x == 0) *count = warps[31];
 }
 
 // Where not every token counts: the hidden states of those that do, one after another, zeros up to the next multiple of 64, and
@@ -154,6 +168,7 @@ head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number,
     const T* h = counted == tokens ? all + (first + other) * ld_all : packed + (first + other) * ld_packed;
     const T* w = weight + word * ld_weight;
     float dot = 0.f;
+#pragma unroll 4
     for (int run = threadIdx.x; run < depth / 8; run += 32) {      // (rows lie on 16-byte boundaries)
       Eight<T> a, b;
       a.load(h + 8 * run);
@@ -204,6 +219,7 @@ head_reduced_loss_kernel(const int* __restrict__ count, const int* __restrict__ 
   let_successor_start();
   const int counted = *count;
   double sum = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < counted; i += kSingleThreads) sum += token_loss(column[i], lse[i], picked[i]);
   sum = block_reduce(sum, [](double a, double b) { return a + b; }, shared);
   if (threadIdx.x == 0) *loss = static_cast<float>(mean && counted ? sum / counted : sum);
@@ -228,9 +244,10 @@ head_factors_kernel(const int* __restrict__ count, const int* __restrict__ where
       relative = ldexpf(1.f, -exponent);
     }
   } else {
-    if (grad_loss) common = *grad_loss;
+    common = *grad_loss;
     if (reduction == kLossMean) common = counted ? common / static_cast<float>(counted) : 0.f;
   }
+#pragma unroll 4
   for (int i = threadIdx.x; i < counted; i += kSingleThreads) {
     const float own = reduction == kLossNone ? grad_loss[where[i]] : 1.f;
     factor[i] = column[i] == kUnknown ? nanf("") : stored * relative * own;
@@ -336,9 +353,10 @@ Gemm16Problem logits_of(const HeadProblem& p, const LogitRows& r) {
 
 }  // namespace
 
-void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaStream_t stream) {
+void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, LossReduction reduction, float* factor, float* alpha, cudaStream_t stream) {
+  if (factor && (reduction == kLossNone || !p.bf16)) throw std::invalid_argument("head_prepare: these factors want the loss's gradient");
   check(launch_dependent(head_count_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.targets, p.tokens, p.ignore_index, p.first_word,
-                         p.words, p.vocabulary, p.count, p.where, p.column, p.split_counters),
+                         p.words, p.vocabulary, p.count, p.where, p.column, p.split_counters, reduction == kLossMean, factor, alpha),
         "head_count");
   const int blocks = std::min((p.tokens + 7) / 8, 8 * multiprocessors());
   check(launch_dependent(head_gather_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<const uint16_t*>(p.hidden.data), p.hidden.ld,

@@ -28,7 +28,8 @@ struct HeadProblem {
 constexpr int kElsewhere = -1, kUnknown = -2;
 
 // Fills count, where, column, split_counters and packed; with `d_hidden`, clears the rows of the tokens that do not count.
-void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, cudaStream_t stream);
+// With `factor` (bf16, sum or mean) what head_factors leaves for a gradient of one as well.
+void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, LossReduction reduction, float* factor, float* alpha, cudaStream_t stream);
 
 // For tokens first .. first + rows of those that count: lse[i] = log sum_j exp(l_ij) over this rank's words, picked[i] = l_i,t_i where the
 // target is one of them and 0 elsewhere.  `parts`: ceil(words / kLogitPart) x rows pairs.  With `logits` (bf16) the exponentials stay
@@ -46,7 +47,7 @@ void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float
 void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, cudaStream_t stream);
 
 // What the gradient of the loss multiplies the row of a token that counts by: factor[i] * *alpha.  `grad_loss` has one value per token,
-// or one; null: one.
+// or one.
 void head_factors(const HeadProblem& p, LossReduction reduction, const float* grad_loss, float* factor, float* alpha, cudaStream_t stream);
 
 // The exponentials that head_statistics left become the logits' gradient, factor (exp(l - lse) - [target]).

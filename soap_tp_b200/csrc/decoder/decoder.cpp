@@ -355,6 +355,15 @@ struct LossOptions {
   }
 };
 
+// Which capture the current stream is part of; 0: none.
+int64_t capture_id() {
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return 0;
+  cudaStreamCaptureStatus status;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(current_stream(), &status, &id));
+  return static_cast<int64_t>(id);
+}
+
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets, const LossOptions& o) {
     const c10::cuda::CUDAGuard guard(hidden.device());
@@ -370,8 +379,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     const bool with_loss = (o.want_hidden || o.want_weight) && reduction != kLossNone && p.bf16;
     if (with_loss) {
       const Gradients g(head, o.want_hidden, o.want_weight, o.workspace_bytes);
-      head_prepare(p, pointer(g.hidden), p.depth, stream);
-      head_factors(p, reduction, nullptr, g.factors(), g.alpha(), stream);
+      head_prepare(p, pointer(g.hidden), p.depth, reduction, g.factors(), g.alpha(), stream);
       const Tensor parts = head.parts(g.rows);
       for (int first = 0; first < p.tokens; first += g.rows) {
         const LogitRows r = g.turn(head, first, pairs(parts));
@@ -383,21 +391,25 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       }
       ctx->saved_data["hidden"] = g.hidden;
       ctx->saved_data["weight"] = g.weight;
-      count(3);
     } else {
-      const Tensor parts = head.parts(p.tokens);
-      head_prepare(p, nullptr, 0, stream);
-      head_statistics(p, LogitRows{0, p.tokens, nullptr, 0, pairs(parts)}, lse_at, picked_at, head.status, stream);
+      head_prepare(p, nullptr, 0, reduction, nullptr, nullptr, stream);
+      const int64_t parts_of_token = 8 * ((p.words + kLogitPart - 1) / kLogitPart);
+      const int rows = static_cast<int>(std::min<int64_t>(p.tokens, std::max<int64_t>(256, o.workspace_bytes / parts_of_token / 256 * 256)));
+      const Tensor parts = head.parts(rows);
+      for (int first = 0; first < p.tokens; first += rows) {
+        head_statistics(p, LogitRows{first, std::min(rows, p.tokens - first), nullptr, 0, pairs(parts)}, lse_at, picked_at, head.status, stream);
+        count(2);
+      }
       if (o.join) o.join(lse, picked);
-      count(4);
     }
+    count(2);
     Tensor loss = reduction == kLossNone ? at::empty(targets.sizes(), floats) : at::empty({}, floats);
     head_losses(p, lse_at, picked_at, reduction, loss.data_ptr<float>(), stream);
     count(1);
     ctx->save_for_backward({hidden, weight, targets, lse});
     ctx->saved_data["numbers"] = o.numbers();
     ctx->saved_data["made"] = with_loss;
-    ctx->saved_data["captured"] = at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None;
+    ctx->saved_data["capture"] = capture_id();
     return loss;
   }
 
@@ -412,10 +424,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       const auto stream = current_stream();
       const auto o = ctx->saved_data["numbers"].toIntVector();
       const Tensor grad_loss = grads[0].to(at::kFloat).contiguous();
-      const bool captured = at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None;
       Tensor d_hidden, d_weight;
-      // Handed over once: they are the caller's from then on.  A graph of the backward pass alone would scale them again at every replay.
-      const bool made = ctx->saved_data["made"].toBool() && ctx->saved_data["captured"].toBool() == captured;
+      // Handed over once: they are the caller's from then on.  A graph without the forward pass would scale them again at every replay.
+      const bool made = ctx->saved_data["made"].toBool() && ctx->saved_data["capture"].toInt() == capture_id();
       if (ctx->saved_data["made"].toBool()) {
         if (made) {
           if (o[6]) d_hidden = ctx->saved_data["hidden"].toTensor();
@@ -431,7 +442,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const Head head(hidden.reshape({-1, hidden.size(-1)}), weight, targets.reshape({-1}), o[1], o[2], o[3], o[5]);
         const HeadProblem& p = head.problem;
         const Gradients g(head, o[6], o[7], o[4]);
-        head_prepare(p, pointer(g.hidden), p.depth, stream);
+        head_prepare(p, pointer(g.hidden), p.depth, static_cast<LossReduction>(o[0]), nullptr, nullptr, stream);
         head_factors(p, static_cast<LossReduction>(o[0]), grad_loss.data_ptr<float>(), g.factors(), g.alpha(), stream);
         for (int first = 0; first < p.tokens; first += g.rows) {
           const LogitRows r = g.turn(head, first, nullptr);

@@ -192,6 +192,38 @@ def test_cross_entropy_backward_pass_captured_alone():
         within(grads[1], exact[2])
 
 
+def test_cross_entropy_of_captured_forward_and_backward_graphs():
+    # two graphs: the backward one is replayed on its own too
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    hidden, weight, targets = _head(100, 64, 300, BF16)
+    up = torch.tensor(0.5, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(linear_cross_entropy(hidden, weight, targets), (hidden, weight), up)
+    torch.cuda.current_stream().wait_stream(side)
+    pool = torch.cuda.graph_pool_handle()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, pool=pool, stream=side):
+        loss = linear_cross_entropy(hidden, weight, targets)
+    with torch.cuda.graph(backward, pool=pool, stream=side):
+        grads = torch.autograd.grad(loss, (hidden, weight), up)
+    exact = head_exact(hidden, weight, targets, "mean", up)
+    for graph in (forward, backward, backward, forward, backward):
+        graph.replay()
+        torch.cuda.synchronize()
+        within(loss, exact[0]) if graph is forward else (within(grads[0], exact[1]), within(grads[1], exact[2]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_cross_entropy_of_many_tokens(dtype):
+    # more tokens than are counted at a time, and than the statistics of one turn hold
+    hidden, weight, targets = _head(20001, 16, 130, dtype, ignored=0.3)
+    for reduction in ("mean", "none"):
+        _check_head(hidden, weight, targets, reduction, workspace_bytes=4096 * 24)
+
+
 def test_cross_entropy_of_large_logits():
     hidden, weight, targets = _head(64, 64, 300, BF16)
     big = (hidden.detach() * 40).requires_grad_()
