@@ -32,7 +32,6 @@ namespace soapb200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kJoinSlices = 16;
 constexpr int kSingleThreads = 1024;
 
 void check(cudaError_t err, const char* what) {
@@ -132,22 +131,24 @@ __global__ void head_gather_kernel(const uint16_t* __restrict__ hidden, int64_t 
   }
 }
 
-// 32 tokens a block, lanes along tokens, the parts dealt to 16 warps and joined in a fixed order.
+// Eight tokens a block, their parts dealt to 64 threads each and joined in a fixed order.
 //
 // The target's logit is then computed anew in fp32, a warp to a token: where the tensor core's truncation makes all large logits a little too small
 // (5e-6 of themselves at K = 4096), a loss, which is a difference from the target's, would be off by 2e-6 of its own size.
+constexpr int kJoinTokens = 8, kJoinWarps = 16, kJoinSlices = kJoinWarps * 32 / kJoinTokens;
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinSlices)
+__global__ void __launch_bounds__(32 * kJoinWarps)
 head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number, const int* __restrict__ count, int first, int rows,
                  const int* __restrict__ column, const T* __restrict__ all, int64_t ld_all, int tokens, const T* __restrict__ packed, int64_t ld_packed,
                  const T* __restrict__ weight, int64_t ld_weight, int depth, float* __restrict__ lse, float* __restrict__ picked) {
-  __shared__ float2 shared[kJoinSlices][32];
-  __shared__ float exact[32];
+  __shared__ float2 shared[kJoinWarps][kJoinTokens];
+  __shared__ float exact[kJoinTokens];
   wait_for_predecessor();
   let_successor_start();
   const int counted = *count;
-  const int token = blockIdx.x * 32 + threadIdx.x;
-  const bool here = token < min(rows, counted - first);
+  const int valid = min(rows, counted - first);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int token = blockIdx.x * kJoinTokens + lane % kJoinTokens;
   float largest = -INFINITY, sum = 0.f;
   auto join = [&](const float2 part) {
     const float most = fmaxf(largest, part.x);
@@ -155,21 +156,22 @@ head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number,
     sum = sum * exp2f((largest - base) * kLog2e) + part.y * exp2f((part.x - base) * kLog2e);
     largest = most;
   };
-  if (here) {
+  if (token < valid) {
 #pragma unroll 4
-    for (int i = threadIdx.y; i < number; i += kJoinSlices) join(parts[i * ld_parts + token]);
+    for (int i = warp * (32 / kJoinTokens) + lane / kJoinTokens; i < number; i += kJoinSlices) join(parts[i * ld_parts + token]);
   }
-  shared[threadIdx.y][threadIdx.x] = make_float2(largest, sum);
 #pragma unroll
-  for (int i = 0; i < 32 / kJoinSlices; ++i) {
-    const int which = threadIdx.y + i * kJoinSlices, other = blockIdx.x * 32 + which;
-    const int word = other < min(rows, counted - first) ? column[first + other] : -1;
-    if (word < 0) continue;                // (the whole warp)
+  for (int o = kJoinTokens; o < 32; o <<= 1)
+    join(make_float2(__shfl_xor_sync(0xffffffffu, largest, o), __shfl_xor_sync(0xffffffffu, sum, o)));
+  if (lane < kJoinTokens) shared[warp][lane] = make_float2(largest, sum);
+  const int other = blockIdx.x * kJoinTokens + warp;
+  const int word = warp < kJoinTokens && other < valid ? column[first + other] : -1;
+  if (word >= 0) {                         // (the whole warp)
     const T* h = counted == tokens ? all + (first + other) * ld_all : packed + (first + other) * ld_packed;
     const T* w = weight + word * ld_weight;
     float dot = 0.f;
 #pragma unroll 4
-    for (int run = threadIdx.x; run < depth / 8; run += 32) {      // (rows lie on 16-byte boundaries)
+    for (int run = lane; run < depth / 8; run += 32) {      // (rows lie on 16-byte boundaries)
       Eight<T> a, b;
       a.load(h + 8 * run);
       b.load(w + 8 * run);
@@ -179,19 +181,19 @@ head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number,
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot = fmaf(u[j], v[j], dot);
     }
-    for (int j = depth / 8 * 8 + threadIdx.x; j < depth; j += 32) dot = fmaf(to_float(h[j]), to_float(w[j]), dot);
+    for (int j = depth / 8 * 8 + lane; j < depth; j += 32) dot = fmaf(to_float(h[j]), to_float(w[j]), dot);
 #pragma unroll
     for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (threadIdx.x == 0) exact[which] = dot;
+    if (lane == 0) exact[warp] = dot;
   }
   __syncthreads();
-  if (threadIdx.y == 0 && here) {
+  if (threadIdx.x < kJoinTokens && token < valid) {
 #pragma unroll
-    for (int s = 1; s < kJoinSlices; ++s) join(shared[s][threadIdx.x]);
+    for (int s = 1; s < kJoinWarps; ++s) join(shared[s][lane]);
     const float base = largest == -INFINITY ? 0.f : largest;
     float target = 0.f;
     if (column[first + token] >= 0) {
-      target = exact[threadIdx.x];
+      target = exact[lane];
       sum = sum - exp2f((picked[first + token] - base) * kLog2e) + exp2f((target - base) * kLog2e);
     }
     lse[first + token] = logf(sum) + base;
@@ -372,7 +374,7 @@ void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float
   gemm16(r.logits ? kLogitExponential : kLogitStatistics, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
   auto join = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    check(launch_dependent(head_join_kernel<T>, dim3((r.rows + 31) / 32), dim3(32, kJoinSlices), 0, stream, r.parts,
+    check(launch_dependent(head_join_kernel<T>, dim3((r.rows + kJoinTokens - 1) / kJoinTokens), dim3(32 * kJoinWarps), 0, stream, r.parts,
                            static_cast<int64_t>(r.rows), (p.words + kLogitPart - 1) / kLogitPart, p.count, r.first, r.rows, p.column,
                            static_cast<const T*>(p.hidden.data), p.hidden.ld, p.tokens, static_cast<const T*>(p.packed.data), p.packed.ld,
                            static_cast<const T*>(p.weight.data), p.weight.ld, p.depth, lse, picked),
