@@ -10,6 +10,10 @@
     python -m soap_tp_b200.bench.kernel_cases eig --size 4096 [--solver householder|jacobi]
     python -m torch.distributed.run --nproc-per-node 2 --master-addr 127.0.0.1 -m soap_tp_b200.bench.kernel_cases \
         gather --size 8192                                          # peer pull, traffic mix of an 8-GPU (2, 4) grid
+    python -m soap_tp_b200.bench.kernel_cases head --rows 4096 --size 4096 --words 16032     # cross entropy, loss and gradients
+    python -m soap_tp_b200.bench.kernel_cases norm --rows 16384 --size 4096                 # norm, gate and scale, forward and backward
+    python -m soap_tp_b200.bench.kernel_cases swiglu8 --rows 4096 --size 14336              # gated activation in 8 bits, the same
+    python -m soap_tp_b200.bench.kernel_cases pack8 --rows 32768 --size 4096                # there and back
 
 Each case allocates a few hundred MB at most, launches the kernel ``--repeats`` times and prints
 the CUDA-event time per launch, so the same command line serves for timing and, under ``ncu -k
@@ -104,12 +108,44 @@ def gather_case(args) -> int:
     return 0
 
 
+def decoder_case(args) -> int:
+    """One forward and backward pass of an operator of a decoder's training step (bf16)."""
+    from .. import ops
+
+    generator = torch.Generator(device="cuda").manual_seed(0)
+    rand = lambda *shape: torch.randn(*shape, generator=generator, device="cuda").bfloat16()
+    rows, size = args.rows, args.size
+    if args.case == "head":
+        hidden, weight = rand(rows, size).requires_grad_(), (rand(args.words, size) * size ** -0.5).requires_grad_()
+        targets = torch.randint(0, args.words, (rows,), generator=generator, device="cuda")
+        fn = lambda: torch.autograd.grad(ops.linear_cross_entropy(hidden, weight, targets), (hidden, weight))
+        work = f"{6 * rows * size * args.words / 1e12:.2f} TFLOP"
+    elif args.case == "norm":
+        x, branch = rand(rows, size).requires_grad_(), rand(rows, size).requires_grad_()
+        vectors = [torch.ones(size, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(3)]
+        grads = (rand(rows, size), rand(rows, size))
+        fn = lambda: torch.autograd.grad(ops.residual_norm(x, branch, vectors[0], branch_weight=vectors[1], gate=vectors[2], scale=0.5),
+                                         (x, branch, *vectors), grads)
+        work = f"{20 * rows * size / 1e9:.2f} GB"
+    elif args.case == "swiglu8":
+        gate, up, grad = rand(rows, size).requires_grad_(), rand(rows, size).requires_grad_(), rand(rows, size)
+        fn = lambda: torch.autograd.grad(ops.swiglu8(gate, up), (gate, up), grad)
+        work = f"{16.25 * rows * size / 1e9:.2f} GB"
+    else:
+        x = rand(rows, size)
+        fn = lambda: ops.unpack8(ops.pack8(x))
+        work = f"{6.125 * rows * size / 1e9:.2f} GB"
+    print(f"{args.case} {rows} x {size}: {timed(fn, args.repeats):.1f} us a pass of {work}")
+    return 0
+
+
 def main(argv=None) -> int:
     parser = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    parser.add_argument("case", choices=("gemm", "qr", "qrpair", "panel", "update", "adam", "split", "gather", "eig"))
+    parser.add_argument("case", choices=("gemm", "qr", "qrpair", "panel", "update", "adam", "split", "gather", "eig", "head", "norm", "swiglu8", "pack8"))
     parser.add_argument("--solver", choices=("householder", "jacobi"), default="householder", help="eig: which eigensolver")
     parser.add_argument("--size", type=int, default=4096)
     parser.add_argument("--rows", type=int, default=4096)
+    parser.add_argument("--words", type=int, default=16032, help="head: words of the vocabulary")
     parser.add_argument("--mode", default="store")
     parser.add_argument("--repeats", type=int, default=3)
     parser.add_argument("--pairs", action="store_true", help="panel: the two-columns-per-exchange kernel")
@@ -125,6 +161,8 @@ def main(argv=None) -> int:
 
     if args.case == "gather":
         return gather_case(args)
+    if args.case in ("head", "norm", "swiglu8", "pack8"):
+        return decoder_case(args)
     n = args.size
     device = torch.device("cuda", torch.cuda.current_device())
     generator = torch.Generator(device=device).manual_seed(0)

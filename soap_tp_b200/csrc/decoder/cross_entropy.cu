@@ -6,11 +6,13 @@
 // Tokens that do not count are left out from the start: the others' numbers, targets and hidden states are put one after another, every
 // product runs over those alone (their number stays on the device), and what the padding holds, NaN included, reaches nothing.
 //
-// The loss: one product (gemm16.cu) whose epilogue leaves, per token and 64 words, the largest logit and the sum of
-// exponentials relative to it; head_join_kernel joins these parts.  D goes through memory in 16 bits for a bounded number of tokens at a time, then
+// The loss: one product (gemm16.cu) whose epilogue leaves, per token and 64 words, the largest logit and the sum of exponentials relative to
+// it of all words but the target; head_join_kernel joins these parts to r = log sum over those words.  The target's logit t comes from an fp32
+// product of its own, and loss = log(1 + exp(r - t)), lse = t + loss, p_t - 1 = exp(-loss) - 1: a token that the model knows has a loss of 1e-4 and
+// less, of which a difference of lse and t in fp32 would leave two digits.  D goes through memory in 16 bits for a bounded number of tokens at a time, then
 // two products read it in both directions.  It comes about in one of two ways:
-//   * bf16 and one gradient of the loss for all tokens (mean, sum): the first product leaves the exponentials as well, one pass over them
-//     makes D of them once lse is known, and the gradients come with the loss, 6 N V K operations for N tokens.  The pass
+//   * bf16 and one gradient of the loss for all tokens (mean, sum): the first product leaves the exponentials as well (in fp16 times 2^15, which
+//     rounds them an eighth as much as D is rounded then, or to 2^-40 of the largest of their 64 words), one pass over them makes D of them once lse is known, and the gradients come with the loss, 6 N V K operations for N tokens.  The pass
 //     moves 4 N V bytes: 0.7 of 21 ms at 8192 x 4096 x 128256, where the product that it replaces takes 5.
 //   * fp16, whose gradients want the loss's scale before they are rounded, a gradient for each token, or a second backward pass: the logits
 //     are computed again once these are known, 8 N V K operations.
@@ -131,16 +133,14 @@ __global__ void head_gather_kernel(const uint16_t* __restrict__ hidden, int64_t 
   }
 }
 
-// Eight tokens a block, their parts dealt to 64 threads each and joined in a fixed order.
-//
-// The target's logit is then computed anew in fp32, a warp to a token: where the tensor core's truncation makes all large logits a little too small
-// (5e-6 of themselves at K = 4096), a loss, which is a difference from the target's, would be off by 2e-6 of its own size.
+// Eight tokens a block, their parts dealt to 64 threads each and joined in a fixed order.  The target's logit is computed in fp32, a warp to a token:
+// the tensor core's truncation makes all large logits a little too small (5e-6 of themselves at K = 4096).
 constexpr int kJoinTokens = 8, kJoinWarps = 16, kJoinSlices = kJoinWarps * 32 / kJoinTokens;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number, const int* __restrict__ count, int first, int rows,
                  const int* __restrict__ column, const T* __restrict__ all, int64_t ld_all, int tokens, const T* __restrict__ packed, int64_t ld_packed,
-                 const T* __restrict__ weight, int64_t ld_weight, int depth, float* __restrict__ lse, float* __restrict__ picked) {
+                 const T* __restrict__ weight, int64_t ld_weight, int depth, bool whole, TokenResults results) {
   __shared__ float2 shared[kJoinWarps][kJoinTokens];
   __shared__ float exact[kJoinTokens];
   wait_for_predecessor();
@@ -190,39 +190,43 @@ head_join_kernel(const float2* __restrict__ parts, int64_t ld_parts, int number,
   if (threadIdx.x < kJoinTokens && token < valid) {
 #pragma unroll
     for (int s = 1; s < kJoinWarps; ++s) join(shared[s][lane]);
-    const float base = largest == -INFINITY ? 0.f : largest;
-    float target = 0.f;
-    if (column[first + token] >= 0) {
-      target = exact[lane];
-      sum = sum - exp2f((picked[first + token] - base) * kLog2e) + exp2f((target - base) * kLog2e);
+    const float rest = logf(sum) + (largest == -INFINITY ? 0.f : largest);
+    const int at = first + token;
+    const bool known = column[at] >= 0;
+    const float target = known ? exact[lane] : 0.f;
+    if (whole && known) {
+      const float over = rest - target, by = log1pf(expf(-fabsf(over)));
+      results.loss[at] = over > 0.f ? over + by : by;
+      results.lse[at] = over > 0.f ? rest + by : target + by;
+    } else {
+      results.loss[at] = target;
+      results.lse[at] = rest;
     }
-    lse[first + token] = logf(sum) + base;
-    picked[first + token] = target;
   }
 }
 
-__device__ __forceinline__ float token_loss(int column, float lse, float picked) { return column == kUnknown ? nanf("") : lse - picked; }
+__device__ __forceinline__ float token_loss(int column, float loss) { return column == kUnknown ? nanf("") : loss; }
 
 // (the losses of tokens that do not count are cleared first)
 __global__ void head_token_losses_kernel(const int* __restrict__ count, const int* __restrict__ where, const int* __restrict__ column,
-                                         const float* __restrict__ lse, const float* __restrict__ picked, float* __restrict__ losses) {
+                                         const float* __restrict__ of_token, float* __restrict__ losses) {
   wait_for_predecessor();
   let_successor_start();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < *count) losses[where[i]] = token_loss(column[i], lse[i], picked[i]);
+  if (i < *count) losses[where[i]] = token_loss(column[i], of_token[i]);
 }
 
 // One block: the sum does not depend on the order in which blocks end.
 __global__ void __launch_bounds__(kSingleThreads)
-head_reduced_loss_kernel(const int* __restrict__ count, const int* __restrict__ column, const float* __restrict__ lse,
-                         const float* __restrict__ picked, bool mean, float* __restrict__ loss) {
+head_reduced_loss_kernel(const int* __restrict__ count, const int* __restrict__ column, const float* __restrict__ of_token, bool mean,
+                         float* __restrict__ loss) {
   __shared__ double shared[32];
   wait_for_predecessor();
   let_successor_start();
   const int counted = *count;
   double sum = 0.0;
 #pragma unroll 8
-  for (int i = threadIdx.x; i < counted; i += kSingleThreads) sum += token_loss(column[i], lse[i], picked[i]);
+  for (int i = threadIdx.x; i < counted; i += kSingleThreads) sum += token_loss(column[i], of_token[i]);
   sum = block_reduce(sum, [](double a, double b) { return a + b; }, shared);
   if (threadIdx.x == 0) *loss = static_cast<float>(mean && counted ? sum / counted : sum);
 }
@@ -263,7 +267,7 @@ constexpr int kRescaleThreads = 256, kRescaleRuns = 4;
 __global__ void __launch_bounds__(kRescaleThreads)
 head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, const int* __restrict__ count, int first, int rows,
                     const float2* __restrict__ parts, int64_t ld_parts, const int* __restrict__ column, const float* __restrict__ lse,
-                    const float* __restrict__ picked, const float* __restrict__ factor) {
+                    const float* __restrict__ loss, const float* __restrict__ factor) {
   wait_for_predecessor();
   let_successor_start();
   const int row = blockIdx.y;
@@ -275,13 +279,13 @@ head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, c
   __nv_bfloat16* line = logits + row * ld;
   const int run0 = blockIdx.x * kRescaleThreads * kRescaleRuns + threadIdx.x;
   const int runs = (words + 7) / 8;        // (the pitch is a multiple of 8)
-  Eight<__nv_bfloat16> e[kRescaleRuns];
+  Eight<__half> e[kRescaleRuns];
   float largest[kRescaleRuns];
 #pragma unroll
   for (int i = 0; i < kRescaleRuns; ++i) {
     const int run = run0 + i * kRescaleThreads;
     if (here && run < runs) {
-      e[i].load(line + 8 * run);
+      e[i].load(reinterpret_cast<const __half*>(line + 8 * run));
       largest[i] = parts[(run / (kLogitPart / 8)) * ld_parts + row].x;
     }
   }
@@ -289,24 +293,24 @@ head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, c
   for (int i = 0; i < kRescaleRuns; ++i) {
     const int run = run0 + i * kRescaleThreads;
     if (run >= runs) break;
+    Eight<__nv_bfloat16> d;
     if (here) {
       float v[8];
       e[i].get(v);
-      const float by = exp2f((largest[i] - l) * kLog2e) * f;
+      const float by = exp2f((largest[i] - l) * kLog2e) * (f * (1.f / 32768.f));
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= by;
       if (target >= 8 * run && target < 8 * run + 8) {
-        // from the target's logit itself: its probability, less one, is small where the model knows the word
-        const float d = expm1f(picked[first + row] - l) * f;
+        const float of_target = expm1f(-loss[first + row]) * f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (target == 8 * run + j) v[j] = d;
+          if (target == 8 * run + j) v[j] = of_target;
       }
-      e[i].set(v);
+      d.set(v);
     } else {
-      e[i].clear();
+      d.clear();
     }
-    e[i].store(line + 8 * run);
+    d.store(line + 8 * run);
   }
 }
 
@@ -367,31 +371,30 @@ void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, LossR
         "head_gather");
 }
 
-void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float* picked, int* status, cudaStream_t stream) {
-  Gemm16Problem g = logits_of(p, r);
-  g.picked = picked + r.first;
+void head_statistics(const HeadProblem& p, const LogitRows& r, const TokenResults& t, bool whole, int* status, cudaStream_t stream) {
+  const Gemm16Problem g = logits_of(p, r);
   const Hidden16 hidden = hidden_of(p, r.first);
   gemm16(r.logits ? kLogitExponential : kLogitStatistics, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
-  auto join = [&](auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
+  auto join = [&](auto* type) {
+    using T = std::remove_pointer_t<decltype(type)>;
     check(launch_dependent(head_join_kernel<T>, dim3((r.rows + kJoinTokens - 1) / kJoinTokens), dim3(32 * kJoinWarps), 0, stream, r.parts,
                            static_cast<int64_t>(r.rows), (p.words + kLogitPart - 1) / kLogitPart, p.count, r.first, r.rows, p.column,
                            static_cast<const T*>(p.hidden.data), p.hidden.ld, p.tokens, static_cast<const T*>(p.packed.data), p.packed.ld,
-                           static_cast<const T*>(p.weight.data), p.weight.ld, p.depth, lse, picked),
+                           static_cast<const T*>(p.weight.data), p.weight.ld, p.depth, whole, t),
           "head_join");
   };
   if (p.bf16) join(static_cast<__nv_bfloat16*>(nullptr));
   else join(static_cast<__half*>(nullptr));
 }
 
-void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, cudaStream_t stream) {
+void head_losses(const HeadProblem& p, const TokenResults& t, LossReduction reduction, float* loss, cudaStream_t stream) {
   if (reduction == kLossNone) {
     const cudaError_t err = cudaMemsetAsync(loss, 0, sizeof(float) * p.tokens, stream);
     if (err != cudaSuccess) throw std::runtime_error(std::string("head_losses: ") + cudaGetErrorString(err));
-    check(launch_dependent(head_token_losses_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p.count, p.where, p.column, lse, picked, loss),
+    check(launch_dependent(head_token_losses_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p.count, p.where, p.column, t.loss, loss),
           "head_token_losses");
   } else {
-    check(launch_dependent(head_reduced_loss_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.count, p.column, lse, picked,
+    check(launch_dependent(head_reduced_loss_kernel, dim3(1), dim3(kSingleThreads), 0, stream, p.count, p.column, t.loss,
                            reduction == kLossMean, loss),
           "head_reduced_loss");
   }
@@ -403,7 +406,7 @@ void head_factors(const HeadProblem& p, LossReduction reduction, const float* gr
         "head_factors");
 }
 
-void head_rescale(const HeadProblem& p, const LogitRows& r, const float* lse, const float* picked, const float* factor, cudaStream_t stream) {
+void head_rescale(const HeadProblem& p, const LogitRows& r, const TokenResults& t, const float* factor, cudaStream_t stream) {
   const Gemm16Problem g = logits_of(p, r);
   constexpr int kWords = 8 * kRescaleThreads * kRescaleRuns;
   // (the grid's second extent is at most 65535)
@@ -411,14 +414,14 @@ void head_rescale(const HeadProblem& p, const LogitRows& r, const float* lse, co
     const int rows = std::min(r.rows - begin, 65472);
     check(launch_dependent(head_rescale_kernel, dim3((p.words + kWords - 1) / kWords, rows), dim3(kRescaleThreads), 0, stream,
                            static_cast<__nv_bfloat16*>(g.C) + begin * g.ldc, g.ldc, p.words, p.count, r.first + begin, rows, r.parts + begin,
-                           g.ld_parts, p.column, lse, picked, factor),
+                           g.ld_parts, p.column, t.lse, t.loss, factor),
           "head_rescale");
   }
 }
 
-void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const float* lse, const float* factor, int* status, cudaStream_t stream) {
+void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const TokenResults& t, const float* factor, int* status, cudaStream_t stream) {
   Gemm16Problem g = logits_of(p, r);
-  g.lse = lse + r.first; g.factor = factor + r.first;
+  g.lse = t.lse + r.first; g.loss = t.loss + r.first; g.factor = factor + r.first;
   const Hidden16 hidden = hidden_of(p, r.first);
   gemm16(kLogitGradient, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
 }

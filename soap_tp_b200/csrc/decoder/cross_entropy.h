@@ -31,29 +31,36 @@ constexpr int kElsewhere = -1, kUnknown = -2;
 // With `factor` (bf16, sum or mean) what head_factors leaves for a gradient of one as well.
 void head_prepare(const HeadProblem& p, void* d_hidden, int64_t ld_hidden, LossReduction reduction, float* factor, float* alpha, cudaStream_t stream);
 
-// For tokens first .. first + rows of those that count: lse[i] = log sum_j exp(l_ij) over this rank's words, picked[i] = l_i,t_i where the
-// target is one of them and 0 elsewhere.  `parts`: ceil(words / kLogitPart) x rows pairs.  With `logits` (bf16) the exponentials stay
-// there, each relative to the largest of its part.
+// What the loss and its gradient need of each token that counts, by its number among them.
+struct TokenResults {
+  float* lse;               // log sum_j exp(l_ij)
+  float* loss;              // lse - l_i,t_i
+};
+
+// For tokens first .. first + rows of those that count.  `whole`: this rank has all words, and lse and loss are filled.  Otherwise `lse` gets that of
+// this rank's words but for the target, and `loss` the target's logit where this rank has it and 0 elsewhere; joined over the
+// ranks, rest and logit, they give loss = log(1 + exp(rest - logit)) and lse = logit + loss.
+// `parts`: ceil(words / kLogitPart) x rows pairs.  With `logits` (bf16) the exponentials stay there as fp16, 2^15 times those relative to the
+// largest of their part.
 struct LogitRows {
   int first, rows;
   void* logits;
   int64_t ld_logits;
   float2* parts;
 };
-void head_statistics(const HeadProblem& p, const LogitRows& r, float* lse, float* picked, int* status, cudaStream_t stream);
+void head_statistics(const HeadProblem& p, const LogitRows& r, const TokenResults& t, bool whole, int* status, cudaStream_t stream);
 
-// losses = lse - picked by token; 0 for tokens that do not count, NaN for targets outside the vocabulary.  With a reduction the result
-// goes to `loss`.
-void head_losses(const HeadProblem& p, const float* lse, const float* picked, LossReduction reduction, float* loss, cudaStream_t stream);
+// The losses by token; 0 for tokens that do not count, NaN for targets outside the vocabulary.  With a reduction one number.
+void head_losses(const HeadProblem& p, const TokenResults& t, LossReduction reduction, float* loss, cudaStream_t stream);
 
 // What the gradient of the loss multiplies the row of a token that counts by: factor[i] * *alpha.  `grad_loss` has one value per token,
 // or one.
 void head_factors(const HeadProblem& p, LossReduction reduction, const float* grad_loss, float* factor, float* alpha, cudaStream_t stream);
 
 // The exponentials that head_statistics left become the logits' gradient, factor (exp(l - lse) - [target]).
-void head_rescale(const HeadProblem& p, const LogitRows& r, const float* lse, const float* picked, const float* factor, cudaStream_t stream);
+void head_rescale(const HeadProblem& p, const LogitRows& r, const TokenResults& t, const float* factor, cudaStream_t stream);
 // The logits' gradient from the logits anew.
-void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const float* lse, const float* factor, int* status, cudaStream_t stream);
+void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const TokenResults& t, const float* factor, int* status, cudaStream_t stream);
 
 // Gradients of the hidden states and the weight (either may be null) from the logits' gradient of these rows.  The weight's is summed over
 // the turns in `sum`, words x ld_sum floats, where one does not take all tokens.

@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <pybind11/functional.h>
 
 #include <algorithm>
 #include <atomic>
@@ -349,7 +350,7 @@ float2* pairs(const Tensor& parts) { return reinterpret_cast<float2*>(parts.data
 struct LossOptions {
   int64_t reduction, ignore_index, first_word, vocabulary, workspace_bytes, status;
   bool want_hidden, want_weight;
-  std::function<void(const Tensor&, const Tensor&)> join;      // log-sum-exp and target's logit over several ranks, in place
+  std::function<void(const Tensor&, const Tensor&)> join;      // makes lse and loss of what several ranks have (head_statistics), in place
   std::vector<int64_t> numbers() const {
     return {reduction, ignore_index, first_word, vocabulary, workspace_bytes, status, want_hidden, want_weight};
   }
@@ -373,8 +374,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     const auto reduction = static_cast<LossReduction>(o.reduction);
     const auto floats = hidden.options().dtype(at::kFloat);
     const Tensor both = at::empty({2, p.tokens}, floats);
-    const Tensor lse = both.select(0, 0), picked = both.select(0, 1);
-    float *lse_at = lse.data_ptr<float>(), *picked_at = picked.data_ptr<float>();
+    const Tensor lse = both.select(0, 0), losses = both.select(0, 1);
+    const TokenResults t{lse.data_ptr<float>(), losses.data_ptr<float>()};
+    const bool whole = !o.join;
     // bf16 only: fp16 gradients are rounded after the loss's scale, which the backward pass brings, has been multiplied in
     const bool with_loss = (o.want_hidden || o.want_weight) && reduction != kLossNone && p.bf16;
     if (with_loss) {
@@ -383,9 +385,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       const Tensor parts = head.parts(g.rows);
       for (int first = 0; first < p.tokens; first += g.rows) {
         const LogitRows r = g.turn(head, first, pairs(parts));
-        head_statistics(p, r, lse_at, picked_at, head.status, stream);
-        if (o.join) o.join(lse.narrow(0, first, r.rows), picked.narrow(0, first, r.rows));
-        head_rescale(p, r, lse_at, picked_at, g.factors(), stream);
+        head_statistics(p, r, t, whole, head.status, stream);
+        if (o.join) o.join(lse.narrow(0, first, r.rows), losses.narrow(0, first, r.rows));
+        head_rescale(p, r, t, g.factors(), stream);
         head_gradients(p, r, g.alpha(), g.made, head.status, stream);
         count(3 + g.products());
       }
@@ -397,16 +399,16 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       const int rows = static_cast<int>(std::min<int64_t>(p.tokens, std::max<int64_t>(256, o.workspace_bytes / parts_of_token / 256 * 256)));
       const Tensor parts = head.parts(rows);
       for (int first = 0; first < p.tokens; first += rows) {
-        head_statistics(p, LogitRows{first, std::min(rows, p.tokens - first), nullptr, 0, pairs(parts)}, lse_at, picked_at, head.status, stream);
+        head_statistics(p, LogitRows{first, std::min(rows, p.tokens - first), nullptr, 0, pairs(parts)}, t, whole, head.status, stream);
         count(2);
       }
-      if (o.join) o.join(lse, picked);
+      if (o.join) o.join(lse, losses);
     }
     count(2);
     Tensor loss = reduction == kLossNone ? at::empty(targets.sizes(), floats) : at::empty({}, floats);
-    head_losses(p, lse_at, picked_at, reduction, loss.data_ptr<float>(), stream);
+    head_losses(p, t, reduction, loss.data_ptr<float>(), stream);
     count(1);
-    ctx->save_for_backward({hidden, weight, targets, lse});
+    ctx->save_for_backward({hidden, weight, targets, both});
     ctx->saved_data["numbers"] = o.numbers();
     ctx->saved_data["made"] = with_loss;
     ctx->saved_data["capture"] = capture_id();
@@ -415,7 +417,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &hidden = saved[0], &weight = saved[1], &targets = saved[2], &lse = saved[3];
+    const Tensor &hidden = saved[0], &weight = saved[1], &targets = saved[2], &both = saved[3];
     const c10::cuda::CUDAGuard guard(hidden.device());
     variable_list result(4);
     const bool graph = at::GradMode::is_enabled();
@@ -446,7 +448,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         head_factors(p, static_cast<LossReduction>(o[0]), grad_loss.data_ptr<float>(), g.factors(), g.alpha(), stream);
         for (int first = 0; first < p.tokens; first += g.rows) {
           const LogitRows r = g.turn(head, first, nullptr);
-          head_logit_gradient(p, r, lse.data_ptr<float>(), g.factors(), head.status, stream);
+          head_logit_gradient(p, r, TokenResults{both.data_ptr<float>(), both.data_ptr<float>() + p.tokens}, g.factors(), head.status, stream);
           head_gradients(p, r, g.alpha(), g.made, head.status, stream);
           count(1 + g.products());
         }

@@ -149,12 +149,13 @@ __device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t
   const int rows = min(32, (EPI == kLogitGradient ? min(p.M, (M + kBK - 1) / kBK * kBK) : M) - m_warp);
   const int target = inside ? p.targets[row] - n0 : -1;
   const uint64_t scale = pack_floats(kLog2e, kLog2e);
+  using Stored = std::conditional_t<EPI == kLogitExponential, __half, T>;
   auto store = [&](auto value) {                          // value(j): the 16-bit result's column j
 #pragma unroll
     for (int c = 0; c < kLogitPart; c += 32) {
       uint32_t words[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) words[j] = pack16<T>(value(c + 2 * j), value(c + 2 * j + 1));
+      for (int j = 0; j < 16; ++j) words[j] = pack16<Stored>(value(c + 2 * j), value(c + 2 * j + 1));
       if (rows > 0 && c < cols) store_values<64>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
     }
   };
@@ -171,30 +172,23 @@ __device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t
   auto value = [&](int j) { return pair_element(sums[j / 2], j & 1); };
   if constexpr (EPI == kLogitGradient) {
     const float factor = inside ? p.factor[row] : 0.f;
+    // from the loss itself: the target's probability, less one, is small where the model knows the word
+    const float of_target = inside && target >= 0 && target < cols ? expm1f(-p.loss[row]) : 0.f;
     exponents(inside ? p.lse[row] * kLog2e : 0.f);
-    store([&](int j) {
-      const float e = exp2_fast(value(j));
-      return inside ? (target == j ? e - 1.f : e) * factor : 0.f;
-    });
+    store([&](int j) { return inside ? (target == j ? of_target : exp2_fast(value(j))) * factor : 0.f; });
   } else {
     if (cols < kLogitPart) {
 #pragma unroll
       for (int j = 0; j < kLogitPart; j += 2)
         sums[j / 2] = pack_floats(j < cols ? value(j) : -INFINITY, j + 1 < cols ? value(j + 1) : -INFINITY);
     }
-    if (inside && target >= 0 && target < cols) {
-      float picked = 0.f;
-#pragma unroll
-      for (int j = 0; j < kLogitPart; ++j)
-        if (target == j) picked = value(j);
-      p.picked[row] = picked;
-    }
     float most[4] = {value(0), value(1), value(2), value(3)};
 #pragma unroll
     for (int j = 4; j < kLogitPart; ++j) most[j & 3] = fmaxf(most[j & 3], value(j));
     const float largest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
     // (a row of no finite logit is taken relative to zero, so that its sum is zero, or NaN where a logit is)
-    exponents(largest == -INFINITY ? 0.f : largest * kLog2e);
+    constexpr float kUp = EPI == kLogitExponential ? 15.f : 0.f;
+    exponents(largest == -INFINITY ? -kUp : largest * kLog2e - kUp);
     uint64_t sum[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < kLogitPart; j += 2) {
@@ -202,8 +196,14 @@ __device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t
       add_pair(sum[(j >> 1) & 1], sums[j / 2]);
     }
     add_pair(sum[0], sum[1]);
+    float others = pair_element(sum[0], 0) + pair_element(sum[0], 1);
+    if (inside && target >= 0 && target < cols) {      // (added up without it: where the model knows the word, nothing would be left of a difference)
+      others = 0.f;
+#pragma unroll
+      for (int j = 0; j < kLogitPart; ++j) others += target == j ? 0.f : value(j);
+    }
     if (inside && cols > 0)
-      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.ld_parts + row] = make_float2(largest, pair_element(sum[0], 0) + pair_element(sum[0], 1));
+      p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.ld_parts + row] = make_float2(largest, EPI == kLogitExponential ? others * (1.f / 32768.f) : others);
     if constexpr (EPI == kLogitExponential) store(value);
   }
 }

@@ -15,8 +15,8 @@ struct Matrix16 {
 };
 
 enum Gemm16Epilogue : int {
-  kLogitStatistics = 0,     // largest logit and sum of exponentials per row and 64 columns, and the logit of each row's target
-  kLogitExponential = 1,    // the same, and the exponentials themselves, relative to the largest of their part, as a 16-bit matrix
+  kLogitStatistics = 0,     // largest logit and sum of exponentials, but for the row's target, per row and 64 columns
+  kLogitExponential = 1,    // the same, and the exponentials themselves, relative to the largest of their part, times 2^15 in fp16
   kLogitGradient = 2,       // softmax minus target, times the row's factor, as a 16-bit matrix
   kStore16 = 3,             // the product itself
 };
@@ -31,10 +31,10 @@ struct Gemm16Problem {
   int first;
   // logits: row i is a token, column j a word
   const int* targets;       // [M]: the column that is the token's target; negative where none of them is
-  float2* parts;            // [ceil(N / kLogitPart)][ld_parts]: largest logit, sum of exp(logit - largest)
+  float2* parts;            // [ceil(N / kLogitPart)][ld_parts]: largest logit, sum of exp(logit - largest) over all but the target
   int64_t ld_parts;
-  float* picked;            // [M]: the target's logit, written where the target is a column
   const float* lse;         // [M]
+  const float* loss;        // [M]: lse - the target's logit
   const float* factor;      // [M]
   // 16-bit result [M][ldc]
   void* C;

@@ -18,6 +18,7 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
+import torch.nn.functional as F
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
@@ -67,12 +68,24 @@ def _world(group) -> int:
     return 1 if group is None else dist.get_world_size(group)
 
 
-def _join(group, lse: Tensor, picked: Tensor) -> None:
-    """``lse`` becomes that over all ranks' words, ``picked`` the target's logit on every rank (both in place)."""
-    every = [torch.empty_like(lse) for _ in range(_world(group))]
-    dist.all_gather(every, lse, group=group)
-    dist.all_reduce(picked, group=group)
-    lse.copy_(torch.logsumexp(torch.stack(every), dim=0))
+def _finish(rest: Tensor, picked: Tensor):
+    """Log-sum-exp and loss from the log-sum-exp of all words but the target and the target's logit.  (Not their difference: of the loss of
+    a token that the model knows nothing would be left.)"""
+    over = rest - picked
+    loss = F.softplus(over)
+    return torch.where(over > 0, rest + F.softplus(-over), picked + loss), loss
+
+
+def _join(group, lse: Tensor, loss: Tensor) -> None:
+    """From this rank's log-sum-exp of its words but the target and the target's logit (0 where it has it not) to those of all ranks' words and
+    the loss, in place."""
+    most = lse.clone()
+    dist.all_reduce(most, op=dist.ReduceOp.MAX, group=group)
+    most = torch.where(most == float("-inf"), torch.zeros_like(most), most)
+    sums = torch.stack(((lse - most).exp(), loss))
+    dist.all_reduce(sums, group=group)
+    for to, value in zip((lse, loss), _finish(most + sums[0].log(), sums[1])):
+        to.copy_(value)
 
 
 def _wide(dtype: torch.dtype) -> torch.dtype:
@@ -92,11 +105,14 @@ class _HostHead:
         self.local = torch.where(self.mine, local, 0).unsqueeze(1)
 
     def statistics(self):
+        """Log-sum-exp of these words but the target, and the target's logit (0 where it is elsewhere)."""
         logits = self.hidden @ self.weight.t()
-        return torch.logsumexp(logits, dim=1), logits.gather(1, self.local).squeeze(1) * self.mine
+        picked = logits.gather(1, self.local).squeeze(1) * self.mine
+        logits.scatter_(1, self.local, torch.where(self.mine.unsqueeze(1), float("-inf"), logits.gather(1, self.local)))
+        return torch.logsumexp(logits, dim=1), picked
 
-    def losses(self, lse, picked, reduction):
-        losses = torch.where(self.counts, lse - picked, torch.zeros_like(lse))
+    def losses(self, losses, reduction):
+        losses = torch.where(self.counts, losses, torch.zeros_like(losses))
         counted = self.counts.sum().to(losses.dtype)
         if reduction == "none":
             return losses, counted
@@ -124,10 +140,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
         shape = targets.shape
         hidden, targets = hidden.detach().reshape(-1, hidden.shape[-1]), targets.reshape(-1)
         head = _HostHead(hidden, weight, targets, *ctx.arguments)
-        lse, picked = head.statistics()
+        lse, losses = head.statistics()
         if world > 1:
-            _join(group, lse, picked)
-        loss, counted = head.losses(lse, picked, reduction)
+            _join(group, lse, losses)
+        else:
+            lse, losses = _finish(lse, losses)
+        loss, counted = head.losses(losses, reduction)
         ctx.save_for_backward(hidden, weight, targets, lse, counted)
         return loss.view(shape) if reduction == "none" else loss
 

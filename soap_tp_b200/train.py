@@ -8,7 +8,8 @@ SOAP-TP runs on every 2-D tensor-parallel weight: two-sided where both sides are
 one-sided (identity basis on the sharded, vocabulary-sized side, as original SOAP does above its
 ``max_precond_dim``) for the embedding and the head; AdamW on 1-D parameters.  Token ids are uniform
 random (there is no dataset here); weights are random-initialised in bf16, optimizer state is fp32.
-Rank 0 prints one ``SOAP_TIMING``-style JSON line per step and a summary.
+Rank 0 prints one ``SOAP_TIMING``-style JSON line per step and a summary.  ``--fused-loss``, ``--fused-norms``, ``--mlp-bits 8`` and
+``--checkpoint-activations --checkpoint-bits 8`` run the model's own step on the package's operators (``soap_tp_b200.ops``).
 """
 from __future__ import annotations
 

@@ -224,6 +224,27 @@ def test_cross_entropy_of_many_tokens(dtype):
         _check_head(hidden, weight, targets, reduction, workspace_bytes=4096 * 24)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_cross_entropy_of_known_words(dtype, reduction):
+    # targets far ahead of all others: losses from 1 down to 1e-30, each to its own size
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    weight = torch.eye(128, 64, device="cuda", dtype=dtype) * 4
+    targets = torch.arange(60, device="cuda")
+    hidden = torch.zeros(60, 64, device="cuda", dtype=dtype)
+    hidden[targets, targets] = torch.linspace(1.0, 16.0, 60, device="cuda").to(dtype)
+    hidden, weight = hidden.requires_grad_(), weight.requires_grad_()
+    losses = linear_cross_entropy(hidden, weight, targets, reduction="none")
+    exact = (127 * torch.exp(-4.0 * hidden.detach().double()[targets, targets])).log1p()
+    # exact logits here: exp, log and sums of 127 equal terms in fp32
+    within(losses, (exact, 2.0 ** -18 * exact))
+    grads = torch.autograd.grad(linear_cross_entropy(hidden, weight, targets, reduction=reduction), hidden,
+                                torch.ones(60, device="cuda") if reduction == "none" else None)[0]
+    exact = 4 * torch.expm1(-exact)                      # by the target's word alone
+    within(grads[targets, targets], (exact, (2 * half_step(dtype) + 2.0 ** -17) * exact.abs() + (2.0 ** -24 if dtype == FP16 else 0.0)))
+
+
 def test_cross_entropy_of_large_logits():
     hidden, weight, targets = _head(64, 64, 300, BF16)
     big = (hidden.detach() * 40).requires_grad_()
@@ -235,6 +256,35 @@ def test_cross_entropy_refuses_fp32_on_cuda():
 
     with pytest.raises(TypeError):
         linear_cross_entropy(_rand(2, 8), _rand(4, 8), torch.zeros(2, dtype=torch.int64, device="cuda"))
+
+
+def _sharded_case(rank, world):
+    # two ranks on one GPU, whose collectives go over the host; nothing on the device waits for the other rank
+    import torch.distributed as dist
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    for dtype, reduction, workspace in ((BF16, "mean", 1), (BF16, "sum", 2**31), (FP16, "none", 1), (BF16, "none", 2**31)):
+        hidden, weight, targets = _head(600, 72, 640, dtype, ignored=0.2)
+        per_rank = 640 // world
+        mine = weight.detach()[rank * per_rank:(rank + 1) * per_rank].clone().requires_grad_()
+        loss = linear_cross_entropy(hidden, mine, targets, reduction=reduction, group=dist.group.WORLD, workspace_bytes=workspace)
+        up = torch.rand(600, generator=torch.Generator("cuda").manual_seed(9), device="cuda") if reduction == "none" else None
+        d_hidden, d_weight = torch.autograd.grad(loss, (hidden, mine), up)
+        losses, exact_hidden, exact_weight = head_exact(hidden, weight, targets, reduction, up)
+        within(loss, losses)
+        # each of the two ranks' parts of the hidden states' gradient is rounded before they are added: by half a step of the sums' magnitudes,
+        # or half of the smallest subnormal number
+        p = torch.softmax(hidden.detach().double() @ weight.detach().double().t(), dim=1)
+        sizes = (p @ weight.detach().double().abs() + weight.detach().double()[targets.clamp(min=0)].abs()) * (targets != IGNORED).unsqueeze(1)
+        sizes = sizes * (up.unsqueeze(1) if up is not None else 1.0 if reduction == "sum" else 1.0 / int((targets != IGNORED).sum()))
+        within(d_hidden, (exact_hidden[0], exact_hidden[1] + 2 * half_step(dtype) * sizes + 2 * smallest(dtype)))
+        within(d_weight, (exact_weight[0][rank * per_rank:(rank + 1) * per_rank], exact_weight[1][rank * per_rank:(rank + 1) * per_rank]))
+
+
+def test_cross_entropy_over_two_ranks():
+    from distributed_helpers import run_distributed
+
+    run_distributed(_sharded_case, 2)
 
 
 def test_cross_entropy_beyond_32_bits():
