@@ -265,7 +265,7 @@ head_factors_kernel(const int* __restrict__ count, const int* __restrict__ where
 // are read as part of K.
 constexpr int kRescaleThreads = 256, kRescaleRuns = 4;
 __global__ void __launch_bounds__(kRescaleThreads)
-head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, const int* __restrict__ count, int first, int rows,
+head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int64_t second, int words, const int* __restrict__ count, int first, int rows,
                     const float2* __restrict__ parts, int64_t ld_parts, const int* __restrict__ column, const float* __restrict__ lse,
                     const float* __restrict__ loss, const float* __restrict__ factor) {
   wait_for_predecessor();
@@ -278,7 +278,8 @@ head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, c
   const int target = here ? column[first + row] : -1;
   __nv_bfloat16* line = logits + row * ld;
   const int run0 = blockIdx.x * kRescaleThreads * kRescaleRuns + threadIdx.x;
-  const int runs = (words + 7) / 8;        // (the pitch is a multiple of 8)
+  // (the pitch is a multiple of 64; with a second term both are cleared up to the next multiple)
+  const int runs = second ? (words + 63) / 64 * 8 : (words + 7) / 8;
   Eight<__half> e[kRescaleRuns];
   float largest[kRescaleRuns];
 #pragma unroll
@@ -293,13 +294,13 @@ head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, c
   for (int i = 0; i < kRescaleRuns; ++i) {
     const int run = run0 + i * kRescaleThreads;
     if (run >= runs) break;
-    Eight<__nv_bfloat16> d;
+    Eight<__nv_bfloat16> d, left;
     if (here) {
       float v[8];
       e[i].get(v);
       const float by = exp2f((largest[i] - l) * kLog2e) * (f * (1.f / 32768.f));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= by;
+      for (int j = 0; j < 8; ++j) v[j] = 8 * run + j < words ? v[j] * by : 0.f;
       if (target >= 8 * run && target < 8 * run + 8) {
         const float of_target = expm1f(-loss[first + row]) * f;
 #pragma unroll
@@ -307,10 +308,17 @@ head_rescale_kernel(__nv_bfloat16* __restrict__ logits, int64_t ld, int words, c
           if (target == 8 * run + j) v[j] = of_target;
       }
       d.set(v);
+      float back[8];
+      d.get(back);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] -= back[j];
+      left.set(v);
     } else {
       d.clear();
+      left.clear();
     }
     d.store(line + 8 * run);
+    if (second) left.store(line + second + 8 * run);
   }
 }
 
@@ -409,11 +417,12 @@ void head_factors(const HeadProblem& p, LossReduction reduction, const float* gr
 void head_rescale(const HeadProblem& p, const LogitRows& r, const TokenResults& t, const float* factor, cudaStream_t stream) {
   const Gemm16Problem g = logits_of(p, r);
   constexpr int kWords = 8 * kRescaleThreads * kRescaleRuns;
+  if (r.second % 64 != 0 || r.ld_logits < r.second + (p.words + 63) / 64 * 64) throw std::invalid_argument("head_rescale: no room for both terms");
   // (the grid's second extent is at most 65535)
   for (int begin = 0; begin < r.rows; begin += 65472) {
     const int rows = std::min(r.rows - begin, 65472);
     check(launch_dependent(head_rescale_kernel, dim3((p.words + kWords - 1) / kWords, rows), dim3(kRescaleThreads), 0, stream,
-                           static_cast<__nv_bfloat16*>(g.C) + begin * g.ldc, g.ldc, p.words, p.count, r.first + begin, rows, r.parts + begin,
+                           static_cast<__nv_bfloat16*>(g.C) + begin * g.ldc, g.ldc, r.second, p.words, p.count, r.first + begin, rows, r.parts + begin,
                            g.ld_parts, p.column, t.lse, t.loss, factor),
           "head_rescale");
   }
@@ -421,6 +430,7 @@ void head_rescale(const HeadProblem& p, const LogitRows& r, const TokenResults& 
 
 void head_logit_gradient(const HeadProblem& p, const LogitRows& r, const TokenResults& t, const float* factor, int* status, cudaStream_t stream) {
   Gemm16Problem g = logits_of(p, r);
+  g.second = r.second;
   g.lse = t.lse + r.first; g.loss = t.loss + r.first; g.factor = factor + r.first;
   const Hidden16 hidden = hidden_of(p, r.first);
   gemm16(kLogitGradient, p.bf16, hidden.packed, p.weight, g, status, stream, &hidden);
@@ -434,7 +444,7 @@ void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha
     d.M = r.rows; d.N = p.depth; d.K = p.words;
     d.count = p.count; d.first = r.first;
     d.C = out.hidden; d.ldc = out.ld_hidden; d.where = p.where + r.first;
-    d.alpha = alpha;
+    d.alpha = alpha; d.second = r.second;
     d.split_parts = out.split_parts; d.split_counters = p.split_counters;
     gemm16(kStore16, p.bf16, Matrix16{r.logits, r.ld_logits, true}, Matrix16{p.weight.data, p.weight.ld, false}, d, status, stream);
   }
@@ -442,7 +452,7 @@ void head_gradients(const HeadProblem& p, const LogitRows& r, const float* alpha
     Gemm16Problem d{};
     d.M = p.words; d.N = p.depth; d.K = r.rows;
     d.count = p.count; d.first = r.first;
-    d.alpha = alpha;
+    d.alpha = alpha; d.second = r.second;
     d.accumulator = out.sum; d.ld_accumulator = out.ld_sum; d.add = r.first > 0;
     d.split_parts = out.split_parts; d.split_counters = p.split_counters;
     if (last) {

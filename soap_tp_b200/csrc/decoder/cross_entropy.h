@@ -47,7 +47,12 @@ struct LogitRows {
   void* logits;
   int64_t ld_logits;
   float2* parts;
+  int64_t second;           // columns from the logits' gradient to what its rounding left, or 0 (Gemm16Problem)
 };
+// Up to so many tokens the logits' gradient has two terms: there the roundings of a few large values, a target's above all, are most of a
+// gradient's error, where over many tokens they average out.  (15 tokens x 228 x 2011: 0.0029 of the gradient, 0.0016 with two; 8192 x
+// 4096 x 128256: 0.0019.)  It costs the tensor cores time that so few tokens leave them.
+constexpr int kFewTokens = 256;
 void head_statistics(const HeadProblem& p, const LogitRows& r, const TokenResults& t, bool whole, int* status, cudaStream_t stream);
 
 // The losses by token; 0 for tokens that do not count, NaN for targets outside the vocabulary.  With a reduction one number.

@@ -319,6 +319,7 @@ struct Head {
 struct Gradients {
   Tensor hidden, weight, logits, sum, factor, split_parts;
   int rows;
+  int64_t second;
   HeadGradients made{};
 
   Gradients(const Head& head, bool want_hidden, bool want_weight, int64_t workspace_bytes) {
@@ -326,7 +327,8 @@ struct Gradients {
     const int64_t pitch = round_up(p.words, 64);
     rows = static_cast<int>(std::min<int64_t>(p.tokens, std::max<int64_t>(256, workspace_bytes / (2 * pitch) / 256 * 256)));
     const auto options = head.hidden.options(), floats = options.dtype(at::kFloat);
-    logits = at::empty({rows, pitch}, options);
+    second = p.tokens <= kFewTokens ? pitch : 0;
+    logits = at::empty({rows, pitch + second}, options);
     if (want_hidden) hidden = at::empty({p.tokens, p.depth}, options);
     if (want_weight) weight = at::empty({p.words, p.depth}, options);
     if (want_weight && rows < p.tokens) sum = at::empty({p.words, round_up(p.depth, 32)}, floats);
@@ -340,7 +342,7 @@ struct Gradients {
   float* alpha() const { return factor.data_ptr<float>(); }
   float* factors() const { return alpha() + 1; }
   LogitRows turn(const Head& head, int first, float2* parts) const {
-    return LogitRows{first, std::min(rows, head.problem.tokens - first), logits.data_ptr(), logits.size(1), parts};
+    return LogitRows{first, std::min(rows, head.problem.tokens - first), logits.data_ptr(), logits.size(1), parts, second};
   }
   int products() const { return (hidden.defined() ? 1 : 0) + (weight.defined() ? 1 : 0); }
 };

@@ -31,6 +31,7 @@
 #include "launch_util.h"
 #include "ptx.cuh"
 #include "tensor_map.h"
+#include "value16.cuh"
 
 namespace soapb200 {
 namespace {
@@ -63,17 +64,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));      // off by 2^-22 at most
   return y;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack16(float low, float high) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(low, high);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
 }
 
 struct Tiles {
@@ -149,16 +139,6 @@ __device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t
   const int rows = min(32, (EPI == kLogitGradient ? min(p.M, (M + kBK - 1) / kBK * kBK) : M) - m_warp);
   const int target = inside ? p.targets[row] - n0 : -1;
   const uint64_t scale = pack_floats(kLog2e, kLog2e);
-  using Stored = std::conditional_t<EPI == kLogitExponential, __half, T>;
-  auto store = [&](auto value) {                          // value(j): the 16-bit result's column j
-#pragma unroll
-    for (int c = 0; c < kLogitPart; c += 32) {
-      uint32_t words[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) words[j] = pack16<Stored>(value(c + 2 * j), value(c + 2 * j + 1));
-      if (rows > 0 && c < cols) store_values<64>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
-    }
-  };
   // sums become the exponents of two that their exponentials are
   auto exponents = [&](float base) {
     const uint64_t shift = pack_floats(-base, -base);
@@ -171,11 +151,29 @@ __device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t
   };
   auto value = [&](int j) { return pair_element(sums[j / 2], j & 1); };
   if constexpr (EPI == kLogitGradient) {
+    const int wide_cols = p.second ? min(kLogitPart, (p.N + kBK - 1) / kBK * kBK - n0) : cols;
     const float factor = inside ? p.factor[row] : 0.f;
     // from the loss itself: the target's probability, less one, is small where the model knows the word
     const float of_target = inside && target >= 0 && target < cols ? expm1f(-p.loss[row]) : 0.f;
     exponents(inside ? p.lse[row] * kLog2e : 0.f);
-    store([&](int j) { return inside ? (target == j ? of_target : exp2_fast(value(j))) * factor : 0.f; });
+    auto gradient = [&](int j) { return inside && j < cols ? (target == j ? of_target : exp2_fast(value(j))) * factor : 0.f; };
+#pragma unroll
+    for (int c = 0; c < kLogitPart; c += 32) {
+      uint32_t words[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) words[j] = pack2<T>(gradient(c + 2 * j), gradient(c + 2 * j + 1));
+      if (rows > 0 && c < wide_cols) {
+        store_values<64>(staging, words, p, m_warp, n0 + c, rows, wide_cols - c, true, lane);
+        if (p.second) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 back = unpack2<T>(words[j]);
+            words[j] = pack2<T>(gradient(c + 2 * j) - back.x, gradient(c + 2 * j + 1) - back.y);
+          }
+          store_values<64>(staging, words, p, m_warp, n0 + c + static_cast<int>(p.second), rows, wide_cols - c, true, lane);
+        }
+      }
+    }
   } else {
     if (cols < kLogitPart) {
 #pragma unroll
@@ -204,7 +202,15 @@ __device__ __forceinline__ void logits_epilogue(const Gemm16Problem& p, uint64_t
     }
     if (inside && cols > 0)
       p.parts[static_cast<int64_t>(n0 / kLogitPart) * p.ld_parts + row] = make_float2(largest, EPI == kLogitExponential ? others * (1.f / 32768.f) : others);
-    if constexpr (EPI == kLogitExponential) store(value);
+    if constexpr (EPI == kLogitExponential) {
+#pragma unroll
+      for (int c = 0; c < kLogitPart; c += 32) {
+        uint32_t words[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) words[j] = pack2<__half>(value(c + 2 * j), value(c + 2 * j + 1));
+        if (rows > 0 && c < cols) store_values<64>(staging, words, p, m_warp, n0 + c, rows, cols - c, true, lane);
+      }
+    }
   }
 }
 
@@ -240,7 +246,7 @@ __device__ __forceinline__ void product_epilogue(const Gemm16Problem& p, int M, 
       if (to16) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          words[16 * h + j] = pack16<T>(alpha * __uint_as_float(raw[2 * j]), alpha * __uint_as_float(raw[2 * j + 1]));
+          words[16 * h + j] = pack2<T>(alpha * __uint_as_float(raw[2 * j]), alpha * __uint_as_float(raw[2 * j + 1]));
       } else if (rows > 0 && at < cols) {
         store_lines<128>(staging, raw, reinterpret_cast<uint8_t*>(p.accumulator + n0 + at), p.ld_accumulator * 4, nullptr, m_warp, rows, 128, 4, true, lane);
       }
@@ -369,7 +375,9 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     if (count == all_tokens) (kLogits ? source_a : source_b) = &map_all;
   }
   const Tiles tiles(M, prob.N);
-  const int k_blocks = (K + kBK - 1) / kBK;
+  // (with two terms every block of K comes twice, the second time with A's remainder; B's tile is in L2 then)
+  const int term_shift = !kLogits && prob.second ? 1 : 0;
+  const int k_blocks = (K + kBK - 1) / kBK << term_shift;
   const Units units(tiles.count(), k_blocks, clusters, !kLogits && prob.split_parts);
 
   if (warp < kFirstEpiWarp) {
@@ -385,17 +393,19 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         uint8_t* stage = smem + s * kStageBytes;
         if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
         const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
+        const int k = (at.kb >> term_shift) * kBK;
+        const int along = at.kb & term_shift ? static_cast<int>(prob.second) : 0;      // in A's rows
         if constexpr (A_K) {
-          tma_load_2d_pair(stage, source_a, bar, at.kb * kBK, at.m0);
+          tma_load_2d_pair(stage, source_a, bar, k + along, at.m0);
         } else {
-          tma_load_2d_pair(stage, source_a, bar, at.m0, at.kb * kBK);
-          tma_load_2d_pair(stage + kOperandBytes / 2, source_a, bar, at.m0 + 64, at.kb * kBK);
+          tma_load_2d_pair(stage, source_a, bar, at.m0 + along, k);
+          tma_load_2d_pair(stage + kOperandBytes / 2, source_a, bar, at.m0 + 64 + along, k);
         }
         if constexpr (B_K) {
-          tma_load_2d_pair(stage + kOperandBytes, source_b, bar, at.kb * kBK, at.n0);
+          tma_load_2d_pair(stage + kOperandBytes, source_b, bar, k, at.n0);
         } else {
-          tma_load_2d_pair(stage + kOperandBytes, source_b, bar, at.n0, at.kb * kBK);
-          tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, source_b, bar, at.n0 + 64, at.kb * kBK);
+          tma_load_2d_pair(stage + kOperandBytes, source_b, bar, at.n0, k);
+          tma_load_2d_pair(stage + kOperandBytes + kOperandBytes / 2, source_b, bar, at.n0 + 64, k);
         }
         if (++s == kStages) {
           s = 0;
@@ -581,7 +591,8 @@ void launch(const Matrix16& a, const Matrix16& b, const Gemm16Problem& p, int* s
   static PerDeviceOnce configured;
   allow_dynamic_smem(reinterpret_cast<const void*>(gemm16_kernel<EPI, A_K, B_K, T>), kSmemBytes, configured, "gemm16");
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  const CUtensorMap map_a = map_of(kBf16, a, p.M, p.K), map_b = map_of(kBf16, b, p.N, p.K);
+  const int64_t more = EPI == kStore16 ? p.second : 0;
+  const CUtensorMap map_a = a.k_major ? map_of(kBf16, a, p.M, p.K + more) : map_of(kBf16, a, p.M + more, p.K), map_b = map_of(kBf16, b, p.N, p.K);
   const CUtensorMap map_all = !hidden ? map_a : EPI != kStore16 ? map_of(kBf16, hidden->all, p.M, p.K) : map_of(kBf16, hidden->all, p.N, p.K);
   const int64_t tiles = static_cast<int64_t>((p.M + kTile - 1) / kTile) * ((p.N + kTile - 1) / kTile);
   if (tiles > (1 << 30)) throw std::invalid_argument("gemm16: too many tiles");
@@ -613,6 +624,8 @@ void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix1
     throw std::invalid_argument("gemm16: operand pitches are multiples of 8 elements");
   if ((epilogue == kLogitGradient || epilogue == kLogitExponential) && (p.ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(p.C) & 15) != 0))
     throw std::invalid_argument("gemm16: the logits' gradient needs 16-byte rows");
+  if (p.second % kBK != 0 || p.second < 0 || (p.second && p.second < (epilogue == kLogitGradient ? p.N : a.k_major ? p.K : p.M)))
+    throw std::invalid_argument("gemm16: the second term lies a multiple of 64 columns behind the first");
   if (epilogue == kStore16 && (p.add || !p.C) && (!p.accumulator || p.ld_accumulator % 32 != 0 || p.ld_accumulator < p.N ||
                                                   (reinterpret_cast<uintptr_t>(p.accumulator) & 15) != 0))
     throw std::invalid_argument("gemm16: the accumulator's pitch is a multiple of 32 covering the columns");

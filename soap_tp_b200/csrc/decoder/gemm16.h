@@ -39,6 +39,9 @@ struct Gemm16Problem {
   // 16-bit result [M][ldc]
   void* C;
   int64_t ldc;
+  // What is left of the gradient's values when they are rounded, in 16 bits `second` columns further on, zeros up to the next multiple of 64
+  // words in both; as A (kStore16) both terms are multiplied by B.  0: there is none.
+  int64_t second;
   // kStore16: alpha * (product + accumulator), row i of it in row where[i] of C; without `C` the sum goes back into the accumulator
   const int* where;         // null: rows stay where they are
   const float* alpha;       // on the device; null: 1

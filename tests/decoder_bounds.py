@@ -15,14 +15,15 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def head_exact(hidden, weight, targets, reduction, grad_loss=None, ignore_index=IGNORED):
+def head_exact(hidden, weight, targets, reduction, grad_loss=None, ignore_index=IGNORED, tokens=None):
     """Loss, gradients and bounds of a cross entropy of ``hidden @ weight.T``.
 
     A logit is a sum of products that the tensor core adds with truncation, 2^-23 of the sum of magnitudes for each of the K / 16 additions at most:
     ``e`` bounds it.  exp, log and the joining of partial sums err by 2^-20 of one more.  The logits' gradient d has 16 bits (fp16: 2^-25 of
     its largest possible value, times 2^-15, below its normal numbers); its products add up with K / 16 truncated additions again.
     bf16 gradients of a reduced loss are made from exponentials that were rounded to fp16 once (2^-11; the target's entry was not), and an
-    upstream gradient that is not a power of two rounds the results once more.
+    upstream gradient that is not a power of two rounds the results once more.  Of 256 tokens or fewer (in the whole call, ``tokens``)
+    d has two terms, so that u^2 of it is lost.
     """
     dtype = hidden.dtype
     u = half_step(dtype)
@@ -47,7 +48,7 @@ def head_exact(hidden, weight, targets, reduction, grad_loss=None, ignore_index=
     # a probability errs by its logit's and its lse's error, its rounding by u of what is stored
     # (and below 2^-126, the smallest normal fp32 number, it is taken as zero: exp(x) < 2^-126 errs by itself, at most 2^-126)
     with_loss = dtype == torch.bfloat16 and reduction != "none"
-    e_d = (p * (2 * e.unsqueeze(1) + 2.0 ** -19 + (2.0 ** -11 if with_loss else 0.0)) + (u + 4 * F32) * d.abs() + 2.0 ** -126) * factor.abs()
+    e_d = (p * (2 * e.unsqueeze(1) + 2.0 ** -19 + (2.0 ** -11 if with_loss else 0.0)) + ((u * u if (tokens or len(targets)) <= 256 else u) + 4 * F32) * d.abs() + 2.0 ** -126) * factor.abs()
     if dtype == torch.float16:
         e_d = e_d + 2.0 ** -39 * factor.abs().max()
     if with_loss:      # exponentials are kept as fp16 times 2^15, whose subnormal step is 2^-24: half of one is 2^-40 of the largest of 64 words

@@ -297,7 +297,7 @@ def test_cross_entropy_beyond_32_bits():
     up = torch.zeros(tokens, device="cuda")
     up[-50:] = 1.0
     grads = torch.autograd.grad(loss, (hidden, weight), up)
-    exact = head_exact(hidden.detach()[-50:], weight, targets[-50:], "sum")
+    exact = head_exact(hidden.detach()[-50:], weight, targets[-50:], "sum", tokens=tokens)
     within(loss[-50:].sum(), (exact[0][0], exact[0][1] + 64 * F32 * exact[0][0]))
     within(grads[0][-50:], exact[1])
     assert not grads[0][:-50].any()
