@@ -10,8 +10,10 @@
 // read the logits' gradient in both directions, and no matrix is transposed.
 //
 // What bounds it: a pair's tile takes 64 KB of L2's bandwidth every 512 cycles of products, 64 bytes a cycle and SM, which is all that an SM gets; and
-// the power cap in long runs.  8192 x 4096 x 128256 alone 1.31 PFLOP/s (torch.matmul 1.55), for seconds 1.17 to 1.23 (1.38).  Fetching tiles into L2
-// ahead of their loads only adds to that (4096 x 4096 x 16032: 416 -> 493 us).
+// the power cap in long runs.  8192 x 4096 x 128256 alone 1.31 PFLOP/s (torch.matmul 1.55), for seconds 1.21 to 1.24 (1.29 to 1.37).  At 4096 x 4096
+// x 16032 the tensor pipe is busy for 80 (exponentials), 85 and 83 % of a launch, of 97 % that its rounds of tiles allow.  Tried and not kept:
+// tiles fetched into L2 ahead of their loads (416 -> 493 us), a producer thread for each operand (566 -> 574 thousand cycles), waits of the
+// producer that suspend it (541 -> 583 thousand; those of the epilogue, which are long, do).
 //
 // The tensor core truncates as it adds: some 2^-24 of the running sum per 16 of K.  Logits are drained from TMEM into sums in registers (round
 // to nearest) every 2048 of K, gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
@@ -389,7 +391,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
       bool first_round = true;
       Cursor at(units, tiles, cta, cluster, clusters);
       for (; !at.done(); at.advance()) {
-        if (!first_round && !mbar_wait_parked(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) break;
+        if (!first_round && !mbar_wait_bounded(&empty_bar[s], parity, abort_flag, status, kStatusSlotWaitTimeout)) break;
         uint8_t* stage = smem + s * kStageBytes;
         if (cta == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
         const uint32_t bar = map_to_cta(smem_u32(&full_bar[s]), 0);
@@ -434,7 +436,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         units.place(u, tile, begin, end, part);
         for (int kb = begin; kb < end && ok; ++it) {
           const int buf = it & 1;
-          if (it >= 2 && !drained && !mbar_wait_parked(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
+          if (it >= 2 && !drained && !mbar_wait_bounded(&acc_empty[buf], ((it >> 1) - 1) & 1, abort_flag, status, kStatusAccumWaitTimeout)) {
             ok = false;
             break;
           }
@@ -442,7 +444,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
           const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
           const int blocks = drain_blocks<kLogits>(end - kb);
           for (int i = 0; i < blocks; ++i, ++kb) {
-            if (!loaded && !mbar_wait_parked(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
+            if (!loaded && !mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
               ok = false;
               break;
             }
