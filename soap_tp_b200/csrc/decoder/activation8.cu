@@ -10,7 +10,7 @@
 //
 // Memory bounds all four, once instructions do not: eight threads take a group, eight values each (16-byte loads and stores of 16-bit types,
 // 8-byte ones of the kept values), and the group's maximum goes round with three shuffles.  Magnitudes of 16-bit values are compared two at a
-// time as they lie; a value becomes its whole number by one multiply-add that leaves it in the low byte of 1.5 * 2^23 + q, and comes back
+// time as they lie; a value becomes its whole number by a multiply-add and an addition that leave it in the low byte of 1.5 * 2^23 + q, and comes back
 // as the low byte of 2^23 + q + 128.  (Conversion instructions, at a quarter of the rate, and a division for each address made 19
 // instructions a value and bounded packing at 32768 x 4096: 112 us where its bytes take 63.)
 #include <cuda_runtime.h>
@@ -96,10 +96,10 @@ __device__ __forceinline__ void store8(T* p, const Place& place, const float (&v
   }
 }
 
-// The scale of a group whose eight threads hold its values; all 32 lanes call.  Magnitudes are compared as whole numbers: infinities and NaN
+// The largest magnitude of a group whose eight threads hold its values, as bits of fp32; all 32 lanes call.  Magnitudes are compared as whole numbers: infinities and NaN
 // come out above all others.
 template <typename T>
-__device__ __forceinline__ float group_scale(const Eight<T>& e) {
+__device__ __forceinline__ uint32_t group_most(const Eight<T>& e) {
   uint32_t most;
   if constexpr (sizeof(T) == 4) {
     const uint32_t w[8] = {e.words[0].x, e.words[0].y, e.words[0].z, e.words[0].w, e.words[1].x, e.words[1].y, e.words[1].z, e.words[1].w};
@@ -117,21 +117,31 @@ __device__ __forceinline__ float group_scale(const Eight<T>& e) {
     if constexpr (std::is_same<T, __half>::value) most = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(most))));
     else most <<= 16;
   }
+  return most;
+}
+__device__ __forceinline__ float scale_of(uint32_t most) {
   return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(most) / 127.f, kSmallestScale);
 }
 
-// 16-bit values are multiplied by the reciprocal, whose rounding can move what lies within 2^-15 of a step from a tie to the other side;
-// fp32 values, which come back exactly but for their step, are divided.
+// 127 x / max of 16-bit values is often a tie, which a rounded reciprocal would move to either side (2e-4 of fp16 values, 1e-3 of bf16 ones).  So
+// x (127 / max) is first rounded to multiples of 2^-15, by adding it to 384: it is off by 127 2^-24 at most, less than half of 2^-15, and every tie is
+// such a multiple.  What is not a tie but within 2^-16 + 127 2^-24 of one may become it (1e-6 of fp16 values).
+// At 32768 x 4096, there and back, it costs 3 to 6 us of 142 to 145.  fp32 values are divided by their scale.
 template <typename T>
-__device__ __forceinline__ uint2 quantise(const Eight<T>& e, float scale) {
+__device__ __forceinline__ uint2 quantise(const Eight<T>& e, uint32_t most, float scale) {
   constexpr float kShift = 12582912.f;       // 1.5 * 2^23: its neighbours are whole numbers, in two's complement in the low byte
+  constexpr float kGrid = 384.f;             // sums with -127 to 127 lie between 2^8 and 2^9
   float v[8];
   e.get(v);
   uint32_t bits[8];
-  const float inverse = __fdividef(1.f, scale);
+  if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    bits[i] = __float_as_uint(std::is_same<T, float>::value ? v[i] / scale + kShift : fmaf(v[i], inverse, kShift));
+    for (int i = 0; i < 8; ++i) bits[i] = __float_as_uint(v[i] / scale + kShift);
+  } else {
+    const float steps = 127.f / fmaxf(__uint_as_float(most), 127.f * kSmallestScale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits[i] = __float_as_uint(fmaf(v[i], steps, kGrid) + (kShift - kGrid));
+  }
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -149,8 +159,9 @@ __device__ __forceinline__ void dequantise(uint2 q, float scale, float (&v)[8]) 
 // All 32 lanes call.
 template <typename T>
 __device__ __forceinline__ void keep(const Kept8& kept, const Shape& shape, const Place& p, const Eight<T>& e) {
-  const float scale = group_scale(e);
-  if (p.valid > 0) *reinterpret_cast<uint2*>(kept.values + p.row * kept.pitch + p.column) = quantise(e, scale);
+  const uint32_t most = group_most(e);
+  const float scale = scale_of(most);
+  if (p.valid > 0) *reinterpret_cast<uint2*>(kept.values + p.row * kept.pitch + p.column) = quantise(e, most, scale);
   if (threadIdx.x % kGroupThreads == 0 && p.group < shape.count) kept.scales[p.group] = scale;
 }
 
@@ -176,7 +187,7 @@ template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t ld, Shape shape, Kept8 kept) {
   wait_for_predecessor();
   let_successor_start();
-  // (two loads under way in a thread: 32768 x 4096 values there and back in 129 us, one 154, four 132)
+  // (two loads under way in a thread: 32768 x 4096 values there and back in 129 us, one 154, four 132, before ties were rounded as ties)
   Eight<T> e[kTurns];
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {

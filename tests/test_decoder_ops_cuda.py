@@ -412,10 +412,28 @@ def test_pack8(rows, dim, dtype):
     scales = padded.abs().amax(-1) / 127
     assert bool(((packed.scales.double() - scales).abs() <= F32 * scales).all())           # one rounding
     step = packed.scales.double().repeat_interleave(64, dim=1)[:, :dim]
-    # the quotient has three roundings (of 127 at most): half a step and 127 * 3 * 2^-24 more
-    assert bool(((packed.values[:, :dim].double() * step - x.double()).abs() <= step * (0.5 + 400 * F32)).all())
+    # a quotient is moved onto a tie from up to 2^-16 + 127 * 2^-24 away (2^-16 = 256 * 2^-24), and the kept scale is rounded, 127 * 2^-24
+    # more: half a step and (256 + 127 + 127) * 2^-24; fp32's three roundings make 127 * 3 * 2^-24
+    assert bool(((packed.values[:, :dim].double() * step - x.double()).abs() <= step * (0.5 + 511 * F32)).all())
     exact = packed.values[:, :dim].double() * step
     within(unpack8(packed), (exact, (half_step(dtype) + F32) * exact.abs() + smallest(dtype)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_pack8_rounds_ties_to_even(dtype):
+    """127 x / max in 64 bits (127 x is exact): what is a tie is rounded as one, and no other value leaves the definition unless it is near one."""
+    from soap_tp_b200.ops import pack8
+
+    x = _rand(4000, 64, dtype=dtype, scale=3.0)
+    x[0, :] = x[0].abs().amax() / 2                                  # max / 2: the tie 63.5, of both signs
+    x[0, :20] *= -1
+    x[0, 0] = 2 * x[0, 1]
+    quotient = 127 * x.double() / x.double().abs().amax(dim=1, keepdim=True)
+    wanted, kept = quotient.round(), pack8(x).values.double()
+    off = ((quotient - quotient.floor()) - 0.5).abs()                # distance from a tie
+    assert int((off == 0).sum()) > 100
+    assert torch.equal(kept[off == 0], wanted[off == 0])
+    assert bool((off[kept != wanted] <= 2.0 ** -16 + 127 * F32).all())
 
 
 def test_pack8_of_strided_rows_and_special_values():
