@@ -12,8 +12,9 @@
 // less, of which a difference of lse and t in fp32 would leave two digits.  D goes through memory in 16 bits for a bounded number of tokens at a time, then
 // two products read it in both directions.  It comes about in one of two ways:
 //   * bf16 and one gradient of the loss for all tokens (mean, sum): the first product leaves the exponentials as well (in fp16 times 2^15, which
-//     rounds them an eighth as much as D is rounded then, or to 2^-40 of the largest of their 64 words), one pass over them makes D of them once lse is known, and the gradients come with the loss, 6 N V K operations for N tokens.  The pass
-//     moves 4 N V bytes: 0.7 of 21 ms at 8192 x 4096 x 128256, where the product that it replaces takes 5.
+//     rounds them an eighth as much as D is rounded then, or to 2^-40 of the largest of their 64 words), one pass over them makes D of them
+//     once lse is known, and the gradients come with the loss, 6 N V K operations for N tokens.  The pass moves 4 N V bytes: 44 us at
+//     4096 x 4096 x 16032, where the product that it replaces takes 354.
 //   * fp16, whose gradients want the loss's scale before they are rounded, a gradient for each token, or a second backward pass: the logits
 //     are computed again once these are known, 8 N V K operations.
 //

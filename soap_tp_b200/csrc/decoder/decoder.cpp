@@ -1,8 +1,8 @@
 // The operators of a decoder's training step as torch operators with gradients (module soap_tp_b200._decoder).
 //
 // The launches of an optimizer step are issued from Python with raw pointers (bindings.cpp); a model calls these operators some hundred times a
-// step, forward and backward, and autograd functions written in Python cost 60 to 120 us of host time a call there, several times
-// what the kernels of ordinary layers take.  So their autograd nodes are native: they allocate what they return and their scratch with
+// step, forward and backward, and autograd functions written in Python cost 25 to 130 us more of host time for a forward and a
+// backward pass (packing 44 -> 19 us, cross entropy 223 -> 134, a gated activation 172 -> 80, a norm 229 -> 100), as much as an ordinary layer's kernels.  So their autograd nodes are native: they allocate what they return and their scratch with
 // torch's allocator on the current stream, and launch.
 //
 // Arguments are checked in Python (soap_tp_b200/ops); what a kernel relies on is checked again where it is launched.
