@@ -100,6 +100,9 @@ class _Checkpoint8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, function, count, x, *rest):
         ctx.function, ctx.count = function, count
+        kind = x.device.type
+        ctx.autocast = dict(device_type=kind, dtype=torch.get_autocast_dtype(kind), enabled=torch.is_autocast_enabled(kind),
+                            cache_enabled=torch.is_autocast_cache_enabled())
         ctx.shape, ctx.dtype = x.shape, x.dtype
         packed = pack8(x)
         ctx.tensors = [isinstance(a, Tensor) for a in rest]
@@ -119,7 +122,7 @@ class _Checkpoint8(torch.autograd.Function):
         arguments = [a.detach().requires_grad_(n) if isinstance(a, Tensor) else a
                      for a, n in zip(rest[: ctx.count], ctx.needs_input_grad[3:])]
         wanted = [a for a, n in zip([x, *arguments, *rest[ctx.count:]], ctx.needs_input_grad[2:]) if n]
-        with torch.enable_grad():
+        with torch.enable_grad(), torch.autocast(**ctx.autocast):
             outputs = ctx.function(x, *arguments)
         outputs = (outputs,) if isinstance(outputs, Tensor) else tuple(outputs)
         pairs = [(o, g) for o, g in zip(outputs, grads) if isinstance(o, Tensor) and o.requires_grad and g is not None]
@@ -133,7 +136,7 @@ def checkpoint8(function: Callable, x: Tensor, *args, parameters: Iterable[Tenso
     the backward pass.
 
     ``function`` takes tensors or anything else, returns a tensor or a tuple of tensors, and does the same on every call (it must not
-    draw random numbers).  Gradients reach ``x``, tensor ``args`` and ``parameters``: by default those of ``function`` where it is a module.
+    draw random numbers); autocast is as it was in the first run.  Gradients reach ``x``, tensor ``args`` and ``parameters``: by default those of ``function`` where it is a module.
     Without gradients it is a plain call.
     """
     _check_values("x", x)

@@ -197,3 +197,29 @@ def test_checkpoint8_runs_again_from_the_kept_input():
         assert not ops.checkpoint8(block, x, shift, 2.0)[0].requires_grad
     with pytest.raises(TypeError):
         ops.checkpoint8(block, torch.zeros(3, dtype=torch.int64))
+
+
+# ---- under autocast -----------------------------------------------------------------------------------------------------
+def test_checkpoint8_runs_again_under_the_autocast_of_the_first_run():
+    torch.manual_seed(4)
+    layer, x = torch.nn.Linear(70, 40), torch.randn(12, 70)
+    direction = torch.randn(12, 40).bfloat16()
+    kept = ops.unpack8(ops.pack8(x)).requires_grad_()
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        wanted = torch.autograd.grad(layer(kept), [kept, *layer.parameters()], direction)
+        y = ops.checkpoint8(layer, x.requires_grad_())
+        expected = layer(x)
+    assert y.dtype == torch.bfloat16 and torch.equal(y, expected)
+    for a, b in zip(torch.autograd.grad(y, [x, *layer.parameters()], direction), wanted):
+        assert torch.equal(a, b)
+
+
+def test_checkpoint8_runs_again_without_the_autocast_around_the_backward_pass():
+    torch.manual_seed(4)
+    layer, x = torch.nn.Linear(70, 40), torch.randn(12, 70, requires_grad=True)
+    plain = torch.autograd.grad(ops.checkpoint8(layer, x).sum(), [x, *layer.parameters()])
+    loss = ops.checkpoint8(layer, x).sum()
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        inside = torch.autograd.grad(loss, [x, *layer.parameters()])
+    for a, b in zip(inside, plain):
+        assert torch.equal(a, b)
