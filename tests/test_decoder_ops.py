@@ -214,12 +214,17 @@ def test_checkpoint8_runs_again_under_the_autocast_of_the_first_run():
         assert torch.equal(a, b)
 
 
-def test_checkpoint8_runs_again_without_the_autocast_around_the_backward_pass():
+def test_checkpoint8_under_autocast_around_the_backward_pass_alone():
+    """What the plain block gives at the kept input.  (Not what it gives without autocast: torch's own products of a backward pass are rounded by
+    the autocast around it, those of the plain block as well.)"""
     torch.manual_seed(4)
     layer, x = torch.nn.Linear(70, 40), torch.randn(12, 70, requires_grad=True)
-    plain = torch.autograd.grad(ops.checkpoint8(layer, x).sum(), [x, *layer.parameters()])
-    loss = ops.checkpoint8(layer, x).sum()
-    with torch.autocast("cpu", dtype=torch.bfloat16):
-        inside = torch.autograd.grad(loss, [x, *layer.parameters()])
-    for a, b in zip(inside, plain):
-        assert torch.equal(a, b)
+    deep = torch.nn.Sequential(layer, torch.nn.Tanh(), torch.nn.Linear(40, 30))     # where the second run's own roundings would show
+    for block in (layer, deep):
+        kept = ops.unpack8(ops.pack8(x)).requires_grad_()
+        plain, loss = block(kept).sum(), ops.checkpoint8(block, x).sum()
+        with torch.autocast("cpu", dtype=torch.bfloat16):
+            wanted = torch.autograd.grad(plain, [kept, *block.parameters()])
+            inside = torch.autograd.grad(loss, [x, *block.parameters()])
+        for a, b in zip(inside, wanted):
+            assert torch.equal(a, b)
