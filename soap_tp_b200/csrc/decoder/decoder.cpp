@@ -88,6 +88,11 @@ double double_of(int64_t bits) {
   return value;
 }
 
+// The linear layer's products are in the type of their operands, forward and backward, whatever autocast says around the one or the other.
+struct NoAutocast {
+  c10::impl::ExcludeDispatchKeyGuard guard{c10::autocast_dispatch_keyset};
+};
+
 Tensor given(const std::optional<Tensor>& x) { return x ? *x : Tensor(); }
 
 // ---- norms --------------------------------------------------------------------------------------------------------------
@@ -253,6 +258,7 @@ struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
     auto out = swiglu_forward(gate, up, true);
     ctx->save_for_backward({out[1], out[2], out[3], out[4], weight});
     ctx->saved_data["want_weight"] = want_weight;
+    const NoAutocast own_type;
     return at::linear(out[0], weight);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -263,6 +269,7 @@ struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
     const bool graph = at::GradMode::is_enabled();
     {
       const at::NoGradGuard no_grad;
+      const NoAutocast own_type;
       const Tensor grad = grads[0].reshape({-1, grads[0].size(-1)});
       auto out = swiglu_backward(at::matmul(grads[0], saved[4]), saved.data(), want_weight);
       result[0] = out[0];
@@ -494,6 +501,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (wanted(gate) || wanted(up) || wanted(weight)) return SwiGLULinear8::apply(gate, up, weight, wanted(weight));
     const c10::cuda::CUDAGuard guard(gate.device());
     const at::NoGradGuard no_grad;
+    const NoAutocast own_type;
     return at::linear(swiglu_forward(gate, up, false)[0], weight);
   });
   m.def("linear_cross_entropy", [](const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t reduction, int64_t ignore_index,

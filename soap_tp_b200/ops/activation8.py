@@ -173,14 +173,16 @@ class _SwiGLU8(torch.autograd.Function):
     def forward(ctx, gate, up, weight):
         ctx.save_for_backward(weight, *_host_pack(gate), *_host_pack(up))
         y = _host_swiglu(gate, up)
-        return y if weight is None else F.linear(y, weight)
+        with torch.autocast("cpu", enabled=False):
+            return y if weight is None else F.linear(y, weight)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         weight, *kept = ctx.saved_tensors
-        d_gate, d_up, y = _host_swiglu_gradients(grad if weight is None else grad @ weight, kept)
-        return d_gate, d_up, grad.t() @ y if ctx.needs_input_grad[2] else None
+        with torch.autocast("cpu", enabled=False):
+            d_gate, d_up, y = _host_swiglu_gradients(grad if weight is None else grad @ weight, kept)
+            return d_gate, d_up, grad.t() @ y if ctx.needs_input_grad[2] else None
 
 
 def swiglu8(gate: Tensor, up: Tensor) -> Tensor:
@@ -193,7 +195,8 @@ def swiglu8(gate: Tensor, up: Tensor) -> Tensor:
 
 
 def swiglu_linear8(gate: Tensor, up: Tensor, weight: Tensor) -> Tensor:
-    """``(silu(gate) * up) @ weight.T``; only gate and up are kept, in 8 bits: 2 bytes and a bit of each pair of features instead of 6."""
+    """``(silu(gate) * up) @ weight.T``; only gate and up are kept, in 8 bits: 2 bytes and a bit of each pair of features instead of 6.
+    In the type of its arguments, under autocast too."""
     _check_swiglu(gate, up)
     if weight.ndim != 2 or weight.shape[1] != gate.shape[-1] or weight.dtype != gate.dtype or weight.device != gate.device:
         raise ValueError(f"weight must be (out, {gate.shape[-1]}) {gate.dtype} on {gate.device}, got {tuple(weight.shape)} {weight.dtype} on {weight.device}.")

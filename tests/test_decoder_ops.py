@@ -228,3 +228,15 @@ def test_checkpoint8_under_autocast_around_the_backward_pass_alone():
             inside = torch.autograd.grad(loss, [x, *block.parameters()])
         for a, b in zip(inside, wanted):
             assert torch.equal(a, b)
+
+
+def test_swiglu_linear8_keeps_its_type_under_autocast():
+    torch.manual_seed(5)
+    gate, up, weight = (torch.randn(*shape, requires_grad=True) for shape in ((9, 70), (9, 70), (33, 70)))
+    plain = ops.swiglu_linear8(gate, up, weight)
+    wanted = torch.autograd.grad(plain.sum(), (gate, up, weight))
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = ops.swiglu_linear8(gate, up, weight)
+        gradients = torch.autograd.grad(y.sum(), (gate, up, weight))
+    for a, b in zip((y, *gradients), (plain, *wanted)):
+        assert a.dtype == torch.float32 and torch.equal(a, b)

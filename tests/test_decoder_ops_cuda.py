@@ -594,3 +594,27 @@ def test_results_are_the_same_on_every_stream_and_run():
     for result in results:
         for a, b in zip(result, expected):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_operators_under_autocast(dtype):
+    """swiglu_linear8 and checkpoint8 are what they are without it, or with it around both runs."""
+    from soap_tp_b200.ops import checkpoint8, pack8, swiglu_linear8, unpack8
+
+    gate, up, weight = (_rand(*shape, dtype=dtype).requires_grad_() for shape in ((40, 136), (40, 136), (72, 136)))
+    direction = _rand(40, 72, dtype=dtype)
+    plain = swiglu_linear8(gate, up, weight)
+    wanted = torch.autograd.grad(plain, (gate, up, weight), direction)
+    with torch.autocast("cuda", dtype=FP16):
+        y = swiglu_linear8(gate, up, weight)
+    for a, b in zip((y, *torch.autograd.grad(y, (gate, up, weight), direction)), (plain, *wanted)):
+        assert a.dtype == dtype and torch.equal(a, b)
+    with torch.no_grad(), torch.autocast("cuda", dtype=FP16):
+        assert torch.equal(swiglu_linear8(gate, up, weight), plain)
+
+    kept, direction = unpack8(pack8(gate)).requires_grad_(), direction.half()
+    with torch.autocast("cuda", dtype=FP16):
+        wanted = torch.autograd.grad(torch.nn.functional.linear(kept, weight), (kept, weight), direction)
+        y = checkpoint8(lambda x, w: torch.nn.functional.linear(x, w), gate, weight)
+    for a, b in zip(torch.autograd.grad(y, (gate, weight), direction), wanted):
+        assert y.dtype == FP16 and torch.equal(a, b)
