@@ -128,10 +128,22 @@ class _HostHead:
         return d @ self.weight, d.t() @ self.hidden
 
 
+def _without_autocast(function):
+    """The loss is computed in 32 bits at least, whatever autocast is around either pass."""
+
+    @functools.wraps(function)
+    def call(*args):
+        with torch.autocast("cpu", enabled=False):
+            return function(*args)
+
+    return call
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     """CPU tensors."""
 
     @staticmethod
+    @_without_autocast
     def forward(ctx, hidden, weight, targets, reduction, ignore_index, group):
         words, world = weight.shape[0], _world(group)
         first_word = 0 if group is None else dist.get_rank(group) * words
@@ -151,6 +163,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     @once_differentiable
+    @_without_autocast
     def backward(ctx, grad_loss):
         hidden, weight, targets, lse, counted = ctx.saved_tensors
         head = _HostHead(hidden, weight, targets, *ctx.arguments)

@@ -240,3 +240,16 @@ def test_swiglu_linear8_keeps_its_type_under_autocast():
         gradients = torch.autograd.grad(y.sum(), (gate, up, weight))
     for a, b in zip((y, *gradients), (plain, *wanted)):
         assert a.dtype == torch.float32 and torch.equal(a, b)
+
+
+def test_cross_entropy_keeps_its_accuracy_under_autocast():
+    torch.manual_seed(6)
+    hidden, weight = torch.randn(9, 70, requires_grad=True), torch.randn(50, 70, requires_grad=True)
+    targets = torch.randint(0, 50, (9,))
+    plain = ops.linear_cross_entropy(hidden, weight, targets)
+    wanted = torch.autograd.grad(plain, (hidden, weight))
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        loss = ops.linear_cross_entropy(hidden, weight, targets)
+        gradients = torch.autograd.grad(loss, (hidden, weight))
+    for a, b in zip((loss, *gradients), (plain, *wanted)):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
