@@ -514,6 +514,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // A plain product, C[m, n] = sum_k A(m, k) B(n, k): `a` is (m, k) or with `turned` (k, m), `b` (k, n), both with 16-byte rows.
   m.def("gemm16", [](const Tensor& a, const Tensor& b, const Tensor& out, bool turned, int64_t status, const std::optional<Tensor>& split_parts,
                      const std::optional<Tensor>& split_counters) {
+    for (const Tensor* t : {&a, &b, &out}) {
+      TORCH_CHECK_VALUE(t->dim() == 2 && t->numel() > 0 && t->stride(1) == 1 && t->stride(0) >= t->size(1), "gemm16 takes matrices whose rows lie in memory one by one.");
+      TORCH_CHECK_TYPE(t->scalar_type() == a.scalar_type() && (a.scalar_type() == at::kBFloat16 || a.scalar_type() == at::kHalf),
+                       "gemm16 takes bfloat16 or float16, all of one type.");
+    }
+    TORCH_CHECK_VALUE(a.size(turned ? 0 : 1) == b.size(0) && out.size(0) >= a.size(turned ? 1 : 0) && out.size(1) >= b.size(1),
+                      "gemm16: sizes do not match, or the result has no room: ", a.sizes(), ", ", b.sizes(), " and ", out.sizes(), ".");
+    TORCH_CHECK_VALUE(split_parts.has_value() == split_counters.has_value(), "gemm16: split_parts and split_counters go together.");
+    if (split_parts) {
+      TORCH_CHECK_TYPE(split_parts->scalar_type() == at::kFloat && split_counters->scalar_type() == at::kInt, "gemm16: split_parts are float32, split_counters int32.");
+      TORCH_CHECK_VALUE(split_parts->is_contiguous() && split_parts->numel() >= kSplitScratch && split_counters->is_contiguous() &&
+                        split_counters->numel() >= kSplitCounters, "gemm16: split_parts or split_counters are too small.");
+      TORCH_CHECK_VALUE(split_parts->device() == a.device() && split_counters->device() == a.device(), "gemm16: scratch is on another device.");
+    }
+    TORCH_CHECK_VALUE(a.is_cuda() && b.device() == a.device() && out.device() == a.device(), "gemm16 takes tensors of one CUDA device.");
     const c10::cuda::CUDAGuard guard(a.device());
     Gemm16Problem p{};
     p.M = size_as_int(turned ? a.size(1) : a.size(0), "m");

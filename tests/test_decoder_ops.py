@@ -253,3 +253,31 @@ def test_cross_entropy_keeps_its_accuracy_under_autocast():
         gradients = torch.autograd.grad(loss, (hidden, weight))
     for a, b in zip((loss, *gradients), (plain, *wanted)):
         assert a.dtype == torch.float32 and torch.equal(a, b)
+
+
+# ---- the plain product of the native library ----------------------------------------------------------------------------
+def _product(**change):
+    from soap_tp_b200 import _decoder
+
+    bf16 = torch.bfloat16
+    given = dict(a=torch.zeros(16, 24, dtype=bf16), b=torch.zeros(24, 32, dtype=bf16), out=torch.zeros(16, 32, dtype=bf16), turned=False, status=0)
+    given.update(change)
+    return _decoder.gemm16(**given)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(), ValueError),                                                              # not on CUDA
+    (dict(out=torch.zeros(16, 24, dtype=torch.bfloat16)), ValueError),
+    (dict(out=torch.zeros(8, 32, dtype=torch.bfloat16)), ValueError),
+    (dict(b=torch.zeros(16, 32, dtype=torch.bfloat16)), ValueError),
+    (dict(turned=True), ValueError),
+    (dict(out=torch.zeros(32, 16, dtype=torch.bfloat16).t()), ValueError),
+    (dict(a=torch.zeros(24, dtype=torch.bfloat16)), ValueError),
+    (dict(out=torch.zeros(16, 32)), TypeError),
+    (dict(b=torch.zeros(24, 32, dtype=torch.float16)), TypeError),
+    (dict(split_parts=torch.zeros(4)), ValueError),
+    (dict(split_parts=torch.zeros(4), split_counters=torch.zeros(4, dtype=torch.int32)), ValueError),
+])
+def test_native_product_refusals(change, error):
+    with pytest.raises(error):
+        _product(**change)
