@@ -349,6 +349,11 @@ scale_gradients_kernel(const float* __restrict__ factor, __nv_bfloat16* __restri
   }
 }
 
+// Up to so many tokens logits are drained every 256 of K, where one token's truncated logits are the whole loss: of 400 drawn cases six, of one to six
+// tokens, had a loss 1.0e-6 to 2.8e-6 off; the largest error of 800 is 1.2e-6 now.  At 4096 x 128256 the loss of one token takes 290 us for 279; of
+// 256 tokens, where none was as far off, it would be 275 for 236.
+constexpr int kExactTokens = 64;
+
 Hidden16 hidden_of(const HeadProblem& p, int first) {
   const int64_t at = static_cast<int64_t>(first);
   return Hidden16{Matrix16{static_cast<const uint16_t*>(p.packed.data) + at * p.packed.ld, p.packed.ld, true},
@@ -359,6 +364,7 @@ Gemm16Problem logits_of(const HeadProblem& p, const LogitRows& r) {
   if (r.rows < 1 || r.first < 0 || r.first + r.rows > p.tokens) throw std::invalid_argument("cross entropy: rows outside the tokens");
   Gemm16Problem g{};
   g.M = r.rows; g.N = p.words; g.K = p.depth;
+  g.drain = p.tokens <= kExactTokens ? 256 : 2048;
   g.count = p.count; g.first = r.first;
   g.targets = p.column + r.first;
   g.parts = r.parts; g.ld_parts = r.rows;

@@ -16,7 +16,7 @@
 // producer that suspend it (541 -> 583 thousand; those of the epilogue, which are long, do).
 //
 // The tensor core truncates as it adds: some 2^-24 of the running sum per 16 of K.  Logits are drained from TMEM into sums in registers (round
-// to nearest) every 2048 of K, gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
+// to nearest) every 2048 of K (`drain`; every 256 for a few tokens), gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
 // Draining every 256 of K costs 150 of 690 thousand cycles at 4096 x 16032 x 4096: handing the accumulator over takes the tensor core about
 // 700 cycles, whatever the epilogue does meanwhile.
 #include <cuda.h>
@@ -287,12 +287,11 @@ struct Units {
   static constexpr int kMostSplit = 16;
 };
 
-// K-blocks that the accumulator takes before it is drained, `left` of them remaining.
-constexpr int kDrainBlocks = 2048 / kBK;
+// K-blocks that the accumulator takes before it is drained (after `most` at the latest), `left` of them remaining.
 template <bool LOGITS>
-__device__ __forceinline__ int drain_blocks(int left) {
-  if (!LOGITS || left <= kDrainBlocks) return left;
-  const int drains = (left + kDrainBlocks - 1) / kDrainBlocks;      // of about the same size
+__device__ __forceinline__ int drain_blocks(int left, int most) {
+  if (!LOGITS || left <= most) return left;
+  const int drains = (left + most - 1) / most;      // of about the same size
   return (left + drains - 1) / drains;
 }
 
@@ -442,7 +441,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
           }
           tc_fence_after_sync();
           const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
-          const int blocks = drain_blocks<kLogits>(end - kb);
+          const int blocks = drain_blocks<kLogits>(end - kb, prob.drain / kBK);
           for (int i = 0; i < blocks; ++i, ++kb) {
             if (!loaded && !mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
               ok = false;
@@ -503,7 +502,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int j = 0; j < kLogitPart / 2; ++j) sums[j] = 0;
         bool ok = true;
         for (int kb = 0; kb < k_blocks;) {
-          kb += drain_blocks<true>(k_blocks - kb);
+          kb += drain_blocks<true>(k_blocks - kb, prob.drain / kBK);
           ok = filled();
           if (!ok) break;
           const uint32_t from = taddr + static_cast<uint32_t>((it & 1) * kTile);
@@ -626,6 +625,7 @@ void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix1
     throw std::invalid_argument("gemm16: operand pitches are multiples of 8 elements");
   if ((epilogue == kLogitGradient || epilogue == kLogitExponential) && (p.ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(p.C) & 15) != 0))
     throw std::invalid_argument("gemm16: the logits' gradient needs 16-byte rows");
+  if (epilogue != kStore16 && (p.drain < kBK || p.drain % kBK != 0)) throw std::invalid_argument("gemm16: logits are drained every multiple of 64 of K");
   if (p.second % kBK != 0 || p.second < 0 || (p.second && p.second < (epilogue == kLogitGradient ? p.N : a.k_major ? p.K : p.M)))
     throw std::invalid_argument("gemm16: the second term lies a multiple of 64 columns behind the first");
   if (epilogue == kStore16 && (p.add || !p.C) && (!p.accumulator || p.ld_accumulator % 32 != 0 || p.ld_accumulator < p.N ||
