@@ -474,6 +474,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 
 // ---- entry points -----------------------------------------------------------------------------------------------------------
 bool wanted(const Tensor& x) { return x.defined() && at::GradMode::is_enabled() && x.requires_grad(); }
+// Whether a call goes through its autograd function: for gradients, and where an input has a tangent (of forward mode, which needs neither
+// requires_grad nor grad mode), so that torch refuses it instead of getting a result without one.
+bool differentiated(const Tensor& x) { return wanted(x) || x._fw_grad(0).defined(); }
 
 }  // namespace
 
@@ -492,13 +495,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return unpack(values, scales, std::move(shape), type);
   });
   m.def("swiglu8", [](const Tensor& gate, const Tensor& up) {
-    if (wanted(gate) || wanted(up)) return SwiGLU8::apply(gate, up);
+    if (differentiated(gate) || differentiated(up)) return SwiGLU8::apply(gate, up);
     const c10::cuda::CUDAGuard guard(gate.device());
     const at::NoGradGuard no_grad;
     return swiglu_forward(gate, up, false)[0];
   });
   m.def("swiglu_linear8", [](const Tensor& gate, const Tensor& up, const Tensor& weight) {
-    if (wanted(gate) || wanted(up) || wanted(weight)) return SwiGLULinear8::apply(gate, up, weight, wanted(weight));
+    if (differentiated(gate) || differentiated(up) || differentiated(weight)) return SwiGLULinear8::apply(gate, up, weight, wanted(weight));
     const c10::cuda::CUDAGuard guard(gate.device());
     const at::NoGradGuard no_grad;
     const NoAutocast own_type;
