@@ -174,12 +174,21 @@ __device__ __forceinline__ void kept_values(const Kept8& kept, const Place& p, f
   dequantise(*reinterpret_cast<const uint2*>(kept.values + p.row * kept.pitch + p.column), kept.scales[p.group], v);
 }
 
+// 1 / (1 + e^-x), down to 2^-150: where 1 + e^-x itself is the divisor, silu is 0 below -87.3 or -88.7, though 1e37 silu(-88) is -0.5.
+// fp32: t / (1 + t) or 1 / (1 + t) with t = e^-|x|, whose divisor is at most 2.
+// 16 bits: 2^-24 / (2^-24 + 2^(-x log2 e - 24)), whose divisor overflows at x = -105 and is no more work.  The exponent's rounding makes it off by 2^-20
+// near zero and by |x| 2^-23 far from it, where results are rounded to 2^-9 or 2^-12.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float x) {
   if constexpr (std::is_same<T, float>::value) {
-    return 1.f / (1.f + expf(-x));
+    const float t = expf(-fabsf(x));
+    return (x < 0.f ? t : 1.f) / (1.f + t);
   } else {
-    return __fdividef(1.f, 1.f + __expf(-x));      // off by some 2^-20 where the result is rounded to 2^-9 or 2^-12
+    constexpr float kLog2e = 1.4426950408889634f, kDown = 5.9604644775390625e-8f;      // 2^-24
+    float power, reciprocal;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(power) : "f"(fmaf(x, -kLog2e, -24.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(reciprocal) : "f"(kDown + power));
+    return reciprocal * kDown;
   }
 }
 

@@ -27,3 +27,38 @@ def test_forward_mode_is_refused(which, grad_mode):
                 ops.residual_norm(gate, up, torch.ones(64, device="cuda"))
             with pytest.raises(RuntimeError, match="jvp"):
                 ops.linear_cross_entropy(gate if which == 0 else up, weight, torch.zeros(4, dtype=torch.int64, device="cuda"))
+
+
+# ---- gates far below zero -----------------------------------------------------------------------------------------------
+def _exp_error(dtype, gate):
+    """Relative error of silu for gates of -20 and below, in 16 bits in units of 2^-23: the exponent, at most |g| log2 e, is rounded (0.5 |g|) and
+    multiplied by a rounded log2 e (0.2 |g|), the power and the reciprocal are off by two and one, products by half a unit each.  fp32: the
+    accurate functions' two units."""
+    return (8 + 1.173 * gate.abs()) * 2.0 ** -23 if dtype != FP32 else torch.full_like(gate, 16 * F32)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_swiglu8_of_gates_far_below_zero(dtype):
+    """exp(g) down to 2^-149 counts: 1e37 silu(-88) is -0.5.  Below 2^-126 it is a multiple of 2^-149, and so is its quotient."""
+    from soap_tp_b200.ops import pack8, swiglu8
+
+    gate = torch.linspace(-96.0, -20.0, 64 * 40, device="cuda").view(40, 64).to(dtype).requires_grad_()
+    large = 1e37 if dtype != FP16 else 4e4
+    up = (_rand(40, 64, seed=1).sign() * (0.5 + _rand(40, 64, seed=2).abs().clamp(max=1.0)) * large).to(dtype).requires_grad_()
+    grad = _rand(40, 64, seed=3, dtype=dtype)
+    y = swiglu8(gate, up)
+    g, v, u = gate.detach().double(), up.detach().double(), half_step(dtype)
+    exact = g * torch.sigmoid(g) * v
+    within(y, (exact, (u + _exp_error(dtype, g)) * exact.abs() + 2.0 ** -148 * (g * v).abs() + smallest(dtype)))
+
+    def kept(t):
+        packed = pack8(t.detach())
+        return packed.values.double() * packed.scales.double().repeat_interleave(64, dim=1)
+
+    got = torch.autograd.grad(y, (gate, up), grad)
+    g, v, d = kept(gate), kept(up), grad.double()
+    # (a kept value is a product rounded to fp32, off by |g| 2^-24: that much of its exponential)
+    s, c = torch.sigmoid(g), _exp_error(dtype, g) + g.abs() * F32
+    d_up, d_gate = d * g * s, d * v * s * (1 + g * (1 - s))
+    within(got[1], (d_up, (u + c) * d_up.abs() + 2.0 ** -148 * (d * g).abs() + smallest(dtype)))
+    within(got[0], (d_gate, u * d_gate.abs() + (d * v).abs() * (1 + g.abs()) * (c * s + 2.0 ** -147) + smallest(dtype)))
