@@ -2,8 +2,8 @@
 //
 //   scale = max |x| / 127 over 64 neighbouring features of a row      q = round(x / scale)      x' = q scale
 //
-// so |x - x'| is at most half a step, max |x| / 254.  A scale is not less than 2^-126, so that its reciprocal is finite; a group with
-// an infinity or a NaN in it gets a NaN as its scale and comes back as NaN: nothing that went wrong is lost.
+// so |x - x'| is at most half a step, max |x| / 254.  A scale is not less than 2^-126, so that its reciprocal is finite, nor so large that 127 of it
+// are not: fp32's largest number, rounded up as a quotient, would come back as an infinity.  A group with an infinity or a NaN in it gets a NaN as its scale and comes back as NaN: nothing that went wrong is lost.
 //
 // y = silu(g) u keeps g and u this way, and its backward pass works from them: dg = dy u' s (1 + g' (1 - s)), du = dy g' s with
 // s = sigmoid(g').
@@ -30,6 +30,7 @@ constexpr int kPerThread = 8;
 constexpr int kTurns = 2;        // runs of eight values that a thread packs or unpacks
 constexpr int kGroupThreads = kScaleGroup / kPerThread;
 constexpr float kSmallestScale = 1.17549435e-38f;      // 2^-126
+constexpr float kLargestScale = 0x1.020406p+121f;      // 127 of it round to a number just below the largest
 
 // Division of numbers below 2^31 by a number that is known before the launch: (n m) >> (32 + s) with m = ceil(2^(32 + s) / d), s =
 // ceil(log2 d) - 1 (Granlund and Montgomery, 1994; d = 1 apart).
@@ -120,7 +121,7 @@ __device__ __forceinline__ uint32_t group_most(const Eight<T>& e) {
   return most;
 }
 __device__ __forceinline__ float scale_of(uint32_t most) {
-  return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(most) / 127.f, kSmallestScale);
+  return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fminf(fmaxf(__uint_as_float(most) / 127.f, kSmallestScale), kLargestScale);
 }
 
 // 127 x / max of 16-bit values is often a tie, which a rounded reciprocal would move to either side (2e-4 of fp16 values, 1e-3 of bf16 ones).  So

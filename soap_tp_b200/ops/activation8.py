@@ -24,6 +24,7 @@ from torch.autograd.function import once_differentiable
 GROUP = 64
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 SMALLEST_SCALE = 2.0 ** -126
+LARGEST_SCALE = float.fromhex("0x1.020406p+121")      # 127 of it are a finite fp32 number
 
 
 class Packed8(NamedTuple):
@@ -60,7 +61,7 @@ def _host_pack(x: Tensor) -> Tuple[Tensor, Tensor]:
     rows, dim = x.shape
     groups = -(-dim // GROUP)
     v = F.pad(x.float(), (0, groups * GROUP - dim)).view(rows, groups, GROUP)
-    scales = (v.abs().amax(dim=2) / 127.0).clamp(min=SMALLEST_SCALE)
+    scales = (v.abs().amax(dim=2) / 127.0).clamp(min=SMALLEST_SCALE, max=LARGEST_SCALE)
     scales = torch.where(torch.isfinite(v).all(dim=2), scales, torch.full_like(scales, float("nan")))
     values = torch.nan_to_num(torch.round(v / scales.unsqueeze(2)), nan=0.0).to(torch.int8).view(rows, groups * GROUP)
     return values[:, : -(-dim // 8) * 8].contiguous(), scales

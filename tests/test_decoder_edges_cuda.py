@@ -62,3 +62,15 @@ def test_swiglu8_of_gates_far_below_zero(dtype):
     d_up, d_gate = d * g * s, d * v * s * (1 + g * (1 - s))
     within(got[1], (d_up, (u + c) * d_up.abs() + 2.0 ** -148 * (d * g).abs() + smallest(dtype)))
     within(got[0], (d_gate, u * d_gate.abs() + (d * v).abs() * (1 + g.abs()) * (c * s + 2.0 ** -147) + smallest(dtype)))
+
+
+# ---- the largest numbers ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_largest_values_stay_finite_in_eight_bits(dtype):
+    from soap_tp_b200.ops import pack8, unpack8
+
+    x = torch.zeros(2, 130, dtype=dtype, device="cuda")
+    x[0, 3], x[1, 70], x[1, 129] = torch.finfo(dtype).max, torch.finfo(dtype).min, torch.finfo(dtype).min
+    back = unpack8(pack8(x))
+    assert bool(torch.isfinite(back).all())
+    within(back, (x.double(), (half_step(dtype) + 4 * F32) * x.double().abs()))
