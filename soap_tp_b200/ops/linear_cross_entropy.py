@@ -96,8 +96,10 @@ class _HostHead:
     """The same quantities from plain tensor operations (CPU tensors)."""
 
     def __init__(self, hidden, weight, targets, ignore_index, first_word, vocabulary) -> None:
-        self.hidden, self.weight = hidden.to(_wide(hidden.dtype)), weight.to(_wide(weight.dtype))
         self.counts = targets != ignore_index
+        self.hidden, self.weight = hidden.to(_wide(hidden.dtype)), weight.to(_wide(weight.dtype))
+        # (what padding holds, NaN included, reaches nothing: zero times it would)
+        self.hidden = torch.where(self.counts.unsqueeze(1), self.hidden, torch.zeros_like(self.hidden[:1]))
         if bool((self.counts & ((targets < 0) | (targets >= vocabulary))).any()):
             raise IndexError(f"a target is neither {ignore_index} nor in [0, {vocabulary}).")
         local = targets.to(torch.int64) - first_word

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from decoder_bounds import F32, half_step, within
+from decoder_bounds import F32, IGNORED, half_step, within
 from soap_tp_b200 import ops
 
 
@@ -16,3 +16,25 @@ def test_largest_values_stay_finite_in_eight_bits(dtype):
     within(back, (x.double(), (half_step(dtype) + 4 * F32) * x.double().abs()))
     x[0, 5] = float("inf")
     assert bool(ops.unpack8(ops.pack8(x))[0, :64].isnan().all())
+
+
+# ---- padding ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("held", [float("nan"), float("inf"), -1e30])
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_leaves_padding_out(reduction, dtype, held):
+    generator = torch.Generator().manual_seed(3)
+    hidden, weight = torch.randn(7, 12, generator=generator).to(dtype), torch.randn(20, 12, generator=generator).to(dtype).requires_grad_()
+    targets = torch.randint(0, 20, (7,), generator=generator)
+    targets[2], targets[6] = IGNORED, IGNORED
+    up = torch.rand(7 if reduction == "none" else (), generator=generator, dtype=torch.float64 if dtype == torch.float64 else torch.float32)
+
+    def results(hidden):
+        loss = ops.linear_cross_entropy(hidden, weight, targets, reduction=reduction)
+        return (loss, *torch.autograd.grad(loss, (hidden, weight), up))
+
+    expected = results(hidden.clone().requires_grad_())
+    hidden[targets == IGNORED] = held
+    for a, b in zip(results(hidden.requires_grad_()), expected):
+        assert torch.equal(a, b)
+    assert not expected[1][targets == IGNORED].any()
