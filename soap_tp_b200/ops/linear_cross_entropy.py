@@ -18,7 +18,6 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
-import torch.nn.functional as F
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
@@ -72,8 +71,8 @@ def _finish(rest: Tensor, picked: Tensor):
     """Log-sum-exp and loss from the log-sum-exp of all words but the target and the target's logit.  (Not their difference: of the loss of
     a token that the model knows nothing would be left.)"""
     over = rest - picked
-    loss = F.softplus(over)
-    return torch.where(over > 0, rest + F.softplus(-over), picked + loss), loss
+    by = torch.log1p(torch.exp(-over.abs()))
+    return torch.where(over > 0, rest + by, picked + by), torch.where(over > 0, over + by, by)
 
 
 def _join(group, lse: Tensor, loss: Tensor) -> None:

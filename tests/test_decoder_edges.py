@@ -1,4 +1,6 @@
 """Operators of a decoder's training step on CPU tensors, at the edges of what they accept: see also ``test_decoder_ops.py``."""
+import math
+
 import pytest
 import torch
 
@@ -38,3 +40,26 @@ def test_cross_entropy_leaves_padding_out(reduction, dtype, held):
     for a, b in zip(results(hidden.requires_grad_()), expected):
         assert torch.equal(a, b)
     assert not expected[1][targets == IGNORED].any()
+
+
+# ---- losses of any size -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("loss", [1e-30, 1e-12, 0.5, 5.0, 19.0, 20.5, 21.0, 25.0, 40.0, 300.0])
+def test_cross_entropy_of_64_bits_has_64_bits(loss):
+    # 64 words of equal logits, 0, and the target's: log(1 + 64 exp(-t)) = loss
+    t = math.log(64) - math.log(math.expm1(loss))
+    hidden = torch.tensor([[t]], dtype=torch.float64, requires_grad=True)
+    weight = torch.zeros(65, 1, dtype=torch.float64)
+    weight[7] = 1.0
+    got = ops.linear_cross_entropy(hidden, weight, torch.tensor([7]))
+    # log 64, t and their difference are rounded to 2^-53 of at most 300 + 2 log 64, and the loss to 2^-53 of itself
+    exact = math.log1p(64 * math.exp(-t))
+    assert abs(float(got.detach()) - exact) <= 8 * 2.0 ** -53 * max(1.0, abs(t)) * exact
+    # the gradient is p - 1 = expm1(-loss), from exp(l - lse) - 1: off by the rounding of lse and of one
+    assert abs(float(torch.autograd.grad(got, hidden)[0]) - math.expm1(-exact)) <= 8 * 2.0 ** -53 * max(1.0, abs(t))
+
+
+def test_cross_entropy_of_words_that_cannot_be():
+    weight = torch.zeros(4, 1, dtype=torch.float64)
+    weight[0], weight[1:] = 1.0, float("-inf")
+    assert float(ops.linear_cross_entropy(torch.ones(1, 1, dtype=torch.float64), weight, torch.tensor([0]))) == 0.0
+    assert float(ops.linear_cross_entropy(torch.ones(1, 1, dtype=torch.float64), weight, torch.tensor([2]))) == float("inf")
