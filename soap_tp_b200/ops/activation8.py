@@ -110,7 +110,13 @@ class _Checkpoint8(torch.autograd.Function):
         ctx.plain = [None if t else a for a, t in zip(rest, ctx.tensors)]
         ctx.save_for_backward(packed.values, packed.scales, *(a for a, t in zip(rest, ctx.tensors) if t))
         with torch.no_grad():
-            return function(x, *rest[:count])
+            outputs = function(x, *rest[:count])
+        if not isinstance(outputs, (Tensor, tuple, list)):
+            raise TypeError(f"checkpoint8: the function must return a tensor or a tuple of tensors, got {type(outputs).__name__}.")
+        # what it returns without having made it (a parameter, a buffer) must not become an output of this node itself
+        given = {id(a) for a in (x, *rest)}
+        own = [o.detach() if isinstance(o, Tensor) and id(o) not in given else o for o in ([outputs] if isinstance(outputs, Tensor) else outputs)]
+        return own[0] if isinstance(outputs, Tensor) else tuple(own)
 
     @staticmethod
     @once_differentiable

@@ -63,3 +63,44 @@ def test_cross_entropy_of_words_that_cannot_be():
     weight[0], weight[1:] = 1.0, float("-inf")
     assert float(ops.linear_cross_entropy(torch.ones(1, 1, dtype=torch.float64), weight, torch.tensor([0]))) == 0.0
     assert float(ops.linear_cross_entropy(torch.ones(1, 1, dtype=torch.float64), weight, torch.tensor([2]))) == float("inf")
+
+
+# ---- what a checkpointed function returns -------------------------------------------------------------------------------
+def test_checkpoint8_leaves_tensors_alone_that_the_function_returns():
+    module, x = torch.nn.Linear(70, 9), torch.randn(4, 70, requires_grad=True)
+    constant = torch.randn(9)
+    module.register_buffer("buffer", constant)
+
+    class Returns(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.inner = module
+
+        def forward(self, t):
+            return self.inner(t), self.inner.weight, self.inner.buffer, t
+
+    y, weight, buffer, same = ops.checkpoint8(Returns(), x)
+    assert module.weight.is_leaf and module.weight.grad_fn is None and not constant.requires_grad and x.is_leaf
+    assert torch.equal(weight, module.weight) and torch.equal(buffer, constant) and torch.equal(same, x)
+    (y.sum() + 2 * weight.sum() + 3 * same.sum()).backward()
+    kept = ops.unpack8(ops.pack8(x))
+    assert torch.allclose(module.weight.grad, kept.sum(0).expand(9, 70) + 2, rtol=1e-6)
+    assert torch.allclose(x.grad, module.weight.detach().sum(0).expand(4, 70) + 3, rtol=1e-6)
+
+
+def test_checkpoint8_of_lists_and_refusals_of_other_containers():
+    module, x = torch.nn.Linear(70, 9), torch.randn(4, 70, requires_grad=True)
+
+    class Returns(torch.nn.Module):
+        def __init__(self, container):
+            super().__init__()
+            self.inner, self.container = module, container
+
+        def forward(self, t):
+            return self.container(self.inner(t))
+
+    a, b = ops.checkpoint8(Returns(lambda y: [y, 2 * y]), x)
+    (a + b).sum().backward()
+    assert torch.allclose(x.grad, 3 * module.weight.detach().sum(0).expand(4, 70), rtol=1e-6, atol=1e-6)
+    with pytest.raises(TypeError, match="tuple"):
+        ops.checkpoint8(Returns(lambda y: {"y": y}), x)
