@@ -97,10 +97,36 @@ def unpack8(packed: Packed8) -> Tensor:
     return _host_unpack(values, scales, dim, dtype).view(shape)
 
 
+def _parameters_of(function: Callable) -> Iterable[Tensor]:
+    """Those of a module, or of the module whose method it is."""
+    while isinstance(function, functools.partial):
+        function = function.func
+    owner = function if isinstance(function, torch.nn.Module) else getattr(function, "__self__", None)
+    return owner.parameters() if isinstance(owner, torch.nn.Module) else ()
+
+
+def _reaches_others(outputs: Iterable[Tensor], known: Iterable[Tensor]) -> bool:
+    """Whether the graph behind ``outputs`` ends at a leaf that is not among ``known``."""
+    known = {id(t) for t in known if isinstance(t, Tensor)}
+    outputs = [o for o in outputs if isinstance(o, Tensor) and o.requires_grad]
+    if any(o.grad_fn is None and id(o) not in known for o in outputs):
+        return True
+    nodes, seen = [o.grad_fn for o in outputs], set()
+    while nodes:
+        node = nodes.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        if node.name() == "torch::autograd::AccumulateGrad" and id(node.variable) not in known:
+            return True
+        nodes.extend(following for following, _ in node.next_functions)
+    return False
+
+
 class _Checkpoint8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, function, count, x, *rest):
-        ctx.function, ctx.count = function, count
+    def forward(ctx, function, count, complete, x, *rest):
+        ctx.function, ctx.count, ctx.complete = function, count, complete
         kind = x.device.type
         ctx.autocast = dict(device_type=kind, dtype=torch.get_autocast_dtype(kind), enabled=torch.is_autocast_enabled(kind),
                             cache_enabled=torch.is_autocast_cache_enabled())
@@ -122,20 +148,24 @@ class _Checkpoint8(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *grads):
         values, scales, *saved = ctx.saved_tensors
-        x = unpack8(Packed8(values, scales, ctx.shape, ctx.dtype)).requires_grad_(ctx.needs_input_grad[2])
+        x = unpack8(Packed8(values, scales, ctx.shape, ctx.dtype)).requires_grad_(ctx.needs_input_grad[3])
         saved = iter(saved)
         rest = [next(saved) if t else a for a, t in zip(ctx.plain, ctx.tensors)]
         # arguments become leaves of the second run; parameters are leaves that the function holds itself
         arguments = [a.detach().requires_grad_(n) if isinstance(a, Tensor) else a
-                     for a, n in zip(rest[: ctx.count], ctx.needs_input_grad[3:])]
-        wanted = [a for a, n in zip([x, *arguments, *rest[ctx.count:]], ctx.needs_input_grad[2:]) if n]
+                     for a, n in zip(rest[: ctx.count], ctx.needs_input_grad[4:])]
+        wanted = [a for a, n in zip([x, *arguments, *rest[ctx.count:]], ctx.needs_input_grad[3:]) if n]
         with torch.enable_grad(), torch.autocast(**ctx.autocast):
             outputs = ctx.function(x, *arguments)
         outputs = (outputs,) if isinstance(outputs, Tensor) else tuple(outputs)
+        if ctx.complete and _reaches_others(outputs, [x, *arguments, *rest[ctx.count:]]):
+            raise RuntimeError("checkpoint8: the function uses a tensor that requires gradients and is neither x, nor an argument, nor a parameter of the "
+                               "module that the function is or belongs to; it would get none.  Hand it over as an argument, or say in "
+                               "`parameters` which tensors get gradients.")
         pairs = [(o, g) for o, g in zip(outputs, grads) if isinstance(o, Tensor) and o.requires_grad and g is not None]
         found = iter(torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs], allow_unused=True) if pairs and wanted
                      else [None] * len(wanted))
-        return (None, None, *(next(found) if n else None for n in ctx.needs_input_grad[2:]))
+        return (None, None, None, *(next(found) if n else None for n in ctx.needs_input_grad[3:]))
 
 
 def checkpoint8(function: Callable, x: Tensor, *args, parameters: Iterable[Tensor] = None):
@@ -143,16 +173,17 @@ def checkpoint8(function: Callable, x: Tensor, *args, parameters: Iterable[Tenso
     the backward pass.
 
     ``function`` takes tensors or anything else, returns a tensor or a tuple of tensors, and does the same on every call (it must not
-    draw random numbers); autocast is as it was in the first run.  Gradients reach ``x``, tensor ``args`` and ``parameters``: by default those of ``function`` where it is a module.
-    Without gradients it is a plain call.
+    draw random numbers); autocast is as it was in the first run.  Gradients reach ``x``, tensor ``args`` and ``parameters``: by default those of
+    the module that ``function`` is, or that it is a method of, and then the backward pass is an error where the function uses any other tensor that requires
+    gradients (of a closure, or inside another argument); ``parameters`` that are given are all that get gradients.  Without gradients of
+    these it is a plain call.
     """
     _check_values("x", x)
-    if parameters is None:
-        parameters = function.parameters() if isinstance(function, torch.nn.Module) else ()
-    parameters = [p for p in parameters if p.requires_grad]
+    complete = parameters is None
+    parameters = [p for p in (_parameters_of(function) if complete else parameters) if p.requires_grad]
     if not torch.is_grad_enabled() or not any(isinstance(a, Tensor) and a.requires_grad for a in (x, *args, *parameters)):
         return function(x, *args)
-    return _Checkpoint8.apply(function, len(args), x, *args, *parameters)
+    return _Checkpoint8.apply(function, len(args), complete, x, *args, *parameters)
 
 
 def _check_swiglu(gate: Tensor, up: Tensor) -> None:

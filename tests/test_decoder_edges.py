@@ -1,4 +1,5 @@
 """Operators of a decoder's training step on CPU tensors, at the edges of what they accept: see also ``test_decoder_ops.py``."""
+import functools
 import math
 
 import pytest
@@ -104,3 +105,56 @@ def test_checkpoint8_of_lists_and_refusals_of_other_containers():
     assert torch.allclose(x.grad, 3 * module.weight.detach().sum(0).expand(4, 70), rtol=1e-6, atol=1e-6)
     with pytest.raises(TypeError, match="tuple"):
         ops.checkpoint8(Returns(lambda y: {"y": y}), x)
+
+
+# ---- what a checkpointed function uses ----------------------------------------------------------------------------------
+class _Scaled(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.layer = torch.nn.Linear(70, 9)
+
+    def forward(self, x, factor=1.0):
+        return self.layer(x).tanh() * factor
+
+    def other(self, x, factor=1.0):
+        return self.layer(x).sigmoid() * factor
+
+
+@pytest.mark.parametrize("form", ["forward", "other", "partial"])
+def test_checkpoint8_of_a_method_reaches_its_modules_parameters(form):
+    torch.manual_seed(1)
+    module, x = _Scaled(), torch.randn(4, 70, requires_grad=True)
+    function = {"forward": module.forward, "other": module.other, "partial": functools.partial(module, factor=3.0)}[form]
+    kept = ops.unpack8(ops.pack8(x)).requires_grad_()
+    direction = torch.randn(4, 9)
+    wanted = torch.autograd.grad(function(kept), (kept, *module.parameters()), direction)
+    got = torch.autograd.grad(ops.checkpoint8(function, x), (x, *module.parameters()), direction)
+    for a, b in zip(got, wanted):
+        assert torch.equal(a, b)
+    # x without gradients, as a first block's input: kept in 8 bits for the parameters all the same
+    for a, b in zip(torch.autograd.grad(ops.checkpoint8(function, x.detach()), tuple(module.parameters()), direction), wanted[1:]):
+        assert torch.equal(a, b)
+
+
+def test_checkpoint8_refuses_to_lose_gradients():
+    torch.manual_seed(2)
+    module, x, shift = _Scaled(), torch.randn(4, 70, requires_grad=True), torch.randn(9, requires_grad=True)
+    made = shift * 2
+    for function, args in ((lambda t: module(t), ()), (lambda t: t + x, ()), (lambda t: module.layer.weight, ()), (lambda t: module(t) + made, ()),
+                           (lambda t, pair: t[:, :9] * pair[0], ((shift,),)), (lambda t: (t, shift), ())):
+        y = ops.checkpoint8(function, x, *args)
+        with pytest.raises(RuntimeError, match="checkpoint8"):
+            (y if isinstance(y, torch.Tensor) else y[0]).sum().backward()
+    assert x.grad is None and shift.grad is None and module.layer.weight.grad is None
+    # said in so many words, in `parameters`, or with nothing to lose
+    ops.checkpoint8(lambda t: module(t), x, parameters=module.parameters()).sum().backward()
+    assert module.layer.weight.grad is not None and x.grad is not None
+    module.zero_grad()
+    ops.checkpoint8(lambda t: module(t), x, parameters=()).sum().backward()
+    assert module.layer.weight.grad is None
+    ops.checkpoint8(lambda t, s: t[:, :9] * s, x, shift).sum().backward()
+    assert shift.grad is not None
+    module.requires_grad_(False)
+    ops.checkpoint8(lambda t: module(t), x).sum().backward()
+    ops.checkpoint8(module.requires_grad_(True), x).sum().backward()
+    assert module.layer.weight.grad is not None
