@@ -134,6 +134,7 @@ class _Checkpoint8(torch.autograd.Function):
         packed = pack8(x)
         ctx.tensors = [isinstance(a, Tensor) for a in rest]
         ctx.plain = [None if t else a for a, t in zip(rest, ctx.tensors)]
+        ctx.parameters = rest[count:]      # (themselves: hooks on saved tensors may bring back others; saved too, so that a change of theirs is noticed)
         ctx.save_for_backward(packed.values, packed.scales, *(a for a, t in zip(rest, ctx.tensors) if t))
         with torch.no_grad():
             outputs = function(x, *rest[:count])
@@ -151,14 +152,14 @@ class _Checkpoint8(torch.autograd.Function):
         x = unpack8(Packed8(values, scales, ctx.shape, ctx.dtype)).requires_grad_(ctx.needs_input_grad[3])
         saved = iter(saved)
         rest = [next(saved) if t else a for a, t in zip(ctx.plain, ctx.tensors)]
-        # arguments become leaves of the second run; parameters are leaves that the function holds itself
+        # arguments become leaves of the second run; parameters are what the function holds itself
         arguments = [a.detach().requires_grad_(n) if isinstance(a, Tensor) else a
                      for a, n in zip(rest[: ctx.count], ctx.needs_input_grad[4:])]
-        wanted = [a for a, n in zip([x, *arguments, *rest[ctx.count:]], ctx.needs_input_grad[3:]) if n]
+        wanted = [a for a, n in zip([x, *arguments, *ctx.parameters], ctx.needs_input_grad[3:]) if n]
         with torch.enable_grad(), torch.autocast(**ctx.autocast):
             outputs = ctx.function(x, *arguments)
         outputs = (outputs,) if isinstance(outputs, Tensor) else tuple(outputs)
-        if ctx.complete and _reaches_others(outputs, [x, *arguments, *rest[ctx.count:]]):
+        if ctx.complete and _reaches_others(outputs, [x, *arguments, *ctx.parameters]):
             raise RuntimeError("checkpoint8: the function uses a tensor that requires gradients and is neither x, nor an argument, nor a parameter of the "
                                "module that the function is or belongs to; it would get none.  Hand it over as an argument, or say in "
                                "`parameters` which tensors get gradients.")

@@ -158,3 +158,20 @@ def test_checkpoint8_refuses_to_lose_gradients():
     ops.checkpoint8(lambda t: module(t), x).sum().backward()
     ops.checkpoint8(module.requires_grad_(True), x).sum().backward()
     assert module.layer.weight.grad is not None
+
+
+@pytest.mark.parametrize("hooks", [lambda: torch.autograd.graph.saved_tensors_hooks(torch.clone, lambda t: t), torch.autograd.graph.save_on_cpu])
+def test_checkpoint8_under_hooks_on_saved_tensors(hooks):
+    torch.manual_seed(3)
+    module, x, direction = _Scaled(), torch.randn(4, 70, requires_grad=True), torch.randn(4, 9)
+    wanted = torch.autograd.grad(ops.checkpoint8(module, x), (x, *module.parameters()), direction)
+    for function, options in ((module, {}), (lambda t: module(t), dict(parameters=module.parameters()))):
+        with hooks():
+            y = ops.checkpoint8(function, x, **options)
+        for a, b in zip(torch.autograd.grad(y, (x, *module.parameters()), direction, allow_unused=True), wanted):
+            assert a is not None and torch.equal(a, b)
+    y = ops.checkpoint8(module, x)
+    with torch.no_grad():
+        module.layer.weight.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
