@@ -206,20 +206,20 @@ def _host_swiglu_gradients(grad: Tensor, kept) -> Tuple[Tensor, Tensor, Tensor]:
 
 
 class _SwiGLU8(torch.autograd.Function):
-    """CPU tensors: with a weight, the linear layer behind it too."""
+    """CPU tensors, and empty ones anywhere: with a weight, the linear layer behind it too."""
 
     @staticmethod
     def forward(ctx, gate, up, weight):
         ctx.save_for_backward(weight, *_host_pack(gate), *_host_pack(up))
         y = _host_swiglu(gate, up)
-        with torch.autocast("cpu", enabled=False):
+        with torch.autocast(gate.device.type, enabled=False):
             return y if weight is None else F.linear(y, weight)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         weight, *kept = ctx.saved_tensors
-        with torch.autocast("cpu", enabled=False):
+        with torch.autocast(grad.device.type, enabled=False):
             d_gate, d_up, y = _host_swiglu_gradients(grad if weight is None else grad @ weight, kept)
             return d_gate, d_up, grad.t() @ y if ctx.needs_input_grad[2] else None
 

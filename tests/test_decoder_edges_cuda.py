@@ -74,3 +74,14 @@ def test_largest_values_stay_finite_in_eight_bits(dtype):
     back = unpack8(pack8(x))
     assert bool(torch.isfinite(back).all())
     within(back, (x.double(), (half_step(dtype) + 4 * F32) * x.double().abs()))
+
+
+# ---- nothing to do ------------------------------------------------------------------------------------------------------
+def test_empty_swiglu_linear8_keeps_its_type_under_autocast():
+    from soap_tp_b200.ops import swiglu_linear8
+
+    gate, weight = torch.zeros(0, 64, dtype=BF16, device="cuda", requires_grad=True), _rand(5, 64, dtype=BF16).requires_grad_()
+    with torch.autocast("cuda", dtype=FP16):
+        y = swiglu_linear8(gate, gate, weight)
+        grads = torch.autograd.grad(y.sum(), (gate, weight))
+    assert y.dtype == BF16 and y.shape == (0, 5) and all(g.dtype == BF16 for g in grads) and not grads[1].any()
