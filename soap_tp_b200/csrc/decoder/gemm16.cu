@@ -16,7 +16,7 @@
 // producer that suspend it (541 -> 583 thousand; those of the epilogue, which are long, do).
 //
 // The tensor core truncates as it adds: some 2^-24 of the running sum per 16 of K.  Logits are drained from TMEM into sums in registers (round
-// to nearest) every 2048 of K (`drain`; every 256 for a few tokens), gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
+// to nearest) every 2048 of K (`drain`; every 256 where few tokens count), gradients once: 5e-4 of one over 128256 words at most, a quarter of what its rounding to bf16 costs.
 // Draining every 256 of K costs 150 of 690 thousand cycles at 4096 x 16032 x 4096: handing the accumulator over takes the tensor core about
 // 700 cycles, whatever the epilogue does meanwhile.
 #include <cuda.h>
@@ -368,11 +368,13 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
   let_successor_start();
 
   int M = prob.M, K = prob.K;
+  int drain = prob.drain / kBK;                // in k-blocks
   const CUtensorMap *source_a = &map_a, *source_b = &map_b;
   if (prob.count) {
     const int count = *prob.count;
     int& tokens = A_K ? M : K;
     tokens = max(0, min(tokens, count - prob.first));
+    if (count <= prob.few) drain = prob.drain_few / kBK;
     if (count == all_tokens) (kLogits ? source_a : source_b) = &map_all;
   }
   const Tiles tiles(M, prob.N);
@@ -441,7 +443,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
           }
           tc_fence_after_sync();
           const uint32_t acc = tmem_base + static_cast<uint32_t>(buf * kTile);
-          const int blocks = drain_blocks<kLogits>(end - kb, prob.drain / kBK);
+          const int blocks = drain_blocks<kLogits>(end - kb, drain);
           for (int i = 0; i < blocks; ++i, ++kb) {
             if (!loaded && !mbar_wait_bounded(&full_bar[s], parity, abort_flag, status, kStatusTmaWaitTimeout)) {
               ok = false;
@@ -502,7 +504,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int j = 0; j < kLogitPart / 2; ++j) sums[j] = 0;
         bool ok = true;
         for (int kb = 0; kb < k_blocks;) {
-          kb += drain_blocks<true>(k_blocks - kb, prob.drain / kBK);
+          kb += drain_blocks<true>(k_blocks - kb, drain);
           ok = filled();
           if (!ok) break;
           const uint32_t from = taddr + static_cast<uint32_t>((it & 1) * kTile);
@@ -625,7 +627,9 @@ void gemm16(Gemm16Epilogue epilogue, bool bf16, const Matrix16& a, const Matrix1
     throw std::invalid_argument("gemm16: operand pitches are multiples of 8 elements");
   if ((epilogue == kLogitGradient || epilogue == kLogitExponential) && (p.ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(p.C) & 15) != 0))
     throw std::invalid_argument("gemm16: the logits' gradient needs 16-byte rows");
-  if (epilogue != kStore16 && (p.drain < kBK || p.drain % kBK != 0)) throw std::invalid_argument("gemm16: logits are drained every multiple of 64 of K");
+  auto drains = [](int every) { return every >= kBK && every % kBK == 0; };
+  if (epilogue != kStore16 && (!drains(p.drain) || (p.few > 0 && !drains(p.drain_few))))
+    throw std::invalid_argument("gemm16: logits are drained every multiple of 64 of K");
   if (p.second % kBK != 0 || p.second < 0 || (p.second && p.second < (epilogue == kLogitGradient ? p.N : a.k_major ? p.K : p.M)))
     throw std::invalid_argument("gemm16: the second term lies a multiple of 64 columns behind the first");
   if (epilogue == kStore16 && (p.add || !p.C) && (!p.accumulator || p.ld_accumulator % 32 != 0 || p.ld_accumulator < p.N ||

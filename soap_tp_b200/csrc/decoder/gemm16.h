@@ -33,7 +33,8 @@ struct Gemm16Problem {
   const int* targets;       // [M]: the column that is the token's target; negative where none of them is
   float2* parts;            // [ceil(N / kLogitPart)][ld_parts]: largest logit, sum of exp(logit - largest) over all but the target
   int64_t ld_parts;
-  int drain;                // of K, a multiple of 64: the accumulator is drained into fp32 sums that often
+  int drain;                // of K, a multiple of 64: the accumulator is drained into fp32 sums that often;
+  int drain_few, few;       // drain_few where there are at most `few` tokens in all (`count`)
   const float* lse;         // [M]
   const float* loss;        // [M]: lse - the target's logit
   const float* factor;      // [M]

@@ -76,6 +76,23 @@ def test_largest_values_stay_finite_in_eight_bits(dtype):
     within(back, (x.double(), (half_step(dtype) + 4 * F32) * x.double().abs()))
 
 
+# ---- padding ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("counted", [1, 64])
+def test_loss_of_a_token_does_not_depend_on_padding(dtype, counted):
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    hidden, weight, targets = _head(counted, 4200, 700, dtype)
+    padded, padded_targets = torch.cat((hidden.detach(), _rand(300, 4200, seed=7, dtype=dtype))), torch.full((counted + 300,), IGNORED, device="cuda")
+    padded_targets[:counted] = targets
+    for reduction in ("none", "mean"):
+        alone = linear_cross_entropy(hidden, weight, targets, reduction=reduction)
+        among = linear_cross_entropy(padded.requires_grad_(), weight, padded_targets, reduction=reduction)
+        assert torch.equal(alone, among[:counted] if reduction == "none" else among)
+        with torch.no_grad():
+            assert torch.equal(alone, linear_cross_entropy(hidden, weight, targets, reduction=reduction))
+
+
 # ---- nothing to do ------------------------------------------------------------------------------------------------------
 def test_empty_swiglu_linear8_keeps_its_type_under_autocast():
     from soap_tp_b200.ops import swiglu_linear8
