@@ -102,3 +102,52 @@ def test_empty_swiglu_linear8_keeps_its_type_under_autocast():
         y = swiglu_linear8(gate, gate, weight)
         grads = torch.autograd.grad(y.sum(), (gate, weight))
     assert y.dtype == BF16 and y.shape == (0, 5) and all(g.dtype == BF16 for g in grads) and not grads[1].any()
+
+
+# ---- paths that small sizes do not take ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+# logits drained twice and three times, in tiles that pairs of thread blocks take one and several of; every 256 of K for a few tokens
+@pytest.mark.parametrize("tokens,depth,words", [(300, 2112, 700), (300, 4200, 700), (300, 4200, 10000), (600, 6000, 5000), (40, 1000, 300), (64, 2100, 20000)])
+def test_cross_entropy_of_deep_hidden_states(tokens, depth, words, reduction, dtype):
+    _check_head(*_head(tokens, depth, words, dtype, ignored=0.1), reduction)
+
+
+# more rows than the blocks' rings hold at once, off 16-byte boundaries and on them
+@pytest.mark.parametrize("rows,dim,dtype", [(4000, 3001, BF16), (4000, 3000, FP16), (40000, 67, BF16), (40000, 72, FP16), (6000, 1001, FP32), (3000, 5001, BF16),
+                                            (3000, 5120, BF16)])
+@pytest.mark.parametrize("after,gated", [(False, False), (True, True)])
+def test_residual_norm_of_many_rows(rows, dim, dtype, after, gated):
+    _check_norm(rows, dim, dtype, after, gated)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_cross_entropy_by_token_in_a_graph(dtype):
+    from soap_tp_b200.ops import linear_cross_entropy
+
+    def step(hidden, weight, targets, up):
+        loss = linear_cross_entropy(hidden, weight, targets, reduction="none", workspace_bytes=1)
+        return (loss, *torch.autograd.grad(loss, (hidden, weight), up))
+
+    def inputs(seed):
+        up = torch.rand(300, generator=torch.Generator("cuda").manual_seed(seed + 9), device="cuda") - 0.3
+        return [*_head(300, 72, 400, dtype, seed=seed, ignored=0.2 + 0.0005 * seed), up]
+
+    held = inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = step(*held)
+    for seed in (100, 1000):
+        with torch.no_grad():
+            for old, new in zip(held, inputs(seed)):
+                old.copy_(new)
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outputs, step(*inputs(seed))):
+            assert torch.equal(a, b)
