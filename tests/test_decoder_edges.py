@@ -175,3 +175,33 @@ def test_checkpoint8_under_hooks_on_saved_tensors(hooks):
         module.layer.weight.add_(1.0)
     with pytest.raises(RuntimeError, match="modified"):
         y.sum().backward()
+
+
+# ---- the plain product of the native library ----------------------------------------------------------------------------
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("change,error,message", [
+    (dict(), ValueError, "of one CUDA device"),
+    (dict(out=torch.zeros(16, 24, dtype=BF16)), ValueError, "sizes do not match"),
+    (dict(out=torch.zeros(8, 32, dtype=BF16)), ValueError, "sizes do not match"),
+    (dict(b=torch.zeros(16, 32, dtype=BF16)), ValueError, "sizes do not match"),
+    (dict(turned=True), ValueError, "sizes do not match"),
+    (dict(out=torch.zeros(32, 16, dtype=BF16).t()), ValueError, "rows lie in memory"),
+    (dict(out=torch.zeros(512, dtype=BF16).as_strided((16, 32), (8, 1))), ValueError, "rows lie in memory"),
+    (dict(a=torch.zeros(24, dtype=BF16)), ValueError, "rows lie in memory"),
+    (dict(a=torch.zeros(16, 0, dtype=BF16), b=torch.zeros(0, 32, dtype=BF16)), ValueError, "rows lie in memory"),
+    (dict(out=torch.zeros(16, 32)), TypeError, "all of one type"),
+    (dict(b=torch.zeros(24, 32, dtype=FP16)), TypeError, "all of one type"),
+    (dict(a=torch.zeros(16, 24), b=torch.zeros(24, 32), out=torch.zeros(16, 32)), TypeError, "bfloat16 or float16"),
+    (dict(split_parts=torch.zeros(4)), ValueError, "go together"),
+    (dict(split_counters=torch.zeros(4, dtype=torch.int32)), ValueError, "go together"),
+    (dict(split_parts=torch.zeros(4), split_counters=torch.zeros(4, dtype=torch.int32)), ValueError, "too small"),
+    (dict(split_parts=torch.zeros(4), split_counters=torch.zeros(4)), TypeError, "split_counters int32"),
+    (dict(split_parts=torch.zeros(4, dtype=BF16), split_counters=torch.zeros(4, dtype=torch.int32)), TypeError, "split_parts are float32"),
+])
+def test_what_the_native_product_says_it_refuses(change, error, message):
+    native = pytest.importorskip("soap_tp_b200._decoder")
+    given = dict(a=torch.zeros(16, 24, dtype=BF16), b=torch.zeros(24, 32, dtype=BF16), out=torch.zeros(16, 32, dtype=BF16), turned=False, status=0)
+    with pytest.raises(error, match=message):
+        native.gemm16(**given | change)
