@@ -45,10 +45,6 @@ struct Eight {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) words[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-  __device__ __forceinline__ void load_streamed(const T* p) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) words[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-  }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = words[i];
