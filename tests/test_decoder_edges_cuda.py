@@ -89,8 +89,6 @@ def test_loss_of_a_token_does_not_depend_on_padding(dtype, counted):
         alone = linear_cross_entropy(hidden, weight, targets, reduction=reduction)
         among = linear_cross_entropy(padded.requires_grad_(), weight, padded_targets, reduction=reduction)
         assert torch.equal(alone, among[:counted] if reduction == "none" else among)
-        with torch.no_grad():
-            assert torch.equal(alone, linear_cross_entropy(hidden, weight, targets, reduction=reduction))
 
 
 # ---- nothing to do ------------------------------------------------------------------------------------------------------
