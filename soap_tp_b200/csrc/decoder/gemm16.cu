@@ -11,7 +11,7 @@
 //
 // What bounds it: a pair's tile takes 64 KB of L2's bandwidth every 512 cycles of products, 64 bytes a cycle and SM, which is all that an SM gets; and
 // the power cap in long runs.  8192 x 4096 x 128256 alone 1.31 PFLOP/s (torch.matmul 1.55), for seconds 1.21 to 1.24 (1.29 to 1.37).  At 4096 x 4096
-// x 16032 the tensor pipe is busy for 80 (exponentials), 85 and 83 % of a launch, of 97 % that its rounds of tiles allow.  Tried and not kept:
+// x 16032 the tensor pipe is busy for 79 (exponentials), 86 and 84 % of a launch, of 97 % that its rounds of tiles allow.  Tried and not kept:
 // tiles fetched into L2 ahead of their loads (416 -> 493 us), a producer thread for each operand (566 -> 574 thousand cycles), waits of the
 // producer that suspend it (541 -> 583 thousand; those of the epilogue, which are long, do).
 //

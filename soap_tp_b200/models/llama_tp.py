@@ -16,7 +16,8 @@ Every 2-D weight carries ``tp_shard_dim`` and ``tp_global_shape`` so the optimiz
 ``soap_step`` unchanged.  Works on CPU (gloo) for tests and on CUDA (NCCL) for training.
 
 What is not a plain product can run on the package's own operators instead of eager torch, each switched on by an attribute of
-``LlamaTP`` (all off, and the results then those of eager torch): ``fused_loss`` (the head's cross entropy without logits),
+``LlamaTP`` (all off, and the results then those of eager torch): ``fused_loss`` (the head's cross entropy without logits; targets of -100 are
+left out of the mean, which without it count as words that no rank has),
 ``fused_norms`` (residual sums, norms, gates in one pass), ``mlp_bits = 8`` and ``checkpoint_bits = 8`` (the MLPs' inputs of the down
 projection, and the blocks' inputs where activations are checkpointed, kept in 8 bits).
 """

@@ -234,7 +234,8 @@ def swiglu8(gate: Tensor, up: Tensor) -> Tensor:
 
 
 def swiglu_linear8(gate: Tensor, up: Tensor, weight: Tensor) -> Tensor:
-    """``(silu(gate) * up) @ weight.T``; only gate and up are kept, in 8 bits: 2 bytes and a bit of each pair of features instead of 6.
+    """``(silu(gate) * up) @ weight.T``; only gate and up are kept, in 8 bits: 2.1 bytes of each pair of features instead of the 8
+    that eager torch keeps (gate, silu(gate), up and their product).
     In the type of its arguments, under autocast too."""
     _check_swiglu(gate, up)
     if weight.ndim != 2 or weight.shape[1] != gate.shape[-1] or weight.dtype != gate.dtype or weight.device != gate.device:

@@ -206,7 +206,9 @@ def linear_cross_entropy(
     ``hidden`` (..., depth) and ``weight`` (words, depth) are bf16 or fp16 on CUDA; ``targets`` (...) counts over the whole
     vocabulary.  Tokens whose target is ``ignore_index`` have loss 0 and no gradient; ``"mean"`` is over the others, and 0 where there
     are none.  Another target outside the vocabulary is an error on CPU and makes the loss NaN on CUDA, where nobody waits for
-    the device to find out.  ``group``: see the module's text.  Up to ``workspace_bytes`` of softmax are in memory at a time
+    the device to find out.  On CUDA a token's loss is the same whatever padding surrounds it; it changes by roundings where more than 64
+    tokens count (of fewer, logits are rounded to fp32 more often), its gradients where the call has more than 256 tokens (of fewer, the logits'
+    gradient has two 16-bit terms).  ``group``: see the module's text.  Up to ``workspace_bytes`` of softmax are in memory at a time
     (256 tokens' at least) and, where the tokens need more than one turn, the weight's gradient in fp32.
     """
     _validate(hidden, weight, targets, reduction, workspace_bytes)
