@@ -105,6 +105,12 @@ def _parameters_of(function: Callable) -> Iterable[Tensor]:
     return owner.parameters() if isinstance(owner, torch.nn.Module) else ()
 
 
+def _holds_tensors(value) -> bool:
+    """Whether ``value`` is a container with a tensor somewhere in it."""
+    inside = value.values() if isinstance(value, dict) else value if isinstance(value, (tuple, list)) else ()
+    return any(isinstance(v, Tensor) or _holds_tensors(v) for v in inside)
+
+
 def _reaches_others(outputs: Iterable[Tensor], known: Iterable[Tensor]) -> bool:
     """Whether the graph behind ``outputs`` ends at a leaf that is not among ``known``."""
     known = {id(t) for t in known if isinstance(t, Tensor)}
@@ -138,8 +144,9 @@ class _Checkpoint8(torch.autograd.Function):
         ctx.save_for_backward(packed.values, packed.scales, *(a for a, t in zip(rest, ctx.tensors) if t))
         with torch.no_grad():
             outputs = function(x, *rest[:count])
-        if not isinstance(outputs, (Tensor, tuple, list)):
-            raise TypeError(f"checkpoint8: the function must return a tensor or a tuple of tensors, got {type(outputs).__name__}.")
+        if not isinstance(outputs, (Tensor, tuple, list)) or not isinstance(outputs, Tensor) and any(map(_holds_tensors, outputs)):
+            raise TypeError(f"checkpoint8: the function must return a tensor or a tuple of tensors, got {type(outputs).__name__} "
+                            "or containers in it, whose tensors would have no gradients.")
         # what it returns without having made it (a parameter, a buffer) must not become an output of this node itself
         given = {id(a) for a in (x, *rest)}
         own = [o.detach() if isinstance(o, Tensor) and id(o) not in given else o for o in ([outputs] if isinstance(outputs, Tensor) else outputs)]

@@ -107,6 +107,23 @@ def test_checkpoint8_of_lists_and_refusals_of_other_containers():
         ops.checkpoint8(Returns(lambda y: {"y": y}), x)
 
 
+def test_checkpoint8_refuses_tensors_inside_its_outputs():
+    class Returns(torch.nn.Linear):
+        def __init__(self, form):
+            super().__init__(70, 9)
+            self.form = form
+
+        def forward(self, t):
+            return self.form(super().forward(t))
+
+    x = torch.randn(4, 70, requires_grad=True)
+    for form in (lambda y: (y, (2 * y, 3 * y)), lambda y: [y, {"twice": [2 * y]}]):
+        with pytest.raises(TypeError, match="containers"):
+            ops.checkpoint8(Returns(form), x)
+    y, shape, nothing = ops.checkpoint8(Returns(lambda y: (y, y.shape, None)), x)
+    assert y.requires_grad and shape == (4, 9) and nothing is None
+
+
 # ---- what a checkpointed function uses ----------------------------------------------------------------------------------
 class _Scaled(torch.nn.Module):
     def __init__(self):
